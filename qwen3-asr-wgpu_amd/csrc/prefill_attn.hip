@@ -44,6 +44,7 @@
 #include <algorithm>
 
 #include "kernels.hpp"
+#include "mfma_attn.hpp"
 
 namespace qasr {
 
@@ -61,38 +62,15 @@ constexpr int kTileKeys = kPrefillTileKeys;         // keys per LDS tile
 constexpr int kGroupKeys = kTileKeys / kPrefillKeyGroups;  // keys per key group
 static_assert(kGroupKeys == 64, "a key group's half tile is one 64-key wave step");
 constexpr int kTileHalves = kTileKeys * kHeadDim;  // one 32 KB K or V tile
-constexpr float kNegInf = -__builtin_inff();
-constexpr float kRescaleSlack = 8.0f;  // log2 of the largest p before the max moves
-
-typedef short short4v __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) void lds_void;
-typedef __attribute__((address_space(3))) short4v lds_short4v;
-
-__device__ __forceinline__ float16v mfma32(const half8v& a, const half8v& b, const float16v& c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-}
-
-// Lanes l and l^32 hold the two key halves of one query column.  One
-// v_permlane32_swap gives every lane both values (no LDS round trip).
-__device__ __forceinline__ float halves_max(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float halves_sum(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
 
 // ---- LDS tile layouts ----------------------------------------------------
 // LDS serves 16 lanes of a 16-byte read (or 32 lanes of an 8-byte read) per
 // cycle from 64 banks, so each such lane group must cover 256 distinct bytes
 // modulo 256.
 //
-// K tile: row r (key) is 256 contiguous bytes; its 16-byte chunk c (dims
-// 8c..8c+7) sits at slot c ^ swz16(r).  swz16 permutes 0..15 over every 16
-// consecutive rows, so the K operand read (16 consecutive rows, one chunk)
-// hits 16 different slots.
-__device__ __forceinline__ int swz16(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
+// K tile: rows of 256 bytes, their 16-byte chunks permuted by swz16
+// (mfma_attn.hpp).
+//
 // V tile: four slabs of 32 dims, [dims/32][row][32 dims], 8 KB each.  The
 // transposing read of 4 consecutive rows x 32 dims is then 256 contiguous
 // bytes, and every operand address is a per-lane base plus a constant.
@@ -178,117 +156,6 @@ __device__ __forceinline__ void dma_q(u32x4v qr, int row0, int last_row, int ldq
         const int c = (lane & 31) ^ (r & 15);
         dma16(qr, min(row0 + r, last_row) * ldq_bytes + c * 16, lds_addr(qdst + (NW * j + wave) * 512));
     }
-}
-
-// 4 halves of V^T: ds_read_b64_tr_b16 transposes 16-bit elements within each
-// 16-lane group (result lane 4m+e, element k <- source lane 4k+m, element e).
-__device__ __forceinline__ half4v read_tr(const f16* p) {
-    return __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v*)p));
-}
-
-// Per-wave state.
-struct Wave {
-    half8v qb[8];     // Q^T B operand, k-step ks: dims 16*ks + 8*g .. +8 of query n
-    float16v o[4];    // O^T: o[db][i] = dim db*32 + 8*(i/4) + 4*g + i%4 of query n
-    float m;          // running max the exponents are taken against
-    float l;          // running row sum
-    int kaddr[8];     // K operand of k-step ks, rows 0..31 of the half tile (halves)
-    int vbase;        // V^T operand source address, slab 0, key 0 (halves)
-    int g, qpos;
-    float scale_log2;
-};
-
-// First half of a step over NB * 32 keys: S^T from K rows kt[0..32 NB - 1]
-// (first key k0), row max, the running-max update, P^T (f16, B-operand
-// layout) and its row sum.  MASK: some key is past some row's position.
-template <bool MASK, int NB>
-__device__ __forceinline__ void step_s(Wave& w, const f16* kt, int k0, half8v (&pb)[2 * NB]) {
-    // S^T: keys kb*32 + (8*(i/4) + 4*g + i%4) x query n, accumulated over dims.
-    float16v s[NB];
-#pragma unroll
-    for (int kb = 0; kb < NB; ++kb) s[kb] = (float16v){};
-#pragma unroll
-    for (int ks = 0; ks < 8; ++ks)
-#pragma unroll
-        for (int kb = 0; kb < NB; ++kb) {
-            const half8v ka = *(const half8v*)&kt[kb * 32 * kHeadDim + w.kaddr[ks]];
-            s[kb] = mfma32(ka, w.qb[ks], s[kb]);
-        }
-    // Operand reads run at most two k-steps ahead of the MFMAs (bounded
-    // register lifetime; 8 NB reads + 8 NB MFMAs).
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * NB, 0);
-#pragma unroll
-    for (int i = 0; i < 6; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, NB, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, NB, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, 2 * NB, 0);
-    float mx = kNegInf;
-#pragma unroll
-    for (int kb = 0; kb < NB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if (MASK) {
-                const int key = k0 + kb * 32 + 8 * (i >> 2) + 4 * w.g + (i & 3);
-                s[kb][i] = key > w.qpos ? kNegInf : s[kb][i];
-            }
-            mx = fmaxf(mx, s[kb][i]);
-        }
-    mx = halves_max(mx) * w.scale_log2;
-    // Move the running max when a row max passed it by more than the slack.
-    {
-        const bool up = mx > w.m + kRescaleSlack;
-        if (__ballot(up)) {
-            const float mn = up ? mx : w.m;
-            const float alpha = w.m == kNegInf ? 0.0f : fast_exp2(w.m - mn);
-#pragma unroll
-            for (int db = 0; db < 4; ++db) w.o[db] *= alpha;
-            w.l *= alpha;
-            w.m = mn;
-        }
-    }
-    const float mu = w.m == kNegInf ? 0.0f : w.m;
-    // P^T = 2^(s*scale_log2 - m), k-step w4 covering keys 16*w4 + 4*g +
-    // {0..3, 8..11}; the row sum from the same f16 values (v_dot2, f32 sum).
-#pragma unroll
-    for (int w4 = 0; w4 < 2 * NB; ++w4)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            pb[w4][j] = (f16)softmax_w_raw(s[w4 >> 1][8 * (w4 & 1) + j], w.scale_log2, mu);
-    const half2v ones2 = {(f16)1.0f, (f16)1.0f};
-    float ps = 0.0f;
-#pragma unroll
-    for (int w4 = 0; w4 < 2 * NB; ++w4)
-#pragma unroll
-        for (int q2 = 0; q2 < 4; ++q2) {
-            const half2v pr = {pb[w4][2 * q2], pb[w4][2 * q2 + 1]};
-            ps = __builtin_amdgcn_fdot2(pr, ones2, ps, false);
-        }
-    w.l += halves_sum(ps);
-}
-
-// Second half: O^T += V^T P^T with V rows vt[0..32 NB - 1] (slab stride
-// kTileKeys*32 halves).
-template <int NB>
-__device__ __forceinline__ void step_pv(Wave& w, const f16* vt, const half8v (&pb)[2 * NB]) {
-#pragma unroll
-    for (int w4 = 0; w4 < 2 * NB; ++w4)
-#pragma unroll
-        for (int db = 0; db < 4; ++db) {
-            const f16* vp = vt + w.vbase + db * (kTileKeys * 32) + w4 * 16 * 32;
-            const half4v lo = read_tr(vp);
-            const half4v hi = read_tr(vp + 8 * 32);
-            const half8v va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            w.o[db] = mfma32(va, pb[w4], w.o[db]);
-        }
-    // Two transposing reads per MFMA, at most two MFMAs ahead.
-    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
-#pragma unroll
-    for (int i = 0; i < 8 * NB - 2; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-    }
-    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
 }
 
 // Merge of the nsp split-K partials of one wave's 32 rows (lane = query row),
@@ -778,7 +645,7 @@ __global__ __launch_bounds__(NW * 64, 1) void prefill_attn_kernel(
                 step_s<false, NB>(w, kh, k0, pb);
             else
                 step_s<true, NB>(w, kh, k0, pb);
-            step_pv<NB>(w, vh, pb);
+            step_pv<kTileKeys, NB>(w, vh, pb);
         }
         if constexpr (SLICE) {
             if (t + 2 < t_end) {
