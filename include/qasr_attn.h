@@ -194,6 +194,118 @@ int qasr_prefill_layer(qasr_ctx* ctx, qasr_kv* kv, int layer, int slot, int kv_s
                        const void* qkv_dev, const void* q_gain_dev, const void* k_gain_dev,
                        void* q_work_dev, void* out_dev, void* stream);
 
+/* ---- Paged KV cache -------------------------------------------------------
+ * One pool of pages for all sequences, instead of one block per slot: a
+ * sequence holds ceil(length / page_rows) pages, listed by its row of a block
+ * table, wherever they lie.  Lengths, tables and the free pages are DEVICE
+ * arrays, and a step is planned on the GPU (qasr_paged_plan_build), so nothing
+ * waits for the host and a captured graph of [plan, layers] that updates the
+ * lengths in place can be replayed token after token.  The reference's caches
+ * are one buffer per slot (decoder.rs:1270-1271, 2453-2457): these entry points
+ * have no counterpart in it; their arithmetic is that of the stages above.
+ *
+ * A step: qasr_paged_plan_build once, then per layer qasr_paged_append (stage
+ * (a)) and qasr_paged_attn (stages (b) and (c): single rows, chunks and any
+ * mix of them).  No call allocates or synchronises after the two creates, and
+ * every call may be captured.  A context outlives its pools, a pool its plans.
+ * Calls that share a plan must be ordered on one
+ * stream (they share its arrays and split workspace); so must calls that
+ * write pages of a pool and those that read them. */
+typedef struct qasr_pages qasr_pages;
+typedef struct qasr_paged_plan qasr_paged_plan;
+
+#define QASR_PAGED_MAX_REQUESTS 1024
+#define QASR_PAGED_MAX_ROWS 65536
+
+/* Element (layer, page, kv, head, row, d), kv 0 = K and 1 = V, f16 at base +
+ * layer*layer_stride + page*page_stride + kv*kv_stride + head*head_stride +
+ * row*head_dim + d. */
+typedef struct qasr_pages_info {
+    void* base_dev;
+    int32_t pages;
+    int32_t page_rows;
+    int32_t layers;
+    int32_t nkvh;
+    int32_t head_dim;
+    int64_t layer_stride; /* elements, = pages * page_stride */
+    int64_t page_stride;  /* = 2 * kv_stride */
+    int64_t kv_stride;    /* = nkvh * head_stride */
+    int64_t head_stride;  /* = page_rows * head_dim */
+    size_t bytes;
+} qasr_pages_info;
+
+/* A pool of `pages` pages of page_rows rows (16, 32, 64, 128 or 256) for
+ * every layer, zeroed.  pages * page_rows < 2^31. */
+int qasr_pages_create(qasr_ctx* ctx, int pages, int page_rows, qasr_pages** out);
+void qasr_pages_destroy(qasr_pages* pool);
+int qasr_pages_get_info(const qasr_pages* pool, qasr_pages_info* out);
+
+/* A step's plan: device arrays of its own, written by each build. */
+typedef struct qasr_paged_plan_info {
+    int32_t max_requests;
+    int32_t max_rows;
+    int32_t* status_dev;    /* [max_requests] QASR_OK, or why a request was refused */
+    int32_t* lens_dev;      /* [max_requests] rows in the cache after the step */
+    int32_t* row_start_dev; /* [max_requests + 1] a request's first row in the step's rows */
+    int32_t* row_pos_dev;   /* [max_rows] position of each row, -1: not placed */
+    int32_t* row_slot_dev;  /* [max_rows] page * page_rows + row of the page, -1: not placed */
+    int32_t* cursor_dev;    /* [2] the ring's {head, free} after the step */
+    size_t bytes;           /* device memory of the plan */
+} qasr_paged_plan_info;
+
+/* A plan for up to max_requests (<= QASR_PAGED_MAX_REQUESTS) requests and
+ * max_rows (<= QASR_PAGED_MAX_ROWS) new rows together in a step.  Its memory
+ * is mostly the attention's split workspace: min(32 * max_rows, 2048 *
+ * max_requests) records of (128 + 2) floats per q head (67 MB for 256 rows and
+ * 16 q heads). */
+int qasr_paged_plan_create(qasr_ctx* ctx, qasr_pages* pool, int max_requests, int max_rows,
+                           qasr_paged_plan** out);
+void qasr_paged_plan_destroy(qasr_paged_plan* plan);
+int qasr_paged_plan_get_info(const qasr_paged_plan* plan, qasr_paged_plan_info* out);
+
+/* Plans a step of nreq requests: request i has len_dev[i] rows in the cache
+ * and appends rows_dev[i] (0: idle; -1: ended, its pages go back).  Its pages
+ * are table_dev[i * table_stride + j], j < ceil(len / page_rows).  New pages
+ * come from ring_dev, `pages` ids of which cursor_dev[1] are free from place
+ * cursor_dev[0] on (the ring wraps), in request order, and are entered in the
+ * table; pages of ended requests go to the ring's end and are free from the
+ * next step on.  ring_dev and cursor_dev NULL: the table holds the new rows'
+ * pages already.
+ *
+ * The step's rows are the requests' new rows one after the other.  A request
+ * is placed whole or not at all: status_dev[i] is QASR_EINVAL for a negative
+ * length, rows below -1, or a page of the new rows outside the pool;
+ * QASR_ERANGE for positions past max_seq, the RoPE tables or table_stride *
+ * page_rows, or rows past max_rows; QASR_ENOMEM when the free pages do not
+ * reach (nor for any later request that needs one).  Rows of refused requests
+ * keep their places in the step, are neither stored nor attended, and their
+ * outputs are left as they were; so are those behind the last row.
+ *
+ * len_dev may be the plan's own lens_dev and cursor_dev its cursor_dev: then
+ * each build goes on where the last one ended.  A table may list one page for
+ * several requests (a shared prefix); a page given back twice corrupts the
+ * ring.  The arrays must be distinct otherwise. */
+int qasr_paged_plan_build(qasr_ctx* ctx, qasr_paged_plan* plan, int nreq, const int32_t* len_dev,
+                          const int32_t* rows_dev, int32_t* table_dev, int table_stride,
+                          int32_t* ring_dev, const int32_t* cursor_dev, void* stream);
+
+/* Stage (a) of the planned step's first `rows` rows (qkv_dev [rows][(nqh +
+ * 2*nkvh)*hd]): roped Q -> q_out_dev [rows][nqh*hd], roped K and raw V -> row
+ * row_slot[r] of the layer's pages.  The bits of qasr_qk_norm_rope_append.  A
+ * row without a place is left out. */
+int qasr_paged_append(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows, const void* qkv_dev,
+                      const void* q_gain_dev, const void* k_gain_dev, void* q_out_dev, void* stream);
+
+/* Attention of the planned step's first `rows` rows (q_dev roped, [rows]
+ * [nqh*hd]; out_dev the same shape): a row at position p attends its request's
+ * keys 0..p.  table_dev: the table of the build, unchanged since.  Keys of
+ * entries outside the pool (an evicted page, say -1) are left out; a row that
+ * sees no key gives zeros.  A request's output bits depend on its rows, length
+ * and keys alone, not on its batch mates or where its pages lie. */
+int qasr_paged_attn(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows,
+                    const int32_t* table_dev, int table_stride, const void* q_dev, void* out_dev,
+                    void* stream);
+
 /* ---- Whole text decoder around the attention path ------------------------
  * The layer sequence of src/cpu_decoder.rs:367-532 (CpuTextDecoder::forward,
  * final_norm_logits, argmax, prefill, step), i.e. what WgpuTextDecoder::step

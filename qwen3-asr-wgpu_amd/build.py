@@ -6,9 +6,10 @@ shared library next to this file.  Flags:
   -fhip-fp32-correctly-rounded-divide-sqrt           IEEE '/' and sqrtf (stage (a)
                                                      is bit-exact against the
                                                      reference CPU path)
-Per file: prefill_attn.hip adds -amdgpu-mfma-vgpr-form, which keeps the MFMA
-accumulators in VGPRs; otherwise its one-wave-per-SIMD kernel puts O in AGPRs
-and every rescale and loop-carried copy goes through v_accvgpr moves.
+Per file: prefill_attn.hip and paged_attn.hip add -amdgpu-mfma-vgpr-form, which
+keeps the MFMA accumulators in VGPRs; otherwise prefill's one-wave-per-SIMD
+kernel puts O in AGPRs and every rescale and loop-carried copy goes through
+v_accvgpr moves.
 """
 from __future__ import annotations
 
@@ -43,6 +44,7 @@ FLAGS = [
 
 PER_FILE = {
     "prefill_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "paged_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -11,8 +11,11 @@
 // bank; gains and the row's cos/sin are staged as well.  The work is tiny
 // (8 KiB in, 8 KiB out per row) and latency-bound.
 
+#include <type_traits>
+
 #include "kernels.hpp"
 #include "norm_rope.hpp"
+#include "paged.hpp"
 
 namespace qasr {
 
@@ -23,14 +26,29 @@ constexpr int kMaxNormHeads = 48;  // nqh + nkvh
 constexpr int kPad = kHeadDim + 8;    // f16 raw heads: padded rows
 constexpr int kSqPad = kHeadDim + 4;  // f32 squares: lanes reading head h at the same j sit 4 banks apart
 
+// Where row `row` of a paged step goes: its position, page and row within the
+// page.  A row that the plan gave no place, or whose map entries lie outside
+// the pool or the tables, gets a readable place and false: nothing of it is
+// stored.
+__device__ __forceinline__ bool map_row(const RowMap& P, int row, int& pos, int& slot, int& at) {
+    pos = P.pos[row];
+    const int s = P.slot[row];
+    const bool ok = (uint32_t)pos < (uint32_t)P.rope_rows && (uint32_t)s < (uint32_t)P.slots;
+    pos = ok ? pos : 0;
+    slot = ok ? s >> P.page_shift : 0;
+    at = ok ? s & ((1 << P.page_shift) - 1) : 0;
+    return ok;
+}
+
 // Per row, one memory round trip and one serial chain: the raw q/k heads go
 // to LDS (with their exact f32 squares, computed in parallel), the V heads to
 // registers and straight back out to the cache; then one lane per head runs
 // the reference's 128 dependent adds over the squares (all reads issued
 // ahead of the adds), and the heads are normed, roped and written.
-template <int QK>  // q/k 16-byte pieces per thread: ceil((nqh + nkvh) * 16 / kRowThreads)
+// Rows: SegPlan (segments of a slot pool) or RowMap (rows of a paged pool).
+template <int QK, class Rows>  // q/k 16-byte pieces per thread: ceil((nqh + nkvh) * 16 / kRowThreads)
 __global__ __launch_bounds__(kRowThreads) void norm_rope_append_kernel(
-    CacheGeom g, int layer, SegPlan P, const f16* __restrict__ qkv,
+    CacheGeom g, int layer, Rows P, const f16* __restrict__ qkv,
     const f16* __restrict__ q_gain, const f16* __restrict__ k_gain,
     const f16* __restrict__ cos_tab, const f16* __restrict__ sin_tab, f16* __restrict__ q_out) {
     __shared__ __attribute__((aligned(16))) f16 s_raw[kMaxNormHeads * kPad];
@@ -64,11 +82,17 @@ __global__ __launch_bounds__(kRowThreads) void norm_rope_append_kernel(
         v = *(const uint4*)(vsrc + (it >> 4) * kHeadDim + (it & 15) * 8);
     }
     // Then the row's segment (position, slot) and the gains and cos/sin row.
-    int sg = 0;
-    while (sg + 1 < P.nseg && P.row_base[sg + 1] <= row) ++sg;
-    const int pos = P.pos0[sg] + (row - P.row_base[sg]);
-    const int slot = P.slot[sg];
-    f16* kdst = g.base + slot * g.slot_stride + layer * g.layer_stride + (int64_t)pos * kHeadDim;
+    int pos, slot, at;
+    bool ok = true;
+    if constexpr (std::is_same_v<Rows, SegPlan>) {
+        int sg = 0;
+        while (sg + 1 < P.nseg && P.row_base[sg + 1] <= row) ++sg;
+        at = pos = P.pos0[sg] + (row - P.row_base[sg]);
+        slot = P.slot[sg];
+    } else {
+        ok = map_row(P, row, pos, slot, at);
+    }
+    f16* kdst = g.base + slot * g.slot_stride + layer * g.layer_stride + (int64_t)at * kHeadDim;
     f16* vdst = kdst + g.kv_stride;
     uint4 a;
     {
@@ -104,7 +128,7 @@ __global__ __launch_bounds__(kRowThreads) void norm_rope_append_kernel(
         }
     }
     if (tid < 64) *(uint4*)&s_aux[(tid >> 4) * kHeadDim + (tid & 15) * 8] = a;
-    if (vt >= 0) *(uint4*)(vdst + (vt >> 4) * g.head_stride + (vt & 15) * 8) = v;
+    if (vt >= 0 && ok) *(uint4*)(vdst + (vt >> 4) * g.head_stride + (vt & 15) * 8) = v;
     __syncthreads();
     if (tid < nh) s_inv[tid] = head_inv_rms_squares_all(&s_sq[tid * kSqPad], P.eps);
     __syncthreads();
@@ -117,6 +141,7 @@ __global__ __launch_bounds__(kRowThreads) void norm_rope_append_kernel(
         const f16* gain = is_q ? &s_aux[0] : &s_aux[kHeadDim];
         const float inv = s_inv[h];
         const uint4 o = rope8(&s_raw[h * kPad], gain, crow, srow, inv, j0);
+        if (!ok) continue;
         if (is_q)
             *(uint4*)(q_out + (int64_t)row * nqh * kHeadDim + h * kHeadDim + j0) = o;
         else
@@ -135,9 +160,9 @@ __global__ __launch_bounds__(kRowThreads) void norm_rope_append_kernel(
 // does a row's work in series).
 // NP: piece pairs per lane, ceil((nqh + nkvh) * 8 / 64).
 constexpr int kManyRows = 800;
-template <int NP>
+template <int NP, class Rows>
 __global__ __launch_bounds__(64) void norm_rope_many_kernel(
-    CacheGeom g, int layer, SegPlan P, const f16* __restrict__ qkv,
+    CacheGeom g, int layer, Rows P, const f16* __restrict__ qkv,
     const f16* __restrict__ q_gain, const f16* __restrict__ k_gain,
     const f16* __restrict__ cos_tab, const f16* __restrict__ sin_tab, f16* __restrict__ q_out) {
     constexpr int kHeads = 8 * NP;
@@ -162,12 +187,18 @@ __global__ __launch_bounds__(64) void norm_rope_many_kernel(
     for (int k = 0; k < NV; ++k) v[k].u = *(const uint4*)(src + (int64_t)nh * kHeadDim + min(lane + 64 * k, nv - 1) * 8);
     // The row's segment: the number of later segment starts at or before it
     // (lane i reads segment i's fields; the arrays hold 64).
-    static_assert(kMaxBatch == 64, "one lane per segment");
-    const int e_slot = P.slot[lane], e_pos = P.pos0[lane], e_r0 = P.row_base[lane], e_r1 = P.row_base[lane + 1];
-    const int sg = __popcll(__ballot(lane + 1 < P.nseg && e_r1 <= row));
-    const int pos = __builtin_amdgcn_readlane(e_pos, sg) + row - __builtin_amdgcn_readlane(e_r0, sg);
-    f16* kdst = g.base + __builtin_amdgcn_readlane(e_slot, sg) * g.slot_stride + layer * g.layer_stride +
-                (int64_t)pos * kHeadDim;
+    int pos, slot, at;
+    bool ok = true;
+    if constexpr (std::is_same_v<Rows, SegPlan>) {
+        static_assert(kMaxBatch == 64, "one lane per segment");
+        const int e_slot = P.slot[lane], e_pos = P.pos0[lane], e_r0 = P.row_base[lane], e_r1 = P.row_base[lane + 1];
+        const int sg = __popcll(__ballot(lane + 1 < P.nseg && e_r1 <= row));
+        at = pos = __builtin_amdgcn_readlane(e_pos, sg) + row - __builtin_amdgcn_readlane(e_r0, sg);
+        slot = __builtin_amdgcn_readlane(e_slot, sg);
+    } else {
+        ok = map_row(P, row, pos, slot, at);
+    }
+    f16* kdst = g.base + slot * g.slot_stride + layer * g.layer_stride + (int64_t)at * kHeadDim;
     f16* vdst = kdst + g.kv_stride;
     H8 c[2], sn[2], gn[NP][2];
 #pragma unroll
@@ -188,7 +219,7 @@ __global__ __launch_bounds__(64) void norm_rope_many_kernel(
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int it = lane + 64 * k;
-        if (it < nv) *(uint4*)(vdst + (it >> 4) * g.head_stride + (it & 15) * 8) = v[k].u;
+        if (it < nv && ok) *(uint4*)(vdst + (it >> 4) * g.head_stride + (it & 15) * 8) = v[k].u;
     }
     __syncthreads();  // one wave: its LDS writes have completed
     float inv = 0.0f;
@@ -198,7 +229,7 @@ __global__ __launch_bounds__(64) void norm_rope_many_kernel(
         const int h = h0 + 8 * k;
         H8 o[2];
         rope16(x[k], gn[k], c, sn, __shfl(inv, h), o);
-        if (h < nh) {
+        if (h < nh && ok) {
             f16* dst = h < nqh ? q_out + ((int64_t)row * nqh + h) * kHeadDim : kdst + (h - nqh) * g.head_stride;
             *(uint4*)(dst + 8 * w) = o[0].u;
             *(uint4*)(dst + 8 * w + kHeadDim / 2) = o[1].u;
@@ -208,11 +239,13 @@ __global__ __launch_bounds__(64) void norm_rope_many_kernel(
 
 }  // namespace
 
-hipError_t launch_norm_rope_append(const CacheGeom& g, int layer, const SegPlan& P,
-                                   const f16* qkv, const f16* q_gain, const f16* k_gain,
-                                   const f16* cos_tab, const f16* sin_tab, f16* q_out,
-                                   hipStream_t stream) {
-    const int rows = P.row_base[P.nseg];
+namespace {
+
+// Rows of a step: P.nqh and P.eps, and where each row goes (SegPlan / RowMap).
+template <class Rows>
+hipError_t launch_rows(const CacheGeom& g, int layer, const Rows& P, int rows, const f16* qkv,
+                       const f16* q_gain, const f16* k_gain, const f16* cos_tab,
+                       const f16* sin_tab, f16* q_out, hipStream_t stream) {
     if (rows <= 0) return hipSuccess;
     if (P.nqh < 1 || g.nkvh < 1 || P.nqh + g.nkvh > kMaxNormHeads || g.nkvh * 16 > kRowThreads)
         return hipErrorInvalidValue;
@@ -222,20 +255,36 @@ hipError_t launch_norm_rope_append(const CacheGeom& g, int layer, const SegPlan&
     // way, 900 take 7.4 against 6.6, 16 segments of 50 rows 8.3 against 6.4).
     if (rows >= kManyRows && P.nqh == kRep * g.nkvh) {
         if (P.nqh + g.nkvh <= 24)
-            hipLaunchKernelGGL(norm_rope_many_kernel<3>, dim3(rows), dim3(64), 0, stream, g, layer, P, qkv, q_gain,
-                               k_gain, cos_tab, sin_tab, q_out);
+            hipLaunchKernelGGL((norm_rope_many_kernel<3, Rows>), dim3(rows), dim3(64), 0, stream, g, layer, P, qkv,
+                               q_gain, k_gain, cos_tab, sin_tab, q_out);
         else
-            hipLaunchKernelGGL(norm_rope_many_kernel<6>, dim3(rows), dim3(64), 0, stream, g, layer, P, qkv, q_gain,
-                               k_gain, cos_tab, sin_tab, q_out);
+            hipLaunchKernelGGL((norm_rope_many_kernel<6, Rows>), dim3(rows), dim3(64), 0, stream, g, layer, P, qkv,
+                               q_gain, k_gain, cos_tab, sin_tab, q_out);
         return hipGetLastError();
     }
     if (nqk <= kRowThreads)
-        hipLaunchKernelGGL(norm_rope_append_kernel<1>, dim3(rows), dim3(kRowThreads), 0, stream, g,
+        hipLaunchKernelGGL((norm_rope_append_kernel<1, Rows>), dim3(rows), dim3(kRowThreads), 0, stream, g,
                            layer, P, qkv, q_gain, k_gain, cos_tab, sin_tab, q_out);
     else
-        hipLaunchKernelGGL(norm_rope_append_kernel<2>, dim3(rows), dim3(kRowThreads), 0, stream, g,
+        hipLaunchKernelGGL((norm_rope_append_kernel<2, Rows>), dim3(rows), dim3(kRowThreads), 0, stream, g,
                            layer, P, qkv, q_gain, k_gain, cos_tab, sin_tab, q_out);
     return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_norm_rope_append(const CacheGeom& g, int layer, const SegPlan& P,
+                                   const f16* qkv, const f16* q_gain, const f16* k_gain,
+                                   const f16* cos_tab, const f16* sin_tab, f16* q_out,
+                                   hipStream_t stream) {
+    return launch_rows(g, layer, P, P.row_base[P.nseg], qkv, q_gain, k_gain, cos_tab, sin_tab, q_out, stream);
+}
+
+hipError_t launch_paged_append(const CacheGeom& g, int layer, const RowMap& P, int rows,
+                               const f16* qkv, const f16* q_gain, const f16* k_gain,
+                               const f16* cos_tab, const f16* sin_tab, f16* q_out,
+                               hipStream_t stream) {
+    return launch_rows(g, layer, P, rows, qkv, q_gain, k_gain, cos_tab, sin_tab, q_out, stream);
 }
 
 }  // namespace qasr

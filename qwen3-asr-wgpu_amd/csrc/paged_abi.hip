@@ -1,0 +1,323 @@
+// paged_abi.hip -- C ABI of the paged KV cache (include/qasr_attn.h): page
+// pools, step plans, argument checks and dispatch.
+//
+// The reference's caches are one buffer per slot (decoder.rs:1270-1271,
+// 2453-2457): nothing here has a counterpart in it.
+
+#include <algorithm>
+#include <limits>
+#include <new>
+
+#include "abi_internal.hpp"
+#include "paged.hpp"
+
+using qasr::f16;
+using qasr_abi::DeviceScope;
+using qasr_abi::fail;
+using qasr_abi::hip_fail;
+
+struct qasr_pages {
+    qasr_ctx* ctx;
+    int device;
+    int32_t pages;
+    int32_t shift;  // log2 of a page's rows
+    f16* base = nullptr;
+    size_t bytes = 0;
+};
+
+struct qasr_paged_plan {
+    qasr_ctx* ctx;
+    int device;
+    qasr_pages* pool;
+    int32_t max_requests;
+    int32_t max_rows;
+    int64_t max_items;
+    char* mem = nullptr;  // everything below, one allocation
+    size_t bytes = 0;
+    int32_t *status, *lens, *row_start, *row_pos, *row_slot, *cursor, *n_items;
+    qasr::PagedItem* items;
+    uint32_t *arrived, *counters;
+    float *ws_o, *ws_ml;
+    // The last build, for the checks of the calls that follow it.
+    int32_t nreq = 0;
+    int32_t stride = 0;
+};
+
+namespace {
+
+qasr::CacheGeom page_geom(const qasr_pages* p) {
+    const qasr_attn_cfg& c = p->ctx->cfg;
+    qasr::CacheGeom g;
+    g.base = p->base;
+    g.head_stride = (int64_t)qasr::kHeadDim << p->shift;
+    g.kv_stride = g.head_stride * c.num_key_value_heads;
+    g.slot_stride = 2 * g.kv_stride;  // page
+    g.layer_stride = g.slot_stride * p->pages;
+    g.nkvh = c.num_key_value_heads;
+    g.cap = 1 << p->shift;
+    return g;
+}
+
+int check_plan(qasr_ctx* ctx, qasr_paged_plan* plan) {
+    if (!ctx || !plan) return fail(QASR_EINVAL, "null context or plan");
+    if (plan->ctx != ctx) return fail(QASR_EINVAL, "plan belongs to another context");
+    return QASR_OK;
+}
+
+int check_layer_rows(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows) {
+    const int rc = check_plan(ctx, plan);
+    if (rc) return rc;
+    if (layer < 0 || layer >= ctx->cfg.num_hidden_layers)
+        return fail(QASR_EINVAL, "layer %d outside [0, %d)", layer, ctx->cfg.num_hidden_layers);
+    if (rows < 0) return fail(QASR_EINVAL, "negative rows");
+    if (rows > plan->max_rows) return fail(QASR_ERANGE, "%d rows, the plan holds %d", rows, plan->max_rows);
+    if (!plan->nreq) return fail(QASR_ESTATE, "plan not built (qasr_paged_plan_build)");
+    return QASR_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int qasr_pages_create(qasr_ctx* ctx, int pages, int page_rows, qasr_pages** out) {
+    if (!ctx || !out) return fail(QASR_EINVAL, "null argument");
+    *out = nullptr;
+    int shift = qasr::kPagedMinShift;
+    while (shift < qasr::kPagedMaxShift && (1 << shift) != page_rows) ++shift;
+    if ((1 << shift) != page_rows)
+        return fail(QASR_EINVAL, "page_rows %d is not a power of two from %d to %d", page_rows,
+                    1 << qasr::kPagedMinShift, 1 << qasr::kPagedMaxShift);
+    if (pages <= 0) return fail(QASR_EINVAL, "pages must be > 0");
+    if ((int64_t)pages << shift > std::numeric_limits<int32_t>::max())
+        return fail(QASR_EINVAL, "%d pages of %d rows pass 2^31 rows", pages, page_rows);
+    qasr_pages* p = new (std::nothrow) qasr_pages();
+    if (!p) return fail(QASR_ENOMEM, "out of host memory");
+    p->ctx = ctx;
+    p->device = ctx->device;
+    p->pages = pages;
+    p->shift = shift;
+    p->bytes = (size_t)page_geom(p).layer_stride * ctx->cfg.num_hidden_layers * sizeof(f16);
+    DeviceScope ds(ctx->device);
+    hipError_t e = ds.err;
+    if (e == hipSuccess) e = hipMalloc(&p->base, p->bytes);
+    if (e == hipSuccess) e = hipMemset(p->base, 0, p->bytes);
+    if (e == hipSuccess) e = hipDeviceSynchronize();
+    if (e != hipSuccess) {
+        if (p->base) (void)hipFree(p->base);
+        delete p;
+        return hip_fail(e, "page pool allocation");
+    }
+    *out = p;
+    return QASR_OK;
+}
+
+void qasr_pages_destroy(qasr_pages* p) {
+    if (!p) return;
+    DeviceScope ds(p->device);
+    (void)hipDeviceSynchronize();
+    if (p->base) (void)hipFree(p->base);
+    delete p;
+}
+
+int qasr_pages_get_info(const qasr_pages* p, qasr_pages_info* out) {
+    if (!p || !out) return fail(QASR_EINVAL, "null argument");
+    const qasr::CacheGeom g = page_geom(p);
+    out->base_dev = p->base;
+    out->pages = p->pages;
+    out->page_rows = 1 << p->shift;
+    out->layers = p->ctx->cfg.num_hidden_layers;
+    out->nkvh = g.nkvh;
+    out->head_dim = qasr::kHeadDim;
+    out->layer_stride = g.layer_stride;
+    out->page_stride = g.slot_stride;
+    out->kv_stride = g.kv_stride;
+    out->head_stride = g.head_stride;
+    out->bytes = p->bytes;
+    return QASR_OK;
+}
+
+int qasr_paged_plan_create(qasr_ctx* ctx, qasr_pages* pool, int max_requests, int max_rows, qasr_paged_plan** out) {
+    if (!ctx || !pool || !out) return fail(QASR_EINVAL, "null argument");
+    *out = nullptr;
+    if (pool->ctx != ctx) return fail(QASR_EINVAL, "page pool belongs to another context");
+    if (max_requests < 1 || max_requests > qasr::kPagedMaxRequests)
+        return fail(QASR_EINVAL, "max_requests %d outside [1, %d]", max_requests, qasr::kPagedMaxRequests);
+    if (max_rows < 1 || max_rows > QASR_PAGED_MAX_ROWS)
+        return fail(QASR_EINVAL, "max_rows %d outside [1, %d]", max_rows, QASR_PAGED_MAX_ROWS);
+    qasr_paged_plan* p = new (std::nothrow) qasr_paged_plan();
+    if (!p) return fail(QASR_ENOMEM, "out of host memory");
+    const int nkvh = ctx->cfg.num_key_value_heads;
+    p->ctx = ctx;
+    p->device = ctx->device;
+    p->pool = pool;
+    p->max_requests = max_requests;
+    p->max_rows = max_rows;
+    p->max_items = qasr::paged_max_items(max_requests, max_rows);
+    const int64_t blocks = qasr::paged_max_blocks(max_requests, max_rows) * nkvh;
+    const int64_t recs = qasr::paged_max_records(max_requests, max_rows) * nkvh * qasr::kRep;
+    // One allocation, each part from a multiple of 256 bytes; the parts up to
+    // `clear` start at zero (counters, and a plan that was never built has no
+    // items).
+    size_t at = 0, clear = 0;
+    auto part = [&](size_t n) {
+        const size_t a = at;
+        at += (n + 255) / 256 * 256;
+        return a;
+    };
+    const size_t o_ni = part(4), o_arr = part(4), o_ctr = part(blocks * 4), o_cur = part(8);
+    const size_t o_st = part(4 * (size_t)max_requests), o_len = part(4 * (size_t)max_requests);
+    const size_t o_rs = part(4 * (size_t)(max_requests + 1));
+    const size_t o_rp = part(4 * (size_t)max_rows), o_sl = part(4 * (size_t)max_rows);
+    clear = at;
+    const size_t o_it = part(sizeof(qasr::PagedItem) * p->max_items);
+    const size_t o_o = part(recs * qasr::kHeadDim * 4), o_ml = part(recs * 8);
+    p->bytes = at;
+    DeviceScope ds(ctx->device);
+    hipError_t e = ds.err;
+    if (e == hipSuccess) e = hipMalloc(&p->mem, p->bytes);
+    if (e == hipSuccess) e = hipMemset(p->mem, 0, clear);
+    if (e == hipSuccess) e = hipDeviceSynchronize();
+    if (e != hipSuccess) {
+        if (p->mem) (void)hipFree(p->mem);
+        delete p;
+        return hip_fail(e, "paged plan allocation");
+    }
+    p->n_items = (int32_t*)(p->mem + o_ni);
+    p->arrived = (uint32_t*)(p->mem + o_arr);
+    p->counters = (uint32_t*)(p->mem + o_ctr);
+    p->cursor = (int32_t*)(p->mem + o_cur);
+    p->status = (int32_t*)(p->mem + o_st);
+    p->lens = (int32_t*)(p->mem + o_len);
+    p->row_start = (int32_t*)(p->mem + o_rs);
+    p->row_pos = (int32_t*)(p->mem + o_rp);
+    p->row_slot = (int32_t*)(p->mem + o_sl);
+    p->items = (qasr::PagedItem*)(p->mem + o_it);
+    p->ws_o = (float*)(p->mem + o_o);
+    p->ws_ml = (float*)(p->mem + o_ml);
+    *out = p;
+    return QASR_OK;
+}
+
+void qasr_paged_plan_destroy(qasr_paged_plan* p) {
+    if (!p) return;
+    DeviceScope ds(p->device);
+    (void)hipDeviceSynchronize();
+    if (p->mem) (void)hipFree(p->mem);
+    delete p;
+}
+
+int qasr_paged_plan_get_info(const qasr_paged_plan* p, qasr_paged_plan_info* out) {
+    if (!p || !out) return fail(QASR_EINVAL, "null argument");
+    out->max_requests = p->max_requests;
+    out->max_rows = p->max_rows;
+    out->status_dev = p->status;
+    out->lens_dev = p->lens;
+    out->row_start_dev = p->row_start;
+    out->row_pos_dev = p->row_pos;
+    out->row_slot_dev = p->row_slot;
+    out->cursor_dev = p->cursor;
+    out->bytes = p->bytes;
+    return QASR_OK;
+}
+
+int qasr_paged_plan_build(qasr_ctx* ctx, qasr_paged_plan* plan, int nreq, const int32_t* len_dev,
+                          const int32_t* rows_dev, int32_t* table_dev, int table_stride,
+                          int32_t* ring_dev, const int32_t* cursor_dev, void* stream) {
+    const int rc = check_plan(ctx, plan);
+    if (rc) return rc;
+    if (nreq < 1) return fail(QASR_EINVAL, "nreq must be > 0");
+    if (nreq > plan->max_requests)
+        return fail(QASR_ERANGE, "%d requests, the plan holds %d", nreq, plan->max_requests);
+    if (table_stride < 1) return fail(QASR_EINVAL, "table_stride must be > 0");
+    if (!len_dev || !rows_dev || !table_dev) return fail(QASR_EINVAL, "null device pointer");
+    if (!ring_dev != !cursor_dev) return fail(QASR_EINVAL, "ring and cursor go together");
+    DeviceScope ds(ctx->device);
+    if (ds.err != hipSuccess) return hip_fail(ds.err, "hipSetDevice");
+    qasr::PagedPlanArgs a;
+    a.len = len_dev;
+    a.rows = rows_dev;
+    a.table = table_dev;
+    a.ring = ring_dev;
+    a.cursor = cursor_dev;
+    a.nreq = nreq;
+    a.stride = table_stride;
+    a.pages = plan->pool->pages;
+    a.page_shift = plan->pool->shift;
+    a.max_seq = ctx->cos ? std::min(ctx->cfg.max_seq, ctx->rope_rows) : ctx->cfg.max_seq;
+    a.max_rows = plan->max_rows;
+    a.status = plan->status;
+    a.lens_out = plan->lens;
+    a.row_start = plan->row_start;
+    a.row_pos = plan->row_pos;
+    a.row_slot = plan->row_slot;
+    a.cursor_out = plan->cursor;
+    a.n_items = plan->n_items;
+    a.items = plan->items;
+    a.arrived = plan->arrived;
+    const hipError_t e = qasr::launch_paged_plan(a, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "paged plan launch");
+    plan->nreq = nreq;
+    plan->stride = table_stride;
+    return QASR_OK;
+}
+
+int qasr_paged_append(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows, const void* qkv_dev,
+                      const void* q_gain_dev, const void* k_gain_dev, void* q_out_dev, void* stream) {
+    const int rc = check_layer_rows(ctx, plan, layer, rows);
+    if (rc) return rc;
+    if (rows == 0) return QASR_OK;
+    if (!qkv_dev || !q_gain_dev || !k_gain_dev || !q_out_dev) return fail(QASR_EINVAL, "null device pointer");
+    if (!ctx->cos) return fail(QASR_ESTATE, "RoPE tables not set (qasr_set_rope_tables)");
+    DeviceScope ds(ctx->device);
+    if (ds.err != hipSuccess) return hip_fail(ds.err, "hipSetDevice");
+    qasr::RowMap P;
+    P.pos = plan->row_pos;
+    P.slot = plan->row_slot;
+    P.slots = plan->pool->pages << plan->pool->shift;
+    P.page_shift = plan->pool->shift;
+    P.rope_rows = ctx->rope_rows;
+    P.nqh = ctx->cfg.num_attention_heads;
+    P.eps = ctx->cfg.rms_norm_eps;
+    const hipError_t e = qasr::launch_paged_append(page_geom(plan->pool), layer, P, rows, (const f16*)qkv_dev,
+                                                   (const f16*)q_gain_dev, (const f16*)k_gain_dev, ctx->cos, ctx->sin,
+                                                   (f16*)q_out_dev, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "paged append launch");
+    return QASR_OK;
+}
+
+int qasr_paged_attn(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows, const int32_t* table_dev,
+                    int table_stride, const void* q_dev, void* out_dev, void* stream) {
+    const int rc = check_layer_rows(ctx, plan, layer, rows);
+    if (rc) return rc;
+    if (table_stride != plan->stride)
+        return fail(QASR_EINVAL, "table_stride %d, the plan was built with %d", table_stride, plan->stride);
+    if (rows == 0) return QASR_OK;
+    if (!table_dev || !q_dev || !out_dev) return fail(QASR_EINVAL, "null device pointer");
+    DeviceScope ds(ctx->device);
+    if (ds.err != hipSuccess) return hip_fail(ds.err, "hipSetDevice");
+    const qasr::CacheGeom g = page_geom(plan->pool);
+    qasr::PagedAttnArgs a;
+    a.q = (const f16*)q_dev;
+    a.out = (f16*)out_dev;
+    a.base = g.base + layer * g.layer_stride;
+    a.page_stride = g.slot_stride;
+    a.kv_stride = g.kv_stride;
+    a.head_stride = g.head_stride;
+    a.table = table_dev;
+    a.stride = table_stride;
+    a.pages = plan->pool->pages;
+    a.page_shift = plan->pool->shift;
+    a.nkvh = g.nkvh;
+    a.rows = rows;
+    a.scale_log2 = ctx->scale_log2;
+    a.n_items = plan->n_items;
+    a.items = plan->items;
+    a.ws_o = plan->ws_o;
+    a.ws_ml = plan->ws_ml;
+    a.counters = plan->counters;
+    const hipError_t e = qasr::launch_paged_attn(a, plan->max_items, ctx->cus, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "paged attention launch");
+    return QASR_OK;
+}
+
+}  // extern "C"

@@ -39,6 +39,9 @@ ABI_SYMBOLS = (
     "qasr_decoder_prefill_batch", "qasr_dequant_i8", "qasr_prefill_attn_batch",
     "qasr_softmax_weights", "qasr_stream_read", "qasr_prefill_attn_noalloc", "qasr_gemm_f16",
     "qasr_mfma_probe", "qasr_plan_decode", "qasr_plan_prefill",
+    "qasr_pages_create", "qasr_pages_destroy", "qasr_pages_get_info", "qasr_paged_plan_create",
+    "qasr_paged_plan_destroy", "qasr_paged_plan_get_info", "qasr_paged_plan_build",
+    "qasr_paged_append", "qasr_paged_attn",
 )
 MAX_PREFILL_SEGMENTS = 64  # segments per qasr_decoder_prefill_batch call
 
@@ -93,6 +96,29 @@ class DecoderCfg(ctypes.Structure):
         ("vocab_size", ctypes.c_int32),
         ("max_rows", ctypes.c_int32),
     ]
+
+
+class PagesInfo(ctypes.Structure):
+    _fields_ = [
+        ("base_dev", ctypes.c_void_p),
+        ("pages", ctypes.c_int32),
+        ("page_rows", ctypes.c_int32),
+        ("layers", ctypes.c_int32),
+        ("nkvh", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("layer_stride", ctypes.c_int64),
+        ("page_stride", ctypes.c_int64),
+        ("kv_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("bytes", ctypes.c_size_t),
+    ]
+
+
+class PagedPlanInfo(ctypes.Structure):
+    _fields_ = [("max_requests", ctypes.c_int32), ("max_rows", ctypes.c_int32)] + [
+        (name, ctypes.c_void_p) for name in ("status_dev", "lens_dev", "row_start_dev",
+                                             "row_pos_dev", "row_slot_dev", "cursor_dev")
+    ] + [("bytes", ctypes.c_size_t)]
 
 
 _lib = None
@@ -157,6 +183,19 @@ def load(path: str = LIB_PATH):
     i32p = ctypes.POINTER(ctypes.c_int32)
     L.qasr_plan_decode.argtypes = [ctypes.c_int, i32p, ctypes.c_int, ctypes.c_int, i32p, i32p, i32p]
     L.qasr_plan_prefill.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int, i32p, i32p, i32p, i32p]
+    L.qasr_pages_create.argtypes = [_vp, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)]
+    L.qasr_pages_destroy.argtypes = [_vp]
+    L.qasr_pages_destroy.restype = None
+    L.qasr_pages_get_info.argtypes = [_vp, ctypes.POINTER(PagesInfo)]
+    L.qasr_paged_plan_create.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)]
+    L.qasr_paged_plan_destroy.argtypes = [_vp]
+    L.qasr_paged_plan_destroy.restype = None
+    L.qasr_paged_plan_get_info.argtypes = [_vp, ctypes.POINTER(PagedPlanInfo)]
+    L.qasr_paged_plan_build.argtypes = [_vp, _vp, ctypes.c_int, _vp, _vp, _vp, ctypes.c_int, _vp,
+                                        _vp, _vp]
+    L.qasr_paged_append.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, _vp, _vp]
+    L.qasr_paged_attn.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int, _vp,
+                                  _vp, _vp]
     _lib = L
     return L
 
@@ -319,12 +358,16 @@ class KVPool:
 
 
 class _DeviceView:
-    """__cuda_array_interface__ over library-owned device memory (f16)."""
+    """__cuda_array_interface__ over library-owned device memory (f16, or
+    int32 with typestr "<i4").  A torch tensor made of it, and every view of
+    that tensor, holds on to it and so to `owner`, the object that frees the
+    memory."""
 
-    def __init__(self, ptr: int, nbytes: int, device: int):
+    def __init__(self, ptr: int, nbytes: int, device: int, typestr: str = "<f2", owner=None):
+        self.owner = owner
         self.__cuda_array_interface__ = {
-            "shape": (nbytes // 2,),
-            "typestr": "<f2",
+            "shape": (nbytes // int(typestr[-1]),),
+            "typestr": typestr,
             "data": (int(ptr), False),
             "version": 3,
             "strides": None,
@@ -430,6 +473,206 @@ def prefill_layer(ctx: Context, kv: KVPool, layer: int, slot: int, kv_start: int
                                      _dev(qkv, "qkv"), _dev(q_gain, "q_gain"),
                                      _dev(k_gain, "k_gain"), _dev(q_work, "q_work"),
                                      _dev(out, "out"), _stream(stream)))
+
+
+# ---- paged KV cache -------------------------------------------------------
+
+PAGED_MAX_REQUESTS = 1024
+PAGED_MAX_ROWS = 65536
+
+
+class PagePool:
+    """One pool of KV pages for all sequences (qasr_pages):
+    [layer][page][K|V][kvh][page_rows][hd] f16, zeroed."""
+
+    def __init__(self, ctx: Context, pages: int, page_rows: int = 16):
+        self.ctx = ctx
+        self.handle = None
+        h = _vp()
+        _check(load().qasr_pages_create(ctx.handle, pages, page_rows, ctypes.byref(h)))
+        self.handle = h
+        self.pages, self.page_rows = pages, page_rows
+
+    def info(self) -> PagesInfo:
+        inf = PagesInfo()
+        _check(load().qasr_pages_get_info(self.handle, ctypes.byref(inf)))
+        return inf
+
+    def tensor(self):
+        """A torch view of the whole pool, shaped
+        [layer][page][2][kvh][page_rows][hd]."""
+        import torch
+
+        inf = self.info()
+        storage = _DeviceView(inf.base_dev, inf.bytes, self.ctx.device, owner=self)
+        t = torch.as_tensor(storage, device=f"cuda:{self.ctx.device}")
+        return t.view(inf.layers, inf.pages, 2, inf.nkvh, inf.page_rows, inf.head_dim)
+
+    def free_ring(self):
+        """The ring and cursor of a pool with every page free: int32 CUDA
+        tensors [pages] and [2]."""
+        import torch
+
+        dev = f"cuda:{self.ctx.device}"
+        return (torch.arange(self.pages, dtype=torch.int32, device=dev),
+                torch.tensor([0, self.pages], dtype=torch.int32, device=dev))
+
+    def close(self):
+        if self.handle:
+            load().qasr_pages_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class _PlanMemory:
+    """A qasr_paged_plan and what it needs alive; destroyed with its last user:
+    the PagedPlan, and the views of its arrays (which a PagedPlan holds itself,
+    so they cannot hold on to the PagedPlan)."""
+
+    def __init__(self, ctx: Context, pool: PagePool, max_requests: int, max_rows: int):
+        self.keep = (ctx, pool)
+        self.handle = None
+        h = _vp()
+        _check(load().qasr_paged_plan_create(ctx.handle, pool.handle, max_requests, max_rows,
+                                             ctypes.byref(h)))
+        self.handle = h
+
+    def close(self):
+        if self.handle:
+            load().qasr_paged_plan_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class PagedPlan:
+    """A step's plan (qasr_paged_plan) and int32 views of its device arrays:
+    `status`, `lens` [max_requests], `row_start` [max_requests + 1],
+    `row_pos`, `row_slot` [max_rows] and `cursor` [2]."""
+
+    def __init__(self, ctx: Context, pool: PagePool, max_requests: int, max_rows: int):
+        import torch
+
+        self.ctx, self.pool = ctx, pool
+        self.max_requests, self.max_rows = max_requests, max_rows
+        self.nreq = 0
+        self._mem = _PlanMemory(ctx, pool, max_requests, max_rows)
+        inf = PagedPlanInfo()
+        _check(load().qasr_paged_plan_get_info(self.handle, ctypes.byref(inf)))
+        self.bytes = inf.bytes
+
+        def view(ptr, n):
+            v = _DeviceView(ptr, 4 * n, ctx.device, "<i4", self._mem)
+            return torch.as_tensor(v, device=f"cuda:{ctx.device}")
+
+        self.status = view(inf.status_dev, max_requests)
+        self.lens = view(inf.lens_dev, max_requests)
+        self.row_start = view(inf.row_start_dev, max_requests + 1)
+        self.row_pos = view(inf.row_pos_dev, max_rows)
+        self.row_slot = view(inf.row_slot_dev, max_rows)
+        self.cursor = view(inf.cursor_dev, 2)
+
+    @property
+    def handle(self):
+        return self._mem.handle
+
+    def close(self):
+        """Free the plan now; its views must not be used any more."""
+        self._mem.close()
+
+
+def _on(ctx: Context, t, name: str, dtype=None) -> int:
+    """`_dev` of a tensor on the context's GPU."""
+    ptr = _dev(t, name, dtype)
+    if t.device.index != ctx.device:
+        raise QasrError(QASR_EINVAL, f"{name} is on {t.device}, the context on GPU {ctx.device}")
+    return ptr
+
+
+def _ctx_stream(ctx: Context, stream) -> int:
+    """`stream`, or torch's current stream of the context's GPU."""
+    if stream is not None:
+        return int(stream)
+    import torch
+
+    return int(torch.cuda.current_stream(ctx.device).cuda_stream)
+
+
+def _table(table, nreq: int):
+    """Row stride of a block table [requests][pages of a request]."""
+    if table.dim() != 2 or table.shape[0] < nreq:
+        raise QasrError(QASR_EINVAL, f"the table must be [{nreq} or more][pages], got "
+                                     f"{list(table.shape)}")
+    return int(table.shape[1])
+
+
+def paged_plan(ctx: Context, plan: PagedPlan, lens, rows, table, ring=None, cursor=None,
+               stream=None):
+    """Plan one step (qasr_paged_plan_build) of len(rows) requests: `lens` rows
+    in the cache each, `rows` new ones (0: idle, -1: ended), `table` [requests]
+    [pages of a request], and the free pages `ring` [pages] and `cursor`
+    ({head, free}), or None for a table that holds the new rows' pages; all
+    int32 CUDA tensors.  `lens` may be plan.lens and `cursor` plan.cursor."""
+    import torch
+
+    i32 = torch.int32
+    n = int(rows.numel())
+    _need(lens, n, "lens")
+    stride = _table(table, n)
+    if (ring is None) != (cursor is None):
+        raise QasrError(QASR_EINVAL, "ring and cursor go together")
+    if ring is not None:
+        _need(ring, plan.pool.pages, "ring", exact=True)
+        _need(cursor, 2, "cursor", exact=True)
+    _check(load().qasr_paged_plan_build(
+        ctx.handle, plan.handle, n, _on(ctx, lens, "lens", i32), _on(ctx, rows, "rows", i32),
+        _on(ctx, table, "table", i32), stride,
+        _on(ctx, ring, "ring", i32) if ring is not None else None,
+        _on(ctx, cursor, "cursor", i32) if cursor is not None else None, _ctx_stream(ctx, stream)))
+    plan.nreq = n
+
+
+def _paged_rows(t, width: int, name: str) -> int:
+    """Rows of a [rows][width] tensor."""
+    if t.dim() != 2 or t.shape[1] != width:
+        raise QasrError(QASR_EINVAL, f"{name} must be [rows][{width}], got {list(t.shape)}")
+    return int(t.shape[0])
+
+
+def paged_append(ctx: Context, plan: PagedPlan, layer: int, qkv, q_gain, k_gain, q_out,
+                 stream=None):
+    """Stage (a) of the planned step's rows into the layer's pages
+    (qasr_paged_append): qkv [rows][(nqh + 2 nkvh) hd], q_out [rows][nqh hd]."""
+    tot, qd = _widths(ctx)
+    rows = _paged_rows(qkv, tot, "qkv")
+    _need(q_out, rows * qd, "q_out")
+    _gains(ctx, q_gain, k_gain)
+    _check(load().qasr_paged_append(
+        ctx.handle, plan.handle, layer, rows, _on(ctx, qkv, "qkv"), _on(ctx, q_gain, "q_gain"),
+        _on(ctx, k_gain, "k_gain"), _on(ctx, q_out, "q_out"), _ctx_stream(ctx, stream)))
+
+
+def paged_attn(ctx: Context, plan: PagedPlan, layer: int, table, q, out, stream=None):
+    """Attention of the planned step's rows over their pages
+    (qasr_paged_attn): q and out [rows][nqh hd], `table` as planned."""
+    import torch
+
+    _, qd = _widths(ctx)
+    rows = _paged_rows(q, qd, "q")
+    _need(out, rows * qd, "out")
+    stride = _table(table, plan.nreq)
+    _check(load().qasr_paged_attn(
+        ctx.handle, plan.handle, layer, rows, _on(ctx, table, "table", torch.int32), stride,
+        _on(ctx, q, "q"), _on(ctx, out, "out"), _ctx_stream(ctx, stream)))
 
 
 class AttnBackend:
