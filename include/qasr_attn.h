@@ -482,6 +482,12 @@ int qasr_plan_decode(int batch, const int32_t* lens, int nkvh, int cus, int32_t*
 int qasr_plan_prefill(int rows, int kv_start, int nkvh, int32_t* rows_per_block, int32_t* nrb,
                       int32_t* tiles_per_split, int32_t* sp_base_out);
 
+/* Paged attention (qasr_paged_attn): how a request of `rows` >= 1 new rows
+ * after `len` cached ones is cut: *wide 0: row blocks of 16 rows, 1: of 64;
+ * *blocks of them; *splits key ranges each.  A function of (len, rows) alone.
+ * len in [0, 1 << 24], rows in [1, QASR_PAGED_MAX_ROWS]. */
+int qasr_plan_paged(int len, int rows, int32_t* wide, int32_t* blocks, int32_t* splits);
+
 #ifdef __cplusplus
 }
 #endif

@@ -79,11 +79,9 @@ __device__ __forceinline__ void step_scores(const Wave& w, const f16* kt, float1
 
 // The softmax of those scores (first key k0): row max, the running-max
 // update, P^T (f16, B-operand layout) and its row sum.  MASK: some key is
-// past some row's position, or in a 16-key group whose bit of `hidden` is set
-// (bit j: keys 16 j .. +16 of the step).
+// past some row's position.
 template <bool MASK, int NB>
-__device__ __forceinline__ void step_softmax(Wave& w, float16v (&s)[NB], int k0, uint32_t hidden,
-                                             half8v (&pb)[2 * NB]) {
+__device__ __forceinline__ void step_softmax(Wave& w, float16v (&s)[NB], int k0, half8v (&pb)[2 * NB]) {
     float mx = kNegInf;
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
@@ -91,7 +89,7 @@ __device__ __forceinline__ void step_softmax(Wave& w, float16v (&s)[NB], int k0,
         for (int i = 0; i < 16; ++i) {
             if (MASK) {
                 const int key = k0 + kb * 32 + 8 * (i >> 2) + 4 * w.g + (i & 3);
-                s[kb][i] = key > w.qpos || (hidden >> (2 * kb + (i >> 3)) & 1) ? kNegInf : s[kb][i];
+                s[kb][i] = key > w.qpos ? kNegInf : s[kb][i];
             }
             mx = fmaxf(mx, s[kb][i]);
         }
@@ -133,7 +131,7 @@ template <bool MASK, int NB>
 __device__ __forceinline__ void step_s(Wave& w, const f16* kt, int k0, half8v (&pb)[2 * NB]) {
     float16v s[NB];
     step_scores<NB>(w, kt, s);
-    step_softmax<MASK, NB>(w, s, k0, 0u, pb);
+    step_softmax<MASK, NB>(w, s, k0, pb);
 }
 
 // Second half: O^T += V^T P^T with V rows vt[0..32 NB - 1] of a tile of ROWS

@@ -31,11 +31,11 @@ struct qasr_paged_plan {
     qasr_pages* pool;
     int32_t max_requests;
     int32_t max_rows;
-    int64_t max_items;
+    int32_t max_narrow, max_wide;  // work items
     char* mem = nullptr;  // everything below, one allocation
     size_t bytes = 0;
     int32_t *status, *lens, *row_start, *row_pos, *row_slot, *cursor, *n_items;
-    qasr::PagedItem* items;
+    qasr::PagedItem *narrow, *wide;
     uint32_t *arrived, *counters;
     float *ws_o, *ws_ml;
     // The last build, for the checks of the calls that follow it.
@@ -152,7 +152,8 @@ int qasr_paged_plan_create(qasr_ctx* ctx, qasr_pages* pool, int max_requests, in
     p->pool = pool;
     p->max_requests = max_requests;
     p->max_rows = max_rows;
-    p->max_items = qasr::paged_max_items(max_requests, max_rows);
+    p->max_narrow = (int32_t)qasr::paged_max_items(max_requests, max_rows, qasr::kNarrowRows);
+    p->max_wide = (int32_t)qasr::paged_max_items(max_requests, max_rows, qasr::kWideRows);
     const int64_t blocks = qasr::paged_max_blocks(max_requests, max_rows) * nkvh;
     const int64_t recs = qasr::paged_max_records(max_requests, max_rows) * nkvh * qasr::kRep;
     // One allocation, each part from a multiple of 256 bytes; the parts up to
@@ -164,12 +165,13 @@ int qasr_paged_plan_create(qasr_ctx* ctx, qasr_pages* pool, int max_requests, in
         at += (n + 255) / 256 * 256;
         return a;
     };
-    const size_t o_ni = part(4), o_arr = part(4), o_ctr = part(blocks * 4), o_cur = part(8);
+    const size_t o_ni = part(8), o_arr = part(4), o_ctr = part(blocks * 4 * qasr::kPagedCounterStep), o_cur = part(8);
     const size_t o_st = part(4 * (size_t)max_requests), o_len = part(4 * (size_t)max_requests);
     const size_t o_rs = part(4 * (size_t)(max_requests + 1));
     const size_t o_rp = part(4 * (size_t)max_rows), o_sl = part(4 * (size_t)max_rows);
     clear = at;
-    const size_t o_it = part(sizeof(qasr::PagedItem) * p->max_items);
+    const size_t o_it = part(sizeof(qasr::PagedItem) * (size_t)p->max_narrow);
+    const size_t o_wi = part(sizeof(qasr::PagedItem) * (size_t)p->max_wide);
     const size_t o_o = part(recs * qasr::kHeadDim * 4), o_ml = part(recs * 8);
     p->bytes = at;
     DeviceScope ds(ctx->device);
@@ -191,7 +193,8 @@ int qasr_paged_plan_create(qasr_ctx* ctx, qasr_pages* pool, int max_requests, in
     p->row_start = (int32_t*)(p->mem + o_rs);
     p->row_pos = (int32_t*)(p->mem + o_rp);
     p->row_slot = (int32_t*)(p->mem + o_sl);
-    p->items = (qasr::PagedItem*)(p->mem + o_it);
+    p->narrow = (qasr::PagedItem*)(p->mem + o_it);
+    p->wide = (qasr::PagedItem*)(p->mem + o_wi);
     p->ws_o = (float*)(p->mem + o_o);
     p->ws_ml = (float*)(p->mem + o_ml);
     *out = p;
@@ -252,7 +255,8 @@ int qasr_paged_plan_build(qasr_ctx* ctx, qasr_paged_plan* plan, int nreq, const 
     a.row_slot = plan->row_slot;
     a.cursor_out = plan->cursor;
     a.n_items = plan->n_items;
-    a.items = plan->items;
+    a.narrow = plan->narrow;
+    a.wide = plan->wide;
     a.arrived = plan->arrived;
     const hipError_t e = qasr::launch_paged_plan(a, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(e, "paged plan launch");
@@ -311,12 +315,26 @@ int qasr_paged_attn(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows, c
     a.rows = rows;
     a.scale_log2 = ctx->scale_log2;
     a.n_items = plan->n_items;
-    a.items = plan->items;
+    a.narrow = plan->narrow;
+    a.wide = plan->wide;
+    a.max_narrow = plan->max_narrow;
+    a.max_wide = qasr::paged_wide(plan->max_rows, (int64_t)plan->stride << plan->pool->shift) ? plan->max_wide : 0;
     a.ws_o = plan->ws_o;
     a.ws_ml = plan->ws_ml;
     a.counters = plan->counters;
-    const hipError_t e = qasr::launch_paged_attn(a, plan->max_items, ctx->cus, (hipStream_t)stream);
+    const hipError_t e = qasr::launch_paged_attn(a, ctx->cus, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(e, "paged attention launch");
+    return QASR_OK;
+}
+
+int qasr_plan_paged(int len, int rows, int32_t* wide, int32_t* blocks, int32_t* splits) {
+    if (len < 0 || len > 1 << 24 || rows < 1 || rows > QASR_PAGED_MAX_ROWS)
+        return fail(QASR_EINVAL, "len %d / rows %d", len, rows);
+    if (!wide || !blocks || !splits) return fail(QASR_EINVAL, "null pointer");
+    const qasr::PagedShape s = qasr::paged_shape(len, rows);
+    *wide = s.wide;
+    *blocks = s.blocks;
+    *splits = s.splits;
     return QASR_OK;
 }
 

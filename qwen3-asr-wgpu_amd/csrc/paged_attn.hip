@@ -41,16 +41,17 @@ namespace qasr {
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kSlice = 32;                        // keys of a wave's slice of a narrow tile
-constexpr int kBufHalves = 4 * 2 * kSlice * kHeadDim;  // 64 KB
-static_assert(kBufHalves == 2 * 2 * kWideTile * kHeadDim, "two wide tiles of K and V");
+constexpr int kSlice = 32;                          // keys of a wave's slice of a narrow tile
+constexpr int kNarrowWaves = kNarrowTile / kSlice;  // 4
+constexpr int kWideWaves = kWideTile / 16;          // 8
 
-// One copy instruction: lane l's 16 bytes from base + voff to lds + 16 l.
-// Waited for by count; the address registers are scalar and constant.
-__device__ __forceinline__ void copy16(const f16* base, uint32_t voff, uint32_t lds) {
-    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "{m0}"(lds) : "memory");
-}
+template <int NW>
+struct Shared {
+    f16 buf[NW * 2 * kSlice * kHeadDim];  // 16 KB a wave: a slice of K and V, or two wide tiles
+    float ml[NW][2][64];
+    int last;
+};
+static_assert(sizeof(Shared<kWideWaves>::buf) == 2 * 2 * kWideTile * kHeadDim * sizeof(f16), "two wide tiles of K and V");
 
 // The thread's index, opaque to the compiler: what is derived from it then
 // lives in one place of the item loop instead of in registers all through it
@@ -74,247 +75,319 @@ __device__ __forceinline__ float2 load_dev2(const float* p) {
 // What a workgroup knows of its item.
 struct Item {
     int row0, rows, pos0, kend, tile0, tile1, splits, split, rec, block, kvh;
+    int page0, last_page;  // first page of the range, last of the row block's keys (table places)
     const int32_t* table;  // the request's pages
+    const f16* base;       // the kv head's K in page 0
 };
 
-// The copies of one 16-key group at `base`: K instruction j reads rows 4 j ..
-// +4 with their 16-byte chunks permuted (swz16: lane l's chunk is (l % 16) ^ (4
-// (l / 16) | j)), V instruction j dims 32 j .. +32 of the 16 rows.  A lane's
-// offsets are two registers of the kernel: what j adds is a scalar, and for K
-// an exclusive or of j.
+// Copies of one 16-key group, 1 KB an instruction (lane l's 16 bytes to m0 +
+// 16 l): K instruction j reads rows 4 j .. +4 with their 16-byte chunks
+// permuted (swz16: lane l's chunk is (l % 16) ^ (4 (l / 16) | j)), V
+// instruction j dims 32 j .. +32 of the 16 rows, `slab` bytes on in the LDS.
+// The group's address is scalar, a lane's offsets are registers of the kernel,
+// so a copy is an instruction and its LDS address (which m0 needs a cycle to
+// take).  Waited for by count.
 struct Offsets {
-    uint32_t k, v;
+    uint32_t k[4], v[4];
 };
-__device__ __forceinline__ Offsets group_offsets(int lane) {
-    const int r = lane >> 4;
-    return {(uint32_t)(r * 256 + (((lane & 15) ^ (r << 2)) * 16)), (uint32_t)((lane >> 2) * 256 + (lane & 3) * 16)};
-}
-__device__ __forceinline__ void copy_k(const f16* base, Offsets o, uint32_t lds) {
-    asm volatile("" : "+v"(o.k), "+s"(lds));  // made here, not kept for the whole kernel
+__device__ __forceinline__ void copy4(const f16* base, const uint32_t (&voff)[4], uint32_t lds, uint32_t step) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) copy16(base + j * 4 * kHeadDim, o.k ^ (16 * j), lds + j * 1024);
+    for (int j = 0; j < 4; ++j)
+        asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff[j]), "s"(base), "{m0}"(lds + j * step)
+                     : "memory");
 }
-__device__ __forceinline__ void copy_v(const f16* base, const Offsets& o, uint32_t lds, uint32_t slab) {
-    asm volatile("" : "+s"(lds));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) copy16(base + j * 32, o.v, lds + j * slab);
-}
-// The same for the group of the last key, or past it (`base`: the last
-// group): row r reads row min(r + add, last).
-__device__ __forceinline__ void copy_k_tail(const f16* base, int add, int last, uint32_t lds) {
-    asm volatile("" : "+s"(lds));
-    const int lane = thread_id() & 63;
+// Row r of the group reads row min(r + add, last): 0 and 15, but in the group
+// of the last key or past it.  `v_from_k`: bytes from a page's K to its V.
+__device__ __forceinline__ Offsets group_offsets(int lane, int add, int last, uint32_t v_from_k) {
+    Offsets o;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int r = lane >> 4;
-        copy16(base, min(4 * j + r + add, last) * 256 + (((lane & 15) ^ (r << 2) ^ j) * 16), lds + j * 1024);
+        o.k[j] = min(4 * j + r + add, last) * 256 + (((lane & 15) ^ (r << 2) ^ j) * 16);
+        o.v[j] = v_from_k + min((lane >> 2) + add, last) * 256 + j * 64 + (lane & 3) * 16;
     }
-}
-__device__ __forceinline__ void copy_v_tail(const f16* base, int add, int last, uint32_t lds, uint32_t slab) {
-    asm volatile("" : "+s"(lds));
-    const int lane = thread_id() & 63;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        copy16(base + j * 32, min((lane >> 2) + add, last) * 256 + (lane & 3) * 16, lds + j * slab);
+    return o;
 }
 
-// Page ids of 64 key groups, a lane each: of the 16-key group (k0 + 16 *
-// stride_groups ...), see the callers.  Keys past the end read the last
-// key's page.  `bad`: lanes whose page lies outside the pool; their id is
-// made 0, which is readable.
-struct Pages {
+// The range's pages, a lane each: lane l of the first registers is page page0
+// + lo + l of the table, of the second the 64 after them.  The work item
+// brings the first 48 ids (lanes 16 .. 63, lo = -16), so that the first copies
+// wait for one load; longer ranges read on from the table.  An id outside the
+// pool sets its lane's bit in `bad` and reads page 0; its keys are hidden.
+struct PageRun {
     int id;
     uint64_t bad;
 };
-__device__ __forceinline__ Pages load_pages(const PagedAttnArgs& a, const Item& it, int key) {
-    Pages p;
-    p.id = it.table[min(key, it.kend - 1) >> a.page_shift];
-    return p;
+struct Pages {
+    PageRun cur, nxt;
+    int lo;
+};
+__device__ __forceinline__ int load_pages(const Item& it, int rel) {
+    return it.last_page - it.page0 >= rel ? it.table[min(it.page0 + rel + (thread_id() & 63), it.last_page)] : 0;
 }
-__device__ __forceinline__ void check_pages(const PagedAttnArgs& a, Pages& p) {
-    const bool bad = (uint32_t)p.id >= (uint32_t)a.pages;
-    p.bad = __ballot(bad);
-    p.id = bad ? 0 : p.id;
+__device__ __forceinline__ PageRun check_pages(const PagedAttnArgs& a, int id) {
+    const bool bad = (uint32_t)id >= (uint32_t)a.pages;
+    return {bad ? 0 : id, __ballot(bad)};
 }
-
-// Address of K of the 16-key group that holds `key`, in page id.
-__device__ __forceinline__ const f16* group_base(const PagedAttnArgs& a, int kvh, int id, int key) {
-    return a.base + id * a.page_stride + kvh * a.head_stride +
-           ((key & ((1 << a.page_shift) - 1)) & ~15) * kHeadDim;
+__device__ __forceinline__ int page_rel(const PagedAttnArgs& a, const Item& it, int key) {
+    return (min(key, it.kend - 1) >> a.page_shift) - it.page0;
+}
+// Before the pages from `key` on are asked for: on to the next 64.
+__device__ __forceinline__ void advance_pages(const PagedAttnArgs& a, const Item& it, Pages& p, int key) {
+    if (__builtin_expect(page_rel(a, it, key) - p.lo >= 64, 0)) {
+        p.cur = p.nxt;
+        p.lo += 64;
+        p.nxt = check_pages(a, load_pages(it, p.lo + 64));
+    }
+}
+// Address of K of the 16-key group of `key` (past the end: of the last key).
+__device__ __forceinline__ const f16* group_base(const PagedAttnArgs& a, const Item& it, const Pages& p, int key) {
+    const int k = min(key, it.kend - 1), r = (k >> a.page_shift) - it.page0 - p.lo;
+    const int id = __builtin_amdgcn_readlane(r < 64 ? p.cur.id : p.nxt.id, r & 63);
+    const uint64_t page = (uint64_t)(uint32_t)id * (uint32_t)a.page_stride;  // a page is < 2^21 elements
+    return it.base + page + ((k & ((1 << a.page_shift) - 1)) & ~15) * kHeadDim;
+}
+// Bit j: the page of keys key + 16 j .. +16 lies outside the pool.
+template <int N>
+__device__ __forceinline__ uint32_t hidden_groups(const PagedAttnArgs& a, const Item& it, const Pages& p, int key) {
+    uint32_t bits = 0;
+    if (__builtin_expect((p.cur.bad | p.nxt.bad) != 0, 0)) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int r = page_rel(a, it, key + 16 * j) - p.lo;
+            bits |= (uint32_t)((r < 64 ? p.cur.bad : p.nxt.bad) >> (r & 63) & 1) << j;
+        }
+    }
+    return bits;
+}
+// K and V of the 16-key group of `key` into kd (1 KB a step) and vd (`slab` a
+// step).
+__device__ __forceinline__ void copy_group(const PagedAttnArgs& a, const Item& it, const f16* base, const Offsets& whole,
+                                           int key, bool v, uint32_t lds, uint32_t step) {
+    if (key + 16 <= it.kend) {
+        copy4(base, v ? whole.v : whole.k, lds, step);
+    } else {
+        const int gkey = min(key, (it.kend - 1) & ~15);
+        const Offsets o = group_offsets(thread_id() & 63, key - gkey, it.kend - 1 - gkey, (uint32_t)a.kv_stride * 2);
+        copy4(base, v ? o.v : o.k, lds, step);
+    }
 }
 
 // ---- results --------------------------------------------------------------
 
-// Merge of the published ranges of a row block: 32 lanes a (row, q head)
-// column, 4 dims a lane.  Weights 2^(m_i - M), sums in range order.
-__device__ __forceinline__ void merge_splits(const PagedAttnArgs& a, const Item& it) {
-    const int tid = thread_id(), lane = tid & 31, sub = tid >> 5;
-    for (int c = sub; c < it.rows * kRep; c += kThreads / 32) {
-        const int r = c >> 1, h = c & 1;
-        const int64_t rec = ((int64_t)(it.rec + r) * a.nkvh + it.kvh) * kRep + h;
-        const int64_t step = (int64_t)it.rows * a.nkvh * kRep;  // records of a range
-        float m = kNegInf, l = 0.0f;
-        if (lane < it.splits) {
-            const float2 ml = load_dev2(a.ws_ml + (rec + lane * step) * 2);
-            m = ml.x;
-            l = ml.y;
-        }
-        float M = m;
+// The published state of a (row block, kv head, range): for each pair of dims
+// the values of all columns next to each other, 2 floats a column, so that a
+// store instruction of an MFMA accumulator (a column a lane) writes whole
+// lines; then (max, sum) of every column.  Columns: q head h of row r is 32
+// (r / 16) + h * (rows of that 16) + r % 16.
+__device__ __forceinline__ int column(const Item& it, int r, int h) {
+    return (r >> 4) * 32 + h * min(16, it.rows - (r & ~15)) + (r & 15);
+}
+__device__ __forceinline__ float* range_o(const PagedAttnArgs& a, const Item& it, int range) {
+    return a.ws_o + ((int64_t)it.rec * a.nkvh + (it.kvh * it.splits + range) * it.rows) * (kRep * kHeadDim);
+}
+__device__ __forceinline__ float* range_ml(const PagedAttnArgs& a, const Item& it, int range) {
+    return a.ws_ml + ((int64_t)it.rec * a.nkvh + (it.kvh * it.splits + range) * it.rows) * (kRep * 2);
+}
+
+// A thread's pairs of dims of a column, kFlight / SP at a time with all their
+// ranges (up to SP) in flight together; more than SP ranges in groups.
+template <int THREADS, int SP>
+__device__ __forceinline__ void merge_pairs(const float* src, int cols, int splits, const float* wt, const float* sums,
+                                            uint32_t* res, int pad) {
+    constexpr int kFlight = 16, kUnits = kFlight / SP;
+    const int units = cols * (kHeadDim / 2);
+    for (int u0 = thread_id(); u0 < units; u0 += THREADS * kUnits) {
+        float o[kUnits][2];
 #pragma unroll
-        for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 32));
-        const float w = m == kNegInf ? 0.0f : fast_exp2(m - M);
-        l *= w;
+        for (int k = 0; k < kUnits; ++k) o[k][0] = o[k][1] = 0.0f;
+        for (int i0 = 0; i0 < splits; i0 += SP) {
+            float2 x[kUnits][SP];
 #pragma unroll
-        for (int d = 16; d; d >>= 1) l += __shfl_xor(l, d, 32);
-        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        const float* src = a.ws_o + rec * kHeadDim + 4 * lane;
-        for (int i0 = 0; i0 < it.splits; i0 += 8) {
-            float2 x[8][2];
+            for (int k = 0; k < kUnits; ++k)
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const float* p = src + min(i0 + u, it.splits - 1) * step * kHeadDim;
-                x[u][0] = load_dev2(p);
-                x[u][1] = load_dev2(p + 2);
-            }
+                for (int i = 0; i < SP; ++i)
+                    x[k][i] = load_dev2(src + (min(i0 + i, splits - 1) * units + min(u0 + k * THREADS, units - 1)) * 2);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                if (i0 + u < it.splits) {
-                    const float wi = __shfl(w, i0 + u, 32);
-                    // A range without a visible key has weight 0 and zeros;
-                    // one with infinities keeps them.
-                    acc.x = fmaf(x[u][0].x, wi, acc.x);
-                    acc.y = fmaf(x[u][0].y, wi, acc.y);
-                    acc.z = fmaf(x[u][1].x, wi, acc.z);
-                    acc.w = fmaf(x[u][1].y, wi, acc.w);
+            for (int k = 0; k < kUnits; ++k) {
+                const int c = min(u0 + k * THREADS, units - 1) % cols;
+#pragma unroll
+                for (int i = 0; i < SP; ++i) {
+                    const bool on = i0 + i < splits;
+                    const float w = wt[c * splits + min(i0 + i, splits - 1)];
+                    o[k][0] = on ? fmaf(x[k][i].x, w, o[k][0]) : o[k][0];
+                    o[k][1] = on ? fmaf(x[k][i].y, w, o[k][1]) : o[k][1];
                 }
             }
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        half4v o = {(f16)(acc.x * inv), (f16)(acc.y * inv), (f16)(acc.z * inv), (f16)(acc.w * inv)};
-        *(half4v*)(a.out + ((int64_t)(it.row0 + r) * a.nkvh + it.kvh) * (kRep * kHeadDim) + h * kHeadDim +
-                   4 * lane) = o;
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+            const int u = u0 + k * THREADS, p = u / cols, c = u - p * cols;
+            if (u < units) {
+                const float inv = sums[c * splits];
+                const half2v y = {(f16)(o[k][0] * inv), (f16)(o[k][1] * inv)};
+                res[c * pad + p] = __builtin_bit_cast(uint32_t, y);
+            }
+        }
     }
 }
 
-// After this range's records are stored: the last range of the row block to
-// arrive merges them.  Called by every thread of the workgroup.
-__device__ __forceinline__ void arrive(const PagedAttnArgs& a, const Item& it, int& s_last) {
-    stores_done_barrier();
-    uint32_t* ctr = a.counters + (int64_t)it.block * a.nkvh + it.kvh;
-    if (threadIdx.x == 0) s_last = ticket_add(ctr) == (uint32_t)(it.splits - 1);
+// Merge of the published ranges of a row block.  The (max, sum) of every
+// column and range turn into weights 2^(m_i - M) in LDS; then the threads take
+// pairs of dims of a column, sums in range order.  Results pass through LDS, as
+// the columns lie in the outputs 4 KB apart.
+template <int NW>
+__device__ __forceinline__ void merge_splits(const PagedAttnArgs& a, const Item& it, Shared<NW>& sh) {
+    constexpr int kThreads = NW * 64, kPairs = kHeadDim / 2, kPad = kPairs + 4;
+    const int tid = thread_id();
+    const int cols = it.rows * kRep, splits = it.splits;
+    const float* src = range_o(a, it, 0);
+    const float* ml = range_ml(a, it, 0);
+    uint32_t* res = reinterpret_cast<uint32_t*>(sh.buf);          // [cols][kPad] pairs of f16
+    float* wt = reinterpret_cast<float*>(res + cols * kPad);      // [cols][splits]
+    float* sums = wt + cols * splits;
+    for (int e = tid; e < cols * splits; e += kThreads) {
+        const int i = e / cols, c = e - i * cols;
+        const float2 x = load_dev2(ml + e * 2);
+        wt[c * splits + i] = x.x;
+        sums[c * splits + i] = x.y;
+    }
     __syncthreads();
-    if (!s_last) return;
-    merge_splits(a, it);
+    for (int c = tid; c < cols; c += kThreads) {
+        float M = kNegInf, l = 0.0f;
+        for (int i = 0; i < splits; ++i) M = fmaxf(M, wt[c * splits + i]);
+        for (int i = 0; i < splits; ++i) {
+            const float m = wt[c * splits + i], w = m == kNegInf ? 0.0f : fast_exp2(m - M);
+            wt[c * splits + i] = w;
+            l = fmaf(sums[c * splits + i], w, l);
+        }
+        sums[c * splits] = l == 0.0f ? 0.0f : 1.0f / l;
+    }
+    __syncthreads();
+    if (splits <= 2)
+        merge_pairs<kThreads, 2>(src, cols, splits, wt, sums, res, kPad);
+    else if (splits <= 4)
+        merge_pairs<kThreads, 4>(src, cols, splits, wt, sums, res, kPad);
+    else if (splits <= 8)
+        merge_pairs<kThreads, 8>(src, cols, splits, wt, sums, res, kPad);
+    else
+        merge_pairs<kThreads, 16>(src, cols, splits, wt, sums, res, kPad);
+    __syncthreads();
+    for (int u = tid; u < cols * (kHeadDim / 8); u += kThreads) {  // 16 bytes a thread, a column 16 threads
+        const int r = u >> 5, h = (u >> 4) & 1, p = u & 15;
+        const uint4 y = *reinterpret_cast<const uint4*>(res + column(it, r, h) * kPad + 4 * p);
+        *(uint4*)(a.out + ((int64_t)(it.row0 + r) * a.nkvh + it.kvh) * (kRep * kHeadDim) + h * kHeadDim + 8 * p) = y;
+    }
+}
+
+// After this range's state is stored: the last range of the row block to
+// arrive merges them.  Called by every thread of the workgroup.
+template <int NW>
+__device__ __forceinline__ void arrive(const PagedAttnArgs& a, const Item& it, Shared<NW>& sh) {
+    stores_done_barrier();
+    uint32_t* ctr = a.counters + ((int64_t)it.block * a.nkvh + it.kvh) * kPagedCounterStep;
+    if (threadIdx.x == 0) sh.last = ticket_add(ctr) == (uint32_t)(it.splits - 1);
+    __syncthreads();
+    if (!sh.last) return;
+    merge_splits(a, it, sh);
     if (threadIdx.x == 0) ticket_reset(ctr);
 }
 
-// Record (range, row, kv head, q head) of this item.
-__device__ __forceinline__ int64_t record(const PagedAttnArgs& a, const Item& it, int r, int h) {
-    return ((int64_t)(it.rec + it.split * it.rows + r) * a.nkvh + it.kvh) * kRep + h;
-}
-
-// 16 accumulator elements of column (r, h), dims db*32 + 8*q4 + 4*g + x:
-// stored as outputs, or as the range's record.
-__device__ __forceinline__ void put_block(const PagedAttnArgs& a, const Item& it, const float16v& o, float l, int db,
-                                          int g, int r, int h) {
+// Accumulator elements 4 q0 .. +4 NQ of column (r, h): dims db*32 + 8*(q0 +
+// q) + 4*g + x; stored as outputs, or as the range's state.
+template <int NQ>
+__device__ __forceinline__ void put_block(const PagedAttnArgs& a, const Item& it, const float* o, float l, int db,
+                                          int q0, int g, int r, int h) {
     if (it.splits == 1) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         f16* dst = a.out + ((int64_t)(it.row0 + r) * a.nkvh + it.kvh) * (kRep * kHeadDim) + h * kHeadDim + db * 32;
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
+        for (int q = 0; q < NQ; ++q) {
             half4v y;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) y[x] = (f16)(o[4 * q4 + x] * inv);
-            *(half4v*)(dst + 8 * q4 + 4 * g) = y;
+            for (int x = 0; x < 4; ++x) y[x] = (f16)(o[4 * q + x] * inv);
+            *(half4v*)(dst + 8 * (q0 + q) + 4 * g) = y;
         }
     } else {
-        float* dst = a.ws_o + record(a, it, r, h) * kHeadDim + db * 32;
+        const int step = it.rows * kRep * 2;  // floats of a pair of dims
+        float* dst = range_o(a, it, it.split) + (db * 16 + 4 * q0 + 2 * g) * step + column(it, r, h) * 2;
 #pragma unroll
-        for (int q4 = 0; q4 < 4; ++q4) {
-            store_dev2(dst + 8 * q4 + 4 * g, o[4 * q4], o[4 * q4 + 1]);
-            store_dev2(dst + 8 * q4 + 4 * g + 2, o[4 * q4 + 2], o[4 * q4 + 3]);
+        for (int q = 0; q < NQ; ++q) {
+            store_dev2(dst + 4 * q * step, o[4 * q], o[4 * q + 1]);
+            store_dev2(dst + (4 * q + 1) * step, o[4 * q + 2], o[4 * q + 3]);
         }
     }
 }
 
 // NaN if some element is not finite.
-__device__ __forceinline__ float not_finite(const float16v& o) {
+template <int N>
+__device__ __forceinline__ float not_finite(const float* o) {
     float t = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t = fmaf(o[i], 0.0f, t);
+    for (int i = 0; i < N; ++i) t = fmaf(o[i], 0.0f, t);
     return t;
 }
 
-// The item again, one (row, q head) column a wave at a time, in f32 and key by
-// key: for items whose fast result is not finite.  The MFMA product weighs a
-// hidden key with 0, and 0 * inf is NaN: here hidden keys are left out, so
-// infinities and NaN reach only the rows that see them.
-__device__ __forceinline__ void exact_item(const PagedAttnArgs& a, const Item& it, int key0, int key1) {
-    const int tid = thread_id(), lane = tid & 63, wave = tid >> 6;
-    for (int c = wave; c < it.rows * kRep; c += kThreads / 64) {
-        const int r = c >> 1, h = c & 1, pos = it.pos0 + r;
-        const int64_t col = ((int64_t)(it.row0 + r) * a.nkvh + it.kvh) * (kRep * kHeadDim) + h * kHeadDim;
-        const f16* q = a.q + col;
-        float m = kNegInf, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
-        for (int k0 = key0; k0 < min(key1, pos + 1); k0 += 64) {
-            const int key = k0 + lane;
-            const int id = it.table[min(key, it.kend - 1) >> a.page_shift];
-            const bool seen = key < key1 && key <= pos && (uint32_t)id < (uint32_t)a.pages;
-            const f16* kp = a.base + (seen ? id : 0) * a.page_stride + it.kvh * a.head_stride +
-                            (key & ((1 << a.page_shift) - 1)) * kHeadDim;
-            float s = 0.0f;
-            for (int d = 0; d < kHeadDim; d += 8) {
-                H8 x, y;
-                x.u = *(const uint4*)(kp + d);
-                y.u = *(const uint4*)(q + d);
+// One column's output dims again, in f32 and key by key, by one wave: for
+// states that are not finite.  The MFMA product weighs a hidden key with 0,
+// and 0 * inf is NaN: here hidden keys are left out, so infinities and NaN
+// reach only the rows that see them.  The weights are taken against the max
+// that the state has; lane l < 32 returns dim 32 db + l of row r, q head h.
+__device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& it, int key0, int key1, float M, int r,
+                                            int h, int db, int lane) {
+    const int pos = it.pos0 + r;
+    const f16* q = a.q + ((int64_t)(it.row0 + r) * a.nkvh + it.kvh) * (kRep * kHeadDim) + h * kHeadDim;
+    float o = 0.0f;
+    for (int k0 = key0; k0 < min(key1, pos + 1); k0 += 64) {
+        const int key = k0 + lane;
+        const int id = it.table[min(key, it.kend - 1) >> a.page_shift];
+        const bool seen = key < key1 && key <= pos && (uint32_t)id < (uint32_t)a.pages;
+        const uint64_t row = (uint64_t)(uint32_t)(seen ? id : 0) * (uint32_t)a.page_stride +
+                             (key & ((1 << a.page_shift) - 1)) * kHeadDim;
+        float s = 0.0f;
+        for (int d = 0; d < kHeadDim; d += 8) {
+            H8 x, y;
+            x.u = *(const uint4*)(it.base + row + d);
+            y.u = *(const uint4*)(q + d);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s = fmaf(h2f(x.e[e]), h2f(y.e[e]), s);
-            }
-            s = seen ? s * a.scale_log2 : kNegInf;
-            float top = s;
-#pragma unroll
-            for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-            const float mn = fmaxf(m, top);
-            const float mu = mn == kNegInf ? 0.0f : mn;
-            const float alpha = m == kNegInf ? 0.0f : fast_exp2(m - mu);
-            const float p = seen ? fast_exp2(s - mu) : 0.0f;
-            m = mn;
-            float ps = p;
-#pragma unroll
-            for (int d = 32; d; d >>= 1) ps += __shfl_xor(ps, d);
-            l = l * alpha + ps;
-            o0 *= alpha;
-            o1 *= alpha;
-            uint64_t todo = __ballot(seen);
-            while (todo) {
-                const int j = __builtin_ctzll(todo);
-                todo &= todo - 1;
-                const f16* vp = a.base + (int64_t)__shfl(id, j) * a.page_stride + it.kvh * a.head_stride +
-                                a.kv_stride + ((k0 + j) & ((1 << a.page_shift) - 1)) * kHeadDim + 2 * lane;
-                const float pj = __shfl(p, j);
-                o0 = fmaf(pj, h2f(vp[0]), o0);
-                o1 = fmaf(pj, h2f(vp[1]), o1);
-            }
+            for (int e = 0; e < 8; ++e) s = fmaf(h2f(x.e[e]), h2f(y.e[e]), s);
         }
-        if (it.splits == 1) {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            a.out[col + 2 * lane] = f2h(o0 * inv);
-            a.out[col + 2 * lane + 1] = f2h(o1 * inv);
-        } else {
-            const int64_t rec = record(a, it, r, h);
-            store_dev2(a.ws_o + rec * kHeadDim + 2 * lane, o0, o1);
-            if (lane == 0) store_dev2(a.ws_ml + rec * 2, m, l);
+        const float p = fast_exp2(s * a.scale_log2 - M);
+        uint64_t todo = __ballot(seen);
+        while (todo) {
+            const int j = __builtin_ctzll(todo);
+            todo &= todo - 1;
+            const uint64_t at = (uint64_t)__shfl((int)(uint32_t)(row >> 32), j) << 32 |
+                                (uint32_t)__shfl((int)(uint32_t)row, j);
+            o = fmaf(__shfl(p, j), h2f(it.base[at + a.kv_stride + 32 * db + (lane & 31)]), o);
         }
+    }
+    return o;
+}
+// Puts the columns of a wave whose dim block db (32 dims) is not finite.
+// every lane: its column's max and sum; valid columns only.
+__device__ __forceinline__ void put_exact(const PagedAttnArgs& a, const Item& it, int key0, int key1, float M, float L,
+                                          int db, int r, int h, bool valid) {
+    const int lane = thread_id() & 63;
+    uint64_t todo = __ballot(valid) & 0xffffffffu;  // a lane a column: those of g = 0
+    while (todo) {
+        const int j = __builtin_ctzll(todo);
+        todo &= todo - 1;
+        const int rj = __shfl(r, j), hj = __shfl(h, j);
+        const float l = __shfl(L, j);
+        const float o = exact_dims(a, it, key0, key1, __shfl(M, j), rj, hj, db, lane);
+        if (lane >= 32) continue;
+        if (it.splits == 1)
+            a.out[((int64_t)(it.row0 + rj) * a.nkvh + it.kvh) * (kRep * kHeadDim) + hj * kHeadDim + db * 32 + lane] =
+                f2h(l == 0.0f ? 0.0f : o / l);
+        else
+            store_dev(range_o(a, it, it.split) + (db * 16 + (lane >> 1)) * it.rows * kRep * 2 +
+                          column(it, rj, hj) * 2 + (lane & 1),
+                      o);
     }
 }
 
 // ---- the two kinds of item ------------------------------------------------
-
-struct Shared {
-    f16 buf[kBufHalves];
-    float ml[4][2][64];
-    int last;
-};
 
 // This lane's query column (row rin of the block, q head h): its Q^T operand
 // straight from memory, its position and the empty softmax state.
@@ -332,237 +405,391 @@ __device__ __forceinline__ void init_wave(Wave& w, const PagedAttnArgs& a, const
     w.l = 0.0f;
     operand_addrs(w, lane);
 }
+// Every load and copy so far has landed, Q among them.  The registers are
+// named here, once: else the compiler, which does not count the copies, waits
+// for Q inside the tile loop, and so for every copy in flight.
+__device__ __forceinline__ void wait_q(Wave& w) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) asm volatile("" : "+v"(w.qb[ks]));
+}
+
+// Marks what the fast path hardly ever takes: the compiler then lays it out
+// away from it.  A launch starts with a cold instruction cache, so that short
+// items cost about what their code's lines cost to fetch.
+__device__ __forceinline__ bool rarely(bool x) { return __builtin_expect(x, 0); }
+
+// Scores of keys past the row's position out of the way: element i of block
+// kb is key k0 + 32 kb + 4 g + 8 (i / 4) + i % 4.
+template <int NB>
+__device__ __forceinline__ void mask_scores(const Wave& w, float16v (&s)[NB], int k0) {
+    const int last = w.qpos - k0 - 4 * w.g;
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = 32 * kb + 8 * (i >> 2) + (i & 3) > last ? kNegInf : s[kb][i];
+}
+// And of the 16-key groups whose bit is set in `hidden`.
+template <int NB>
+__device__ __forceinline__ void hide_scores(float16v (&s)[NB], uint32_t hidden) {
+#pragma unroll
+    for (int j = 0; j < 2 * NB; ++j)
+        if (hidden >> j & 1)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[j >> 1][8 * (j & 1) + i] = kNegInf;
+}
+
+// The running maximum moves when a score passes it by more than the slack.
+template <int NB>
+__device__ __forceinline__ void move_max(Wave& w, const float16v (&s)[NB]) {
+    float mx = kNegInf;
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
+    mx = halves_max(mx) * w.scale_log2;
+    const bool up = mx > w.m + kRescaleSlack;
+    if (__ballot(up)) {
+        if (rarely(__ballot(up && w.m != kNegInf))) {  // not at the first keys
+            const float alpha = !up ? 1.0f : w.m == kNegInf ? 0.0f : fast_exp2(w.m - mx);
+#pragma unroll
+            for (int db = 0; db < 4; ++db) w.o[db] *= alpha;
+            w.l *= alpha;
+        }
+        w.m = up ? mx : w.m;
+    }
+}
+
+// The weights of a step's scores, as P^T (f16, B-operand layout), and their
+// row sum: of the rounded values, so that a rounding shifts weight between
+// keys and does not scale the row.  Four sums of v_fma_mix_f32, which runs
+// beside another wave's MFMAs; v_dot2_f32_f16 does not (MFMA and VALU work of
+// two waves a SIMD: no overlap with it, about half of the smaller part
+// without).
+template <int NB>
+__device__ __forceinline__ void weights(Wave& w, const float16v (&s)[NB], half8v (&pb)[2 * NB]) {
+    const float mu = w.m == kNegInf ? 0.0f : w.m;
+    float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w4 = 0; w4 < 2 * NB; ++w4) {
+        union {
+            half8v h;
+            uint32_t u[4];
+        } p;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p.h[j] = (f16)softmax_w_raw(s[w4 >> 1][8 * (w4 & 1) + j], w.scale_log2, mu);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            asm("v_fma_mix_f32 %0, 1.0, %1, %0 op_sel_hi:[0,1,0]" : "+v"(ps[j]) : "v"(p.u[j]));
+            asm("v_fma_mix_f32 %0, 1.0, %1, %0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "+v"(ps[j]) : "v"(p.u[j]));
+        }
+        pb[w4] = p.h;
+    }
+    w.l += halves_sum((ps[0] + ps[1]) + (ps[2] + ps[3]));
+}
 
 #define WAIT_VM(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
 
-__device__ __forceinline__ void narrow_item(const PagedAttnArgs& a, const Item& it, Shared& sh) {
+// The matrix products of a step.  Operand reads run kAhead products ahead of
+// their MFMA: reads and MFMAs stay in this order (vector and scalar work may
+// move between them), else each MFMA waits out its own read's latency.
+constexpr int kAhead = 3;
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x406); }  // VALU, SALU, exp may cross
+
+// S^T of K rows kt[0 .. 32 NB - 1], keys kb*32 + (8*(i/4) + 4*g + i%4) x query
+// n.
+template <int NB>
+__device__ __forceinline__ void scores(const Wave& w, const f16* kt, float16v (&s)[NB]) {
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb) s[kb] = (float16v){};
+    half8v ka[8 * NB];
+    auto read = [&](int x) { ka[x] = *(const half8v*)&kt[(x % NB) * 32 * kHeadDim + w.kaddr[x / NB]]; };
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) read(x);
+    keep_order();
+#pragma unroll
+    for (int x = 0; x < 8 * NB; ++x) {
+        if (x + kAhead < 8 * NB) read(x + kAhead);
+        keep_order();
+        s[x % NB] = mfma32(ka[x], w.qb[x / NB], s[x % NB]);
+        keep_order();
+    }
+}
+
+// O^T += V^T P^T with V rows vt[0 .. 32 NB - 1] of a tile of ROWS rows.
+template <int ROWS, int NB>
+__device__ __forceinline__ void product(Wave& w, const f16* vt, const half8v (&pb)[2 * NB]) {
+    half4v lo[8 * NB], hi[8 * NB];
+    auto read = [&](int x) {
+        const f16* vp = vt + w.vbase + (x & 3) * (ROWS * 32) + (x >> 2) * 16 * 32;
+        lo[x] = read_tr(vp);
+        hi[x] = read_tr(vp + 8 * 32);
+    };
+#pragma unroll
+    for (int x = 0; x < kAhead; ++x) read(x);
+    keep_order();
+#pragma unroll
+    for (int x = 0; x < 8 * NB; ++x) {
+        if (x + kAhead < 8 * NB) read(x + kAhead);
+        keep_order();
+        const half8v va = __builtin_shufflevector(lo[x], hi[x], 0, 1, 2, 3, 4, 5, 6, 7);
+        w.o[x & 3] = mfma32(va, pb[x >> 2], w.o[x & 3]);
+        keep_order();
+    }
+}
+
+// The state of column lane & 31 that the waves j0, j0 + dj, .. (N of them)
+// left in LDS: dims' elements e0 .. e0 + NE, each wave's weighed by 2^(m_j -
+// M), in wave order.  Wave j's elements lie at buf + j * 16 KB: element e of
+// lane l at (e / 4) * 256 + 4 l + e % 4.
+template <int N, int NE, int NW>
+__device__ __forceinline__ void combine(const Shared<NW>& sh, int j0, int dj, int e0, int lane, float (&o)[NE], float& M,
+                                        float& L) {
+    float4 x[N][NE / 4];
+    float mj[N], lj[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        mj[j] = sh.ml[j0 + j * dj][0][lane];
+        lj[j] = sh.ml[j0 + j * dj][1][lane];
+        const float4* src = reinterpret_cast<const float4*>(sh.buf) + (j0 + j * dj) * 1024 + e0 * 16 + lane;
+#pragma unroll
+        for (int q = 0; q < NE / 4; ++q) x[j][q] = src[q * 64];
+    }
+    keep_order();  // every read is on its way before the first is waited for
+    M = mj[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) M = fmaxf(M, mj[j]);
+    L = 0.0f;
+#pragma unroll
+    for (int e = 0; e < NE; ++e) o[e] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float aj = mj[j] == kNegInf ? 0.0f : fast_exp2(mj[j] - M);
+        L = fmaf(lj[j], aj, L);
+#pragma unroll
+        for (int q = 0; q < NE / 4; ++q) {
+            o[4 * q] = fmaf(x[j][q].x, aj, o[4 * q]);
+            o[4 * q + 1] = fmaf(x[j][q].y, aj, o[4 * q + 1]);
+            o[4 * q + 2] = fmaf(x[j][q].z, aj, o[4 * q + 2]);
+            o[4 * q + 3] = fmaf(x[j][q].w, aj, o[4 * q + 3]);
+        }
+    }
+}
+// A wave leaves its state for combine(): 16 accumulator elements of NDB dim
+// blocks from db0 on.
+template <int NDB, int NW>
+__device__ __forceinline__ void leave(Shared<NW>& sh, const Wave& w, int wave, int db0, int lane) {
+    float4* dst = reinterpret_cast<float4*>(sh.buf) + wave * 1024 + lane;
+#pragma unroll
+    for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float16v& o = w.o[db0 + db];
+            dst[((db0 + db) * 4 + q) * 64] = make_float4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+        }
+}
+
+__device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it, Pages pg, Shared<kNarrowWaves>& sh) {
     const int tid = thread_id(), lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n = lane & 31, h = n >> 4, rin = n & 15;
     f16* kbuf = sh.buf + wave * (2 * kSlice * kHeadDim);
     f16* vbuf = kbuf + kSlice * kHeadDim;
+    const Offsets whole = group_offsets(lane, 0, 15, (uint32_t)a.kv_stride * 2);
 
-    // Lane l of a Pages: group l & 1 of this wave's slice of tile tp + l / 2.
-    int tp = it.tile0;
-    const int lane_key = (lane >> 1) * kNarrowTile + wave * kSlice + 16 * (lane & 1);
-    Pages pg = load_pages(a, it, tp * kNarrowTile + lane_key);
-    Pages next = load_pages(a, it, (tp + 32) * kNarrowTile + lane_key);
-    Wave w;
-    init_wave(w, a, it, rin, h, lane);
-    const Offsets whole = group_offsets(lane);
-    check_pages(a, pg);
-
-    // Copies of group p (0, 1) of the slice of tile t: its K or its V.
-    auto copy_group = [&](int t, int p, bool v) {
-        const int key = t * kNarrowTile + wave * kSlice + 16 * p;
-        const int id = __builtin_amdgcn_readlane(pg.id, 2 * (t - tp) + p);
-        const int gkey = min(key, (it.kend - 1) & ~15);
-        const f16* base = group_base(a, it.kvh, id, gkey) + (v ? a.kv_stride : 0);
-        const uint32_t lds = v ? lds_addr(vbuf) + p * 1024 : lds_addr(kbuf) + p * 4096;
-        if (key + 16 <= it.kend) {
-            if (v)
-                copy_v(base, whole, lds, kSlice * 64);
-            else
-                copy_k(base, whole, lds);
-        } else if (v) {
-            copy_v_tail(base, key - gkey, it.kend - 1 - gkey, lds, kSlice * 64);
-        } else {
-            copy_k_tail(base, key - gkey, it.kend - 1 - gkey, lds);
+    // Copies of the slice of tile t: its K or its V.
+    auto copy_slice = [&](int t, bool v) {
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const int key = t * kNarrowTile + wave * kSlice + 16 * p;
+            const uint32_t lds = v ? lds_addr(vbuf) + p * 1024 : lds_addr(kbuf) + p * 4096;
+            copy_group(a, it, group_base(a, it, pg, key), whole, key, v, lds, v ? kSlice * 64 : 1024);
         }
     };
-    auto copy_slice = [&](int t, bool v) {
-        copy_group(t, 0, v);
-        copy_group(t, 1, v);
-    };
-    const int last_pos = it.pos0 + it.rows - 1;  // == kend - 1
+    Wave w;
+    init_wave(w, a, it, rin, h, lane);
     if (it.tile0 < it.tile1) {
         copy_slice(it.tile0, false);
         copy_slice(it.tile0, true);
     }
+    wait_q(w);
     for (int t = it.tile0; t < it.tile1; ++t) {
         const int k0 = t * kNarrowTile + wave * kSlice;
         const bool more = t + 1 < it.tile1;
-        const uint32_t bad = (uint32_t)(pg.bad >> (2 * (t - tp))) & 3;
-        if (more && t + 1 - tp == 32) {
-            tp += 32;
-            pg = next;
-            check_pages(a, pg);
-            next = load_pages(a, it, (tp + 32) * kNarrowTile + lane_key);
-        }
-        if (k0 > last_pos) {  // only a wave's slice of the last tile: nothing to see
+        const uint32_t hidden = hidden_groups<2>(a, it, pg, k0);
+        if (more) advance_pages(a, it, pg, k0 + kNarrowTile);
+        if (k0 >= it.kend) {  // a wave's slice of the last tile: nothing to see
             WAIT_VM(0);
             break;
         }
         WAIT_VM(8);  // K landed, V in flight
         float16v s[1];
         half8v pb[2];
-        step_scores<1>(w, kbuf, s);
+        scores<1>(w, kbuf, s);
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             copy_slice(t + 1, false);
         }
-        if (k0 + kSlice - 1 <= it.pos0 && !bad)
-            step_softmax<false, 1>(w, s, k0, 0u, pb);
-        else
-            step_softmax<true, 1>(w, s, k0, bad, pb);
+        if (k0 + kSlice - 1 > it.pos0) mask_scores<1>(w, s, k0);
+        if (rarely(hidden)) hide_scores<1>(s, hidden);
+        move_max<1>(w, s);
+        weights<1>(w, s, pb);
         if (more)
             WAIT_VM(8);
         else
             WAIT_VM(0);
-        step_pv<kSlice, 1>(w, vbuf, pb);
+        product<kSlice, 1>(w, vbuf, pb);
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             copy_slice(t + 1, true);
         }
     }
 
-    // The four waves' states combine: wave w finishes dim block w, the other
-    // blocks pass through each wave's own (now free) slice buffer.
-    float* mine = reinterpret_cast<float*>(kbuf);
-#pragma unroll
-    for (int db = 0; db < 4; ++db)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mine[db * 1024 + i * 64 + lane] = w.o[db][i];
+    // The waves' states combine: wave w finishes dim block w, out of each
+    // wave's own (now free) slice buffer.
+    const bool valid = rin < it.rows;
+    if (valid) {
+        leave<4>(sh, w, wave, 0, lane);
+        sh.ml[wave][0][lane] = w.m;
+        sh.ml[wave][1][lane] = w.l;
+    }
+    __syncthreads();
+    float o[16], M = 0.0f, L = 0.0f, t = 0.0f;
+    if (valid) {
+        combine<kNarrowWaves, 16>(sh, 0, 1, 16 * wave, lane, o, M, L);
+        t = not_finite<16>(o) + 0.0f * L;
+    }
+    if (rarely(__ballot(t != t)))
+        put_exact(a, it, it.tile0 * kNarrowTile, min(it.tile1 * kNarrowTile, it.kend), M, L, wave, rin, h, valid);
+    else if (valid)
+        put_block<4>(a, it, o, L, wave, 0, w.g, rin, h);
+    if (it.splits > 1 && valid && wave == 0 && w.g == 0) store_dev2(range_ml(a, it, it.split) + column(it, rin, h) * 2, M, L);
+    if (it.splits > 1) arrive(a, it, sh);
+}
+
+__device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it, Pages pg, Shared<kWideWaves>& sh) {
+    const int tid = thread_id(), lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rw = wave & 3, kg = wave >> 2;  // 16 rows; 64 keys of every tile
+    const int n = lane & 31, h = n >> 4, rin = rw * 16 + (n & 15);
+    constexpr int kTile = kWideTile * kHeadDim, kGroup = kWideTile / 2;
+    const Offsets whole = group_offsets(lane, 0, 15, (uint32_t)a.kv_stride * 2);
+
+    // This wave's 16 keys of tile t into buffer t & 1: K, then V in slabs.
+    auto copy_tile = [&](int t) {
+        const int key = t * kWideTile + wave * 16;
+        const f16* base = group_base(a, it, pg, key);
+        const uint32_t lds = lds_addr(sh.buf) + (t & 1) * (4 * kTile);
+        copy_group(a, it, base, whole, key, false, lds + wave * 4096, 1024);
+        copy_group(a, it, base, whole, key, true, lds + 2 * kTile + wave * 1024, kWideTile * 64);
+    };
+    Wave w;
+    init_wave(w, a, it, rin, h, lane);
+    if (it.tile0 < it.tile1) copy_tile(it.tile0);
+    const int first_pos = it.pos0 + rw * 16;
+    const int last_pos = it.pos0 + min(rw * 16 + 15, it.rows - 1);
+    const bool live = rw * 16 < it.rows;
+    wait_q(w);
+    for (int t = it.tile0; t < it.tile1; ++t) {
+        WAIT_VM(0);
+        __syncthreads();  // tile t is here, and the other buffer is read
+        const int k0 = t * kWideTile + kg * kGroup;
+        const uint32_t hidden = hidden_groups<4>(a, it, pg, k0);
+        if (t + 1 < it.tile1) {
+            advance_pages(a, it, pg, (t + 1) * kWideTile);
+            copy_tile(t + 1);
+        }
+        if (!live || k0 > last_pos) continue;
+        const f16* kt = sh.buf + (t & 1) * 2 * kTile + kg * kGroup * kHeadDim;
+        float16v s[2];
+        half8v pb[4];
+        scores<2>(w, kt, s);
+        if (k0 + kGroup - 1 > first_pos) mask_scores<2>(w, s, k0);
+        if (rarely(hidden)) hide_scores<2>(s, hidden);
+        move_max<2>(w, s);
+        weights<2>(w, s, pb);
+        product<kWideTile, 2>(w, sh.buf + (t & 1) * 2 * kTile + kTile + kg * kGroup * 32, pb);
+    }
+    __syncthreads();  // the buffers are read
+    // The two key groups of a row wave combine: each leaves its state and
+    // finishes two dim blocks.
+    const bool valid = rin < it.rows;
+    leave<4>(sh, w, wave, 0, lane);
     sh.ml[wave][0][lane] = w.m;
     sh.ml[wave][1][lane] = w.l;
     __syncthreads();
-    float M = kNegInf, L = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) M = fmaxf(M, sh.ml[j][0][lane]);
-    float16v o = (float16v){};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float mj = sh.ml[j][0][lane];
-        const float aj = mj == kNegInf ? 0.0f : fast_exp2(mj - M);
-        L = fmaf(sh.ml[j][1][lane], aj, L);
-        const float* src = reinterpret_cast<const float*>(sh.buf) + j * 4096 + wave * 1024;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = fmaf(src[i * 64 + lane], aj, o[i]);
+    float o[16], M, L;
+#pragma unroll 1
+    for (int db = 2 * kg; db < 2 * kg + 2; ++db) {
+        combine<2, 16>(sh, rw, 4, db * 16, lane, o, M, L);
+        const float t = not_finite<16>(o) + 0.0f * L;
+        if (rarely(__ballot(valid && t != t)))
+            put_exact(a, it, it.tile0 * kWideTile, min(it.tile1 * kWideTile, it.kend), M, L, db, rin, h, valid);
+        else if (valid)
+            put_block<4>(a, it, o, L, db, 0, w.g, rin, h);
     }
-    const bool valid = rin < it.rows;
-    const float t = not_finite(o);
-    if (__syncthreads_or(valid && (t != t || L != L))) {
-        exact_item(a, it, it.tile0 * kNarrowTile, min(it.tile1 * kNarrowTile, it.kend));
-    } else if (valid) {
-        put_block(a, it, o, L, wave, w.g, rin, h);
-        if (it.splits > 1 && wave == 0 && w.g == 0) store_dev2(a.ws_ml + record(a, it, rin, h) * 2, M, L);
-    }
-    if (it.splits > 1) arrive(a, it, sh.last);
+    if (it.splits > 1 && valid && kg == 0 && w.g == 0) store_dev2(range_ml(a, it, it.split) + column(it, rin, h) * 2, M, L);
+    if (it.splits > 1) arrive(a, it, sh);
 }
 
-__device__ __forceinline__ void wide_item(const PagedAttnArgs& a, const Item& it, Shared& sh) {
-    const int tid = thread_id(), lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = lane & 31, h = n >> 4, rin = wave * 16 + (n & 15);
-    constexpr int kTile = kWideTile * kHeadDim;
-
-    // Lane l of a Pages: group l & 3 of tile tp + l / 4.
-    int tp = it.tile0;
-    const int lane_key = lane * 16;
-    Pages pg = load_pages(a, it, tp * kWideTile + lane_key);
-    Pages next = load_pages(a, it, (tp + 16) * kWideTile + lane_key);
-    Wave w;
-    init_wave(w, a, it, rin, h, lane);
-    const Offsets whole = group_offsets(lane);
-    check_pages(a, pg);
-
-    // This wave's 16 keys of tile t into buffer b: K 16 KB, V 4 slabs.
-    auto copy_tile = [&](int t, int b) {
-        const int key = t * kWideTile + wave * 16;
-        const int id = __builtin_amdgcn_readlane(pg.id, 4 * (t - tp) + wave);
-        const int gkey = min(key, (it.kend - 1) & ~15);
-        const f16* base = group_base(a, it.kvh, id, gkey);
-        const uint32_t kd = lds_addr(sh.buf + b * 2 * kTile) + wave * 4096;
-        const uint32_t vd = lds_addr(sh.buf + b * 2 * kTile + kTile) + wave * 1024;
-        if (key + 16 <= it.kend) {
-            copy_k(base, whole, kd);
-            copy_v(base + a.kv_stride, whole, vd, kWideTile * 64);
-        } else {
-            copy_k_tail(base, key - gkey, it.kend - 1 - gkey, kd);
-            copy_v_tail(base + a.kv_stride, key - gkey, it.kend - 1 - gkey, vd, kWideTile * 64);
-        }
-    };
-    const int first_pos = it.pos0 + wave * 16;
-    const int last_pos = it.pos0 + min(wave * 16 + 15, it.rows - 1);
-    const bool live = wave * 16 < it.rows;
-    if (it.tile0 < it.tile1) copy_tile(it.tile0, 0);
-    auto run = [&](int t, int b) {
-        WAIT_VM(0);
-        __syncthreads();  // tile t is here, and the other buffer is read
-        const uint32_t bad = (uint32_t)(pg.bad >> (4 * (t - tp))) & 15;
-        if (t + 1 < it.tile1) {
-            if (t + 1 - tp == 16) {
-                tp += 16;
-                pg = next;
-                check_pages(a, pg);
-                next = load_pages(a, it, (tp + 16) * kWideTile + lane_key);
-            }
-            copy_tile(t + 1, b ^ 1);
-        }
-        const int k0 = t * kWideTile;
-        if (!live || k0 > last_pos) return;
-        const f16* kt = sh.buf + b * 2 * kTile;
-        float16v s[2];
-        half8v pb[4];
-        step_scores<2>(w, kt, s);
-        if (k0 + kWideTile - 1 <= first_pos && !bad)
-            step_softmax<false, 2>(w, s, k0, 0u, pb);
-        else
-            step_softmax<true, 2>(w, s, k0, bad, pb);
-        step_pv<kWideTile, 2>(w, kt + kTile, pb);
-    };
-    for (int t = it.tile0; t < it.tile1; t += 2) {
-        run(t, 0);
-        if (t + 1 < it.tile1) run(t + 1, 1);
-    }
-    const bool valid = rin < it.rows;
-    float t = 0.0f;
-#pragma unroll
-    for (int db = 0; db < 4; ++db) t += not_finite(w.o[db]);
-    if (__syncthreads_or(valid && (t != t || w.l != w.l))) {
-        exact_item(a, it, it.tile0 * kWideTile, min(it.tile1 * kWideTile, it.kend));
-    } else if (valid) {
-#pragma unroll
-        for (int db = 0; db < 4; ++db) put_block(a, it, w.o[db], w.l, db, w.g, rin, h);
-        if (it.splits > 1 && w.g == 0) store_dev2(a.ws_ml + record(a, it, rin, h) * 2, w.m, w.l);
-    }
-    if (it.splits > 1) arrive(a, it, sh.last);
-}
-
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_kernel(
+template <int NW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_kernel(
     PagedAttnArgs a) {
-    __shared__ __attribute__((aligned(1024))) Shared sh;
-    const int items = a.n_items[0] * a.nkvh;
+    __shared__ __attribute__((aligned(1024))) Shared<NW> sh;
+    constexpr bool kWide = NW == kWideWaves;
+    const PagedItem* list = kWide ? a.wide : a.narrow;
+    const int last_item = (kWide ? a.max_wide : a.max_narrow) - 1;
+    // Every lane reads a word of the item's record; the next item's is
+    // requested when this one starts.
+    auto load_item = [&](int i) {
+        return reinterpret_cast<const int*>(list + min(i / a.nkvh, last_item))[thread_id() & 63];
+    };
+    int words = load_item(blockIdx.x);
+    const int items = a.n_items[kWide] * a.nkvh;
     for (int i = blockIdx.x; i < items; i += gridDim.x) {
-        const PagedItem p = a.items[i / a.nkvh];
+        auto word = [&](int k) { return __builtin_amdgcn_readlane(words, k); };
         Item it;
         it.kvh = i % a.nkvh;
-        it.row0 = p.row0;
-        it.rows = min(p.shape & 0xff, a.rows - p.row0);  // rows past the caller's q are left out
-        it.pos0 = p.pos0;
-        it.kend = p.pos0 + it.rows;
-        it.tile0 = p.tile0;
-        it.tile1 = p.tile1;
-        it.splits = (p.shape >> 8) & 0xff;
-        it.split = (p.shape >> 16) & 0xff;
-        it.rec = p.rec;
-        it.block = p.block;
-        it.table = a.table + (int64_t)p.req * a.stride;
+        const int shape = word(3);
+        it.row0 = word(1);
+        it.rows = min(shape & 0xff, a.rows - it.row0);  // rows past the caller's q are left out
+        it.pos0 = word(2);
+        it.kend = it.pos0 + it.rows;
+        it.tile0 = word(4);
+        it.tile1 = word(5);
+        it.splits = (shape >> 8) & 0xff;
+        it.split = (shape >> 16) & 0xff;
+        it.rec = word(6);
+        it.block = word(7);
+        it.page0 = word(8);
+        it.last_page = (it.kend - 1) >> a.page_shift;
+        it.table = a.table + (int64_t)word(0) * a.stride;
+        it.base = a.base + it.kvh * a.head_stride;
+        Pages pg;
+        pg.cur = check_pages(a, words);
+        pg.cur.bad &= ~0ull << kPagedItemHead;  // the header's lanes are no pages
+        pg.lo = -kPagedItemHead;
+        if (i + (int)gridDim.x < items) words = load_item(i + gridDim.x);
         if (it.rows <= 0) continue;
-        if (p.shape >> 24)
-            wide_item(a, it, sh);
-        else
-            narrow_item(a, it, sh);
+        pg.nxt = {0, 0};
+        if (it.last_page - it.page0 >= kPagedItemPages) pg.nxt = check_pages(a, load_pages(it, kPagedItemPages));
+        run_item(a, it, pg, sh);
         __syncthreads();  // the next item reuses the LDS
     }
 }
 
 }  // namespace
 
-hipError_t launch_paged_attn(const PagedAttnArgs& a, int64_t max_items, int cus, hipStream_t stream) {
+hipError_t launch_paged_attn(const PagedAttnArgs& a, int cus, hipStream_t stream) {
     if (a.rows <= 0) return hipSuccess;
-    const int64_t wgs = std::min<int64_t>(max_items * a.nkvh, 2 * (int64_t)cus);
-    hipLaunchKernelGGL(paged_attn_kernel, dim3((unsigned)wgs), dim3(kThreads), 0, stream, a);
+    if (a.max_wide > 0) {
+        const int64_t wgs = std::min<int64_t>((int64_t)a.max_wide * a.nkvh, cus);
+        hipLaunchKernelGGL(paged_attn_kernel<kWideWaves>, dim3((unsigned)wgs), dim3(kWideWaves * 64), 0, stream, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    const int64_t wgs = std::min<int64_t>((int64_t)a.max_narrow * a.nkvh, 2 * (int64_t)cus);
+    hipLaunchKernelGGL(paged_attn_kernel<kNarrowWaves>, dim3((unsigned)wgs), dim3(kNarrowWaves * 64), 0, stream, a);
     return hipGetLastError();
 }
 

@@ -81,7 +81,7 @@ __device__ __forceinline__ int find(const int* s, int n, int x) {
 __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PagedPlanArgs a) {
     __shared__ uint64_t s_wave[3][kWavesN];
     __shared__ int s_row[kThreads], s_len[kThreads], s_new[kThreads], s_page[kThreads];
-    __shared__ int s_item[kThreads], s_rec[kThreads], s_block[kThreads], s_gone[kThreads];
+    __shared__ int s_narrow[kThreads], s_wide[kThreads], s_rec[kThreads], s_block[kThreads], s_gone[kThreads];
     __shared__ int s_last;
 
     const int tid = threadIdx.x, ps = 1 << a.page_shift, sh = a.page_shift;
@@ -128,19 +128,21 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PagedPlanArgs a) {
 
     PagedShape shape{0, 0, 0};
     if (placed) shape = paged_shape(len, want);
-    Sums v{{pack2(shape.blocks * shape.splits, shape.blocks),
-            pack2(shape.splits > 1 ? want * shape.splits : 0, placed ? need : 0), pack2(gone ? held : 0, 0)}};
+    const int my_items = shape.blocks * shape.splits;
+    Sums v{{pack2(shape.wide ? 0 : my_items, shape.wide ? my_items : 0),
+            pack2(shape.splits > 1 ? want * shape.splits : 0, shape.blocks), pack2(gone ? held : 0, placed ? need : 0)}};
     Sums t;
     block_scan<3>(v.v, t.v, s_wave);
     s_row[tid] = row0;
     s_len[tid] = len;
     s_new[tid] = placed ? want : 0;
     s_page[tid] = page0;
-    s_item[tid] = lo32(v.v[0]);
-    s_block[tid] = hi32(v.v[0]);
+    s_narrow[tid] = lo32(v.v[0]);
+    s_wide[tid] = hi32(v.v[0]);
     s_rec[tid] = lo32(v.v[1]);
+    s_block[tid] = hi32(v.v[1]);
     s_gone[tid] = lo32(v.v[2]);
-    const int items = lo32(t.v[0]), taken = hi32(t.v[1]), back = lo32(t.v[2]);
+    const int narrow = lo32(t.v[0]), wide = hi32(t.v[0]), back = lo32(t.v[2]), taken = hi32(t.v[2]);
     if (blockIdx.x == 0) {
         if (mine) {
             a.status[tid] = status;
@@ -148,7 +150,8 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PagedPlanArgs a) {
         }
         if (tid == 0) {
             a.row_start[a.nreq] = nrows;
-            a.n_items[0] = items;
+            a.n_items[0] = narrow;
+            a.n_items[1] = wide;
         }
     }
     // Every load of what may alias an output has returned (the sums need
@@ -160,22 +163,22 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PagedPlanArgs a) {
     __syncthreads();
 
     const int n = a.nreq, step = gridDim.x * kThreads, first = blockIdx.x * kThreads + tid;
-    // Row maps: the page of a position is the table's, or a fresh one.
+    // Page at place j of request i's table: the table's, or a fresh one.
+    auto page_at = [&](int i, int j) {
+        const int had = (s_len[i] + ps - 1) >> sh;
+        if (j < had || !a.ring) return a.table[(int64_t)i * a.stride + j];
+        int k = head + s_page[i] + j - had;  // < 2 pages: at most `free` taken
+        k -= k >= a.pages ? a.pages : 0;
+        return a.ring[k];
+    };
+    // Row maps.
     for (int r = first; r < a.max_rows; r += step) {
         int pos = -1, slot = -1;
         if (r < nrows) {
             const int i = find(s_row, n, r), at = r - s_row[i];
             if (at < s_new[i]) {
                 pos = s_len[i] + at;
-                const int j = pos >> sh, had = (s_len[i] + ps - 1) >> sh;
-                int page;
-                if (j < had || !a.ring) {
-                    page = a.table[(int64_t)i * a.stride + j];
-                } else {
-                    int k = head + s_page[i] + j - had;  // < 2 pages: at most `free` taken
-                    k -= k >= a.pages ? a.pages : 0;
-                    page = a.ring[k];
-                }
+                const int page = page_at(i, pos >> sh);
                 slot = (uint32_t)page < (uint32_t)a.pages ? (page << sh) + (pos & (ps - 1)) : -1;
             }
         }
@@ -189,24 +192,34 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PagedPlanArgs a) {
         w -= w >= a.pages ? a.pages : 0;
         a.table[(int64_t)i * a.stride + ((s_len[i] + ps - 1) >> sh) + k - s_page[i]] = a.ring[w];
     }
-    // Work items.
-    for (int k = first; k < items; k += step) {
-        const int i = find(s_item, n, k), l = s_len[i], m = s_new[i];
+    // Work items, a wave each, a word a lane.
+    const int lane = tid & 63;
+    for (int kk = first >> 6; kk < narrow + wide; kk += step >> 6) {
+        const bool is_wide = kk >= narrow;
+        const int k = is_wide ? kk - narrow : kk;
+        const int i = find(is_wide ? s_wide : s_narrow, n, k), l = s_len[i], m = s_new[i];
         const PagedShape p = paged_shape(l, m);
-        const int e = k - s_item[i], b = e / p.splits, split = e - b * p.splits;
+        const int e = k - (is_wide ? s_wide : s_narrow)[i], b = e / p.splits, split = e - b * p.splits;
         const int rb = p.wide ? kWideRows : kNarrowRows, tile = p.wide ? kWideTile : kNarrowTile;
-        const int br = min(rb, m - b * rb);
-        const int tiles = (l + b * rb + br + tile - 1) / tile;
-        PagedItem it;
-        it.req = i;
-        it.row0 = s_row[i] + b * rb;
-        it.pos0 = l + b * rb;
-        it.shape = br | p.splits << 8 | split << 16 | p.wide << 24;
-        it.tile0 = (int)((int64_t)tiles * split / p.splits);
-        it.tile1 = (int)((int64_t)tiles * (split + 1) / p.splits);
-        it.rec = s_rec[i] + b * rb * p.splits;
-        it.block = s_block[i] + b;
-        a.items[k] = it;
+        const int br = min(rb, m - b * rb), end = l + b * rb + br;
+        const int tiles = (end + tile - 1) / tile;
+        const int tile0 = (int)((int64_t)tiles * split / p.splits), tile1 = (int)((int64_t)tiles * (split + 1) / p.splits);
+        const int page0 = tile0 * tile >> sh;
+        int word = 0;
+        switch (lane) {
+            case 0: word = i; break;
+            case 1: word = s_row[i] + b * rb; break;
+            case 2: word = l + b * rb; break;
+            case 3: word = br | p.splits << 8 | split << 16; break;
+            case 4: word = tile0; break;
+            case 5: word = tile1; break;
+            case 6: word = s_rec[i] + b * rb * p.splits; break;
+            case 7: word = s_block[i] + b; break;
+            case 8: word = page0; break;
+            default:
+                if (lane >= kPagedItemHead) word = page_at(i, min(page0 + lane - kPagedItemHead, (end - 1) >> sh));
+        }
+        reinterpret_cast<int*>((is_wide ? a.wide : a.narrow) + k)[lane] = word;
     }
     if (!s_last) return;
     if (mine) a.lens_out[tid] = gone ? 0 : placed ? len + want : len;

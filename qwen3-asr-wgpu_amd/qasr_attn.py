@@ -41,7 +41,7 @@ ABI_SYMBOLS = (
     "qasr_mfma_probe", "qasr_plan_decode", "qasr_plan_prefill",
     "qasr_pages_create", "qasr_pages_destroy", "qasr_pages_get_info", "qasr_paged_plan_create",
     "qasr_paged_plan_destroy", "qasr_paged_plan_get_info", "qasr_paged_plan_build",
-    "qasr_paged_append", "qasr_paged_attn",
+    "qasr_paged_append", "qasr_paged_attn", "qasr_plan_paged",
 )
 MAX_PREFILL_SEGMENTS = 64  # segments per qasr_decoder_prefill_batch call
 
@@ -196,6 +196,7 @@ def load(path: str = LIB_PATH):
     L.qasr_paged_append.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, _vp, _vp, _vp, _vp, _vp]
     L.qasr_paged_attn.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int, _vp,
                                   _vp, _vp]
+    L.qasr_plan_paged.argtypes = [ctypes.c_int, ctypes.c_int, i32p, i32p, i32p]
     _lib = L
     return L
 
@@ -827,6 +828,15 @@ def plan_prefill(rows: int, kv_start: int, nkvh: int = 8):
                                     ctypes.byref(tps), sp))
     return {"rows_per_block": rpb.value, "nrb": nrb.value, "tiles_per_split": tps.value,
             "sp_base": list(sp[:nrb.value + 1])}
+
+
+def plan_paged(length: int, rows: int):
+    """How paged attention cuts a request of `rows` new rows after `length`
+    cached ones (qasr_plan_paged; host only): (rows of a row block, row blocks,
+    key ranges of each)."""
+    w, b, s = ctypes.c_int32(), ctypes.c_int32(), ctypes.c_int32()
+    _check(load().qasr_plan_paged(length, rows, ctypes.byref(w), ctypes.byref(b), ctypes.byref(s)))
+    return (64 if w.value else 16), b.value, s.value
 
 
 LAYER_WEIGHT_NAMES = ("input_layernorm", "q_proj", "k_proj", "v_proj", "q_norm", "k_norm",

@@ -388,13 +388,23 @@ def test_attn_leaves_evicted_pages_out(gpu):
     q = randn(6, 122, QDIM)
     out = run_attn(p, batch, i32(table), q)
     check_attn(p, batch, i32(table), q, out, heads=(0, 11))
-    # Every page of the last request gone after the plan: no key, zeros.
-    t = i32(table)
-    Q.paged_plan(p.ctx, p.plan, i32([c for c, _ in batch]), i32([r for _, r in batch]), t)
-    t[3] = -1
-    Q.paged_attn(p.ctx, p.plan, 0, t, q, out)
+    p.close()
+
+
+def test_attn_of_a_row_without_keys_is_zero(gpu):
+    """Every cached page evicted, and the new row's page an id that the ring
+    should not hold: the row sees no key."""
+    p = Paged(8, 16, 2, 2, rope=False)
+    p.pool.tensor().copy_(randn(5, *p.pool.tensor().shape))
+    table = i32([[-1, 9, -4, 8, -1], [3, -1, -1, -1, -1]])
+    Q.paged_plan(p.ctx, p.plan, i32([64, 5]), i32([1, 1]), table, i32([-1, 1, 2, 4, 5, 6, 7, 0]), i32([0, 1]))
+    assert p.plan.status.tolist() == [0, 0] and p.plan.row_slot.tolist() == [-1, 53]
+    q = randn(6, 2, QDIM)
+    out = torch.full_like(q, 7.0)
+    Q.paged_attn(p.ctx, p.plan, 0, table, q, out)
     torch.cuda.synchronize()
-    assert bool((out[121] == 0).all())
+    assert bool((out[0] == 0).all())
+    check_attn(p, [(5, 1)], table[1:], q[1:], out[1:], heads=(0, 8))
     p.close()
 
 

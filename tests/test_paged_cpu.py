@@ -83,3 +83,25 @@ def test_append_and_attn_refuse_short_tensors():
     _refused(lambda: Q.paged_attn(c, p, 0, _i(2, 4), _h(3, TOT), _h(3, QD)))
     _refused(lambda: Q.paged_attn(c, p, 0, _i(2, 4), _h(3, QD), _h(2, QD)))
     _passed_size_checks(lambda: Q.paged_attn(c, p, 0, _i(2, 4), _h(3, QD), _h(3, QD)))
+
+
+def test_shapes_fit_the_workspaces():
+    """Every (length, rows) stays within what a plan allocates: 32 records a
+    row and 2048 a request, 32 items or one a row block."""
+    seen = set()
+    for rows in list(range(1, 140)) + [255, 256, 257, 511, 512, 1000, 2048, 4097, 16384, 65536]:
+        for length in (0, 1, 100, 496, 511, 512, 513, 1024, 5000, 8192, 16383, 1 << 20, 1 << 24):
+            block, n, splits = Q.plan_paged(length, rows)
+            assert n == -(-rows // block) and 1 <= splits <= 32
+            assert n * splits <= max(32, n)
+            if splits > 1:
+                assert rows * splits <= min(32 * rows, 2048)
+                # no range is empty: a row block has at least as many tiles
+                assert -(-(length + min(rows, block)) // 128) >= splits
+            seen.add((block, min(splits, 2)))
+    assert seen == {(16, 1), (16, 2), (64, 1), (64, 2)}
+
+
+def test_plan_paged_refuses():
+    for length, rows in ((-1, 1), (0, 0), (0, -3), ((1 << 24) + 1, 1), (0, 65537)):
+        _refused(lambda: Q.plan_paged(length, rows))
