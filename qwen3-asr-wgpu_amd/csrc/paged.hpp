@@ -127,6 +127,7 @@ hipError_t launch_paged_append(const CacheGeom& g, int layer, const RowMap& P, i
 // block, kv head, range) (paged_attn.hip); one arrival counter per (row block,
 // kv head), zero at rest, each in a line of its own.
 constexpr int kPagedCounterStep = 32;  // words
+constexpr int kPagedDrawWords = 17 * kPagedCounterStep;  // 16 kv heads and one, a line each
 struct PagedAttnArgs {
     const f16* q;    // [rows][nqh*128], roped
     f16* out;        // [rows][nqh*128]
@@ -141,6 +142,7 @@ struct PagedAttnArgs {
     float* ws_o;
     float* ws_ml;
     uint32_t* counters;
+    uint32_t* drawn;  // [2][kPagedDrawWords], zero at rest: items drawn per kv head, workgroups gone
 };
 hipError_t launch_paged_attn(const PagedAttnArgs& a, int cus, hipStream_t stream);
 

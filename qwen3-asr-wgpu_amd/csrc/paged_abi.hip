@@ -36,7 +36,7 @@ struct qasr_paged_plan {
     size_t bytes = 0;
     int32_t *status, *lens, *row_start, *row_pos, *row_slot, *cursor, *n_items;
     qasr::PagedItem *narrow, *wide;
-    uint32_t *arrived, *counters;
+    uint32_t *arrived, *drawn, *counters;
     float *ws_o, *ws_ml;
     // The last build, for the checks of the calls that follow it.
     int32_t nreq = 0;
@@ -165,7 +165,7 @@ int qasr_paged_plan_create(qasr_ctx* ctx, qasr_pages* pool, int max_requests, in
         at += (n + 255) / 256 * 256;
         return a;
     };
-    const size_t o_ni = part(8), o_arr = part(4), o_ctr = part(blocks * 4 * qasr::kPagedCounterStep), o_cur = part(8);
+    const size_t o_ni = part(8), o_arr = part(4), o_dr = part(2 * 4 * qasr::kPagedDrawWords), o_ctr = part(blocks * 4 * qasr::kPagedCounterStep), o_cur = part(8);
     const size_t o_st = part(4 * (size_t)max_requests), o_len = part(4 * (size_t)max_requests);
     const size_t o_rs = part(4 * (size_t)(max_requests + 1));
     const size_t o_rp = part(4 * (size_t)max_rows), o_sl = part(4 * (size_t)max_rows);
@@ -186,6 +186,7 @@ int qasr_paged_plan_create(qasr_ctx* ctx, qasr_pages* pool, int max_requests, in
     }
     p->n_items = (int32_t*)(p->mem + o_ni);
     p->arrived = (uint32_t*)(p->mem + o_arr);
+    p->drawn = (uint32_t*)(p->mem + o_dr);
     p->counters = (uint32_t*)(p->mem + o_ctr);
     p->cursor = (int32_t*)(p->mem + o_cur);
     p->status = (int32_t*)(p->mem + o_st);
@@ -322,6 +323,7 @@ int qasr_paged_attn(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows, c
     a.ws_o = plan->ws_o;
     a.ws_ml = plan->ws_ml;
     a.counters = plan->counters;
+    a.drawn = plan->drawn;
     const hipError_t e = qasr::launch_paged_attn(a, ctx->cus, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(e, "paged attention launch");
     return QASR_OK;

@@ -49,7 +49,7 @@ template <int NW>
 struct Shared {
     f16 buf[NW * 2 * kSlice * kHeadDim];  // 16 KB a wave: a slice of K and V, or two wide tiles
     float ml[NW][2][64];
-    int last;
+    int last, next;
 };
 static_assert(sizeof(Shared<kWideWaves>::buf) == 2 * 2 * kWideTile * kHeadDim * sizeof(f16), "two wide tiles of K and V");
 
@@ -732,6 +732,10 @@ __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it,
     if (it.splits > 1) arrive(a, it, sh);
 }
 
+// Each kv head has a list of the items; its workgroups (every nkvh-th of the
+// launch) start with one each and, where there are more items, draw the next
+// from the head's counter, so that a workgroup of short items takes more of
+// them.  The last workgroup to leave puts the counters back to zero.
 template <int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_kernel(
     PagedAttnArgs a) {
@@ -739,17 +743,24 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     constexpr bool kWide = NW == kWideWaves;
     const PagedItem* list = kWide ? a.wide : a.narrow;
     const int last_item = (kWide ? a.max_wide : a.max_narrow) - 1;
-    // Every lane reads a word of the item's record; the next item's is
-    // requested when this one starts.
-    auto load_item = [&](int i) {
-        return reinterpret_cast<const int*>(list + min(i / a.nkvh, last_item))[thread_id() & 63];
+    uint32_t* drawn = a.drawn + kWide * kPagedDrawWords;
+    // (The division is done in vector registers.)
+    int i = __builtin_amdgcn_readfirstlane(blockIdx.x / a.nkvh);
+    const int kvh = __builtin_amdgcn_readfirstlane(blockIdx.x - i * a.nkvh);
+    // Every lane reads a word of the item's record.
+    auto load_item = [&](int k) {
+        return reinterpret_cast<const int*>(list + min(k, last_item))[thread_id() & 63];
     };
-    int words = load_item(blockIdx.x);
-    const int items = a.n_items[kWide] * a.nkvh;
-    for (int i = blockIdx.x; i < items; i += gridDim.x) {
+    int words = load_item(i);
+    const int items = a.n_items[kWide], share = __builtin_amdgcn_readfirstlane(gridDim.x / a.nkvh);
+    const int peers = share + (kvh < (int)gridDim.x - share * a.nkvh);  // workgroups of this kv head
+    const bool more = items > share;  // than the launch starts with
+    while (i < items) {
+        uint32_t next = 0;
+        if (more && threadIdx.x == 0) next = ticket_add(drawn + kvh * kPagedCounterStep);
         auto word = [&](int k) { return __builtin_amdgcn_readlane(words, k); };
         Item it;
-        it.kvh = i % a.nkvh;
+        it.kvh = kvh;
         const int shape = word(3);
         it.row0 = word(1);
         it.rows = min(shape & 0xff, a.rows - it.row0);  // rows past the caller's q are left out
@@ -765,16 +776,26 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         it.last_page = (it.kend - 1) >> a.page_shift;
         it.table = a.table + (int64_t)word(0) * a.stride;
         it.base = a.base + it.kvh * a.head_stride;
-        Pages pg;
-        pg.cur = check_pages(a, words);
-        pg.cur.bad &= ~0ull << kPagedItemHead;  // the header's lanes are no pages
-        pg.lo = -kPagedItemHead;
-        if (i + (int)gridDim.x < items) words = load_item(i + gridDim.x);
-        if (it.rows <= 0) continue;
-        pg.nxt = {0, 0};
-        if (it.last_page - it.page0 >= kPagedItemPages) pg.nxt = check_pages(a, load_pages(it, kPagedItemPages));
-        run_item(a, it, pg, sh);
+        if (it.rows > 0) {
+            Pages pg;
+            pg.cur = check_pages(a, words);
+            pg.cur.bad &= ~0ull << kPagedItemHead;  // the header's lanes are no pages
+            pg.lo = -kPagedItemHead;
+            pg.nxt = {0, 0};
+            if (it.last_page - it.page0 >= kPagedItemPages) pg.nxt = check_pages(a, load_pages(it, kPagedItemPages));
+            run_item(a, it, pg, sh);
+        }
+        if (!more) break;
+        if (threadIdx.x == 0) sh.next = peers + (int)next;
         __syncthreads();  // the next item reuses the LDS
+        i = __builtin_amdgcn_readfirstlane(sh.next);
+        words = load_item(i);
+        __syncthreads();
+    }
+    uint32_t* gone = drawn + kPagedDrawWords - kPagedCounterStep;
+    if (more && threadIdx.x == 0 && ticket_add(gone) == gridDim.x - 1) {
+        for (int k = 0; k < a.nkvh; ++k) ticket_reset(drawn + k * kPagedCounterStep);
+        ticket_reset(gone);
     }
 }
 

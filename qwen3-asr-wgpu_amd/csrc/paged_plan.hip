@@ -29,7 +29,7 @@ constexpr int kWavesN = kThreads / 64;
 
 enum : int32_t { kOk = 0, kInvalid = 1, kRange = 2, kNoPage = 3 };  // QASR_OK, _EINVAL, _ERANGE, _ENOMEM
 
-// Six sums below 2^31 in three words.
+// Six sums below 2^31.
 struct Sums {
     uint64_t v[3];
 };
@@ -114,15 +114,14 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PagedPlanArgs a) {
         for (int j = len >> sh; j < j1; ++j)
             if ((uint32_t)trow[j] >= (uint32_t)a.pages) status = kInvalid;
     }
-    uint64_t v1[1] = {(uint64_t)(uint32_t)want}, t1[1];
-    block_scan<1>(v1, t1, s_wave);
-    const int row0 = lo32(v1[0]), nrows = lo32(t1[0]);
-    if (!status && rows > 0 && row0 + want > a.max_rows) status = kRange;
+    // (Once the rows pass max_rows they do for every later request, so whose
+    // pages those count makes no difference.)
     const int need = !status && rows > 0 && a.ring ? full - held : 0;
-    uint64_t v2[1] = {(uint64_t)(uint32_t)need}, t2[1];
-    block_scan<1>(v2, t2, s_wave);
-    const int page0 = lo32(v2[0]);
-    if (need > 0 && page0 + need > free) status = kNoPage;
+    uint64_t v1[1] = {pack2(want, need)}, t1[1];
+    block_scan<1>(v1, t1, s_wave);
+    const int row0 = lo32(v1[0]), nrows = lo32(t1[0]), page0 = hi32(v1[0]);
+    if (!status && rows > 0 && row0 + want > a.max_rows) status = kRange;
+    if (!status && need > 0 && page0 + need > free) status = kNoPage;
     const bool placed = mine && !status && rows > 0;
     const bool gone = mine && !status && rows == -1;
 
@@ -194,12 +193,13 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PagedPlanArgs a) {
     }
     // Work items, a wave each, a word a lane.
     const int lane = tid & 63;
-    for (int kk = first >> 6; kk < narrow + wide; kk += step >> 6) {
-        const bool is_wide = kk >= narrow;
-        const int k = is_wide ? kk - narrow : kk;
-        const int i = find(is_wide ? s_wide : s_narrow, n, k), l = s_len[i], m = s_new[i];
+    for (int k = first >> 6; k < narrow + wide; k += step >> 6) {
+        const int k0 = k < narrow ? 0 : narrow;
+        const int* sums = k < narrow ? s_narrow : s_wide;
+        PagedItem* out = (k < narrow ? a.narrow : a.wide) + k - k0;
+        const int i = find(sums, n, k - k0), l = s_len[i], m = s_new[i];
         const PagedShape p = paged_shape(l, m);
-        const int e = k - (is_wide ? s_wide : s_narrow)[i], b = e / p.splits, split = e - b * p.splits;
+        const int e = k - k0 - sums[i], split = e % p.splits, b = p.blocks - 1 - e / p.splits;  // the longest first
         const int rb = p.wide ? kWideRows : kNarrowRows, tile = p.wide ? kWideTile : kNarrowTile;
         const int br = min(rb, m - b * rb), end = l + b * rb + br;
         const int tiles = (end + tile - 1) / tile;
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PagedPlanArgs a) {
             default:
                 if (lane >= kPagedItemHead) word = page_at(i, min(page0 + lane - kPagedItemHead, (end - 1) >> sh));
         }
-        reinterpret_cast<int*>((is_wide ? a.wide : a.narrow) + k)[lane] = word;
+        reinterpret_cast<int*>(out)[lane] = word;
     }
     if (!s_last) return;
     if (mine) a.lens_out[tid] = gone ? 0 : placed ? len + want : len;
@@ -257,7 +257,8 @@ __global__ __launch_bounds__(kThreads) void paged_plan_kernel(PagedPlanArgs a) {
 
 hipError_t launch_paged_plan(const PagedPlanArgs& a, hipStream_t stream) {
     if (a.nreq < 1 || a.nreq > kPagedMaxRequests || a.max_rows < 1) return hipErrorInvalidValue;
-    const int wgs = a.max_rows <= kThreads ? 1 : (a.max_rows + kThreads - 1) / kThreads;
+    // A workgroup for every 1024 rows and every 16 requests (their work items).
+    const int wgs = a.max_rows / kThreads + (a.nreq + 15) / 16;
     hipLaunchKernelGGL(paged_plan_kernel, dim3(wgs < 64 ? wgs : 64), dim3(kThreads), 0, stream, a);
     return hipGetLastError();
 }
