@@ -593,6 +593,11 @@ class PagedPlan:
 
 def _on(ctx: Context, t, name: str, dtype=None) -> int:
     """`_dev` of a tensor on the context's GPU."""
+    try:  # what a right call takes: no more than it needs, a plan is short
+        if t.dtype is dtype and t.get_device() == ctx.device and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
     ptr = _dev(t, name, dtype)
     if t.device.index != ctx.device:
         raise QasrError(QASR_EINVAL, f"{name} is on {t.device}, the context on GPU {ctx.device}")
@@ -653,13 +658,16 @@ def paged_append(ctx: Context, plan: PagedPlan, layer: int, qkv, q_gain, k_gain,
                  stream=None):
     """Stage (a) of the planned step's rows into the layer's pages
     (qasr_paged_append): qkv [rows][(nqh + 2 nkvh) hd], q_out [rows][nqh hd]."""
+    import torch
+
+    f16 = torch.float16
     tot, qd = _widths(ctx)
     rows = _paged_rows(qkv, tot, "qkv")
     _need(q_out, rows * qd, "q_out")
     _gains(ctx, q_gain, k_gain)
     _check(load().qasr_paged_append(
-        ctx.handle, plan.handle, layer, rows, _on(ctx, qkv, "qkv"), _on(ctx, q_gain, "q_gain"),
-        _on(ctx, k_gain, "k_gain"), _on(ctx, q_out, "q_out"), _ctx_stream(ctx, stream)))
+        ctx.handle, plan.handle, layer, rows, _on(ctx, qkv, "qkv", f16), _on(ctx, q_gain, "q_gain", f16),
+        _on(ctx, k_gain, "k_gain", f16), _on(ctx, q_out, "q_out", f16), _ctx_stream(ctx, stream)))
 
 
 def paged_attn(ctx: Context, plan: PagedPlan, layer: int, table, q, out, stream=None):
@@ -667,13 +675,14 @@ def paged_attn(ctx: Context, plan: PagedPlan, layer: int, table, q, out, stream=
     (qasr_paged_attn): q and out [rows][nqh hd], `table` as planned."""
     import torch
 
+    f16 = torch.float16
     _, qd = _widths(ctx)
     rows = _paged_rows(q, qd, "q")
     _need(out, rows * qd, "out")
     stride = _table(table, plan.nreq)
     _check(load().qasr_paged_attn(
         ctx.handle, plan.handle, layer, rows, _on(ctx, table, "table", torch.int32), stride,
-        _on(ctx, q, "q"), _on(ctx, out, "out"), _ctx_stream(ctx, stream)))
+        _on(ctx, q, "q", f16), _on(ctx, out, "out", f16), _ctx_stream(ctx, stream)))
 
 
 class AttnBackend:
