@@ -74,7 +74,7 @@ __device__ __forceinline__ float2 load_dev2(const float* p) {
 
 // What a workgroup knows of its item.
 struct Item {
-    int row0, rows, pos0, kend, tile0, tile1, splits, split, rec, block, kvh;
+    int row0, rows, planned, pos0, kend, tile0, tile1, splits, split, rec, block, kvh;
     int page0, last_page;  // first page of the range, last of the row block's keys (table places)
     const int32_t* table;  // the request's pages
     const f16* base;       // the kv head's K in page 0
@@ -390,9 +390,9 @@ __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& 
 // Puts the columns of a wave whose dim block db (32 dims) is not finite.
 // every lane: its column's max and sum; valid columns only.
 __device__ __forceinline__ void put_exact(const PagedAttnArgs& a, const Item& it, int key0, int key1, float M, float L,
-                                          int db, int r, int h, bool valid) {
+                                          int db, int r, int h, bool valid, uint32_t cols) {
     const int lane = thread_id() & 63;
-    uint64_t todo = __ballot(valid) & 0xffffffffu;  // a lane a column: those of g = 0
+    uint64_t todo = __ballot(valid) & cols;  // a lane a column: those of g = 0
     while (todo) {
         const int j = __builtin_ctzll(todo);
         todo &= todo - 1;
@@ -612,10 +612,160 @@ __device__ __forceinline__ void leave(Shared<NW>& sh, const Wave& w, int wave, i
         }
 }
 
-__device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it, Pages pg, Shared<kNarrowWaves>& sh) {
+// Narrow items of up to 8 rows: their 16 columns on v_mfma_f32_16x16x32_f16,
+// whose products take half the time, with half the scores a lane.  us a layer
+// on 32 columns against 16: 1 row of 512 keys 8.4 / 7.7, of 8192 14.8 / 14.4, 16 rows
+// of 400-2400 24.7 / 24.1.
+constexpr int kFewRows = 8;
+struct Few {
+    static constexpr int kRows = kFewRows;
+    half8v qb[4];  // Q^T of k-step ks: dims 32*ks + 8*g .. +8 of query n
+    float4v o[8];  // O^T: o[db][i] = dim db*16 + 4*g + i of query n
+    float m, l;
+    int kaddr[4];  // K operand of k-step ks, rows 0..15 (halves)
+    int vbase;
+    int g, qpos;  // g: the lane's quarter
+    float scale_log2;
+};
+__device__ __forceinline__ float quarters_max(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return halves_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quarters_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return halves_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float4v mfma16(const half8v& a, const half8v& b, const float4v& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void init_wave(Few& w, const PagedAttnArgs& a, const Item& it, int rin, int h, int lane) {
+    const int r = min(rin, it.rows - 1), n = lane & 15;
+    w.g = lane >> 4;
+    const f16* q = a.q + ((int64_t)(it.row0 + r) * a.nkvh + it.kvh) * (kRep * kHeadDim) + h * kHeadDim + 8 * w.g;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+        w.qb[ks] = *(const half8v*)(q + 32 * ks);
+        w.kaddr[ks] = n * kHeadDim + (((4 * ks + w.g) ^ swz16(n)) * 8);
+    }
+    w.vbase = (4 * w.g + (n >> 2)) * 32 + 4 * (n & 3);
+    w.qpos = it.pos0 + r;
+    w.scale_log2 = a.scale_log2;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) w.o[db] = (float4v){};
+    w.m = kNegInf;
+    w.l = 0.0f;
+}
+__device__ __forceinline__ void wait_q(Few& w) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) asm volatile("" : "+v"(w.qb[ks]));
+}
+// P^T of a slice: S^T of keys 16 kb + 4 g + i, masked, the running maximum,
+// the weights (B operand: its k 8 g + j is key 16 (j / 4) + 4 g + j % 4) and
+// their sum.
+__device__ __forceinline__ void slice_scores(const Few& w, const f16* kt, float4v (&s)[2]) {
+    half8v ka[8];
+    auto read = [&](int x) { ka[x] = *(const half8v*)&kt[(x & 1) * 16 * kHeadDim + w.kaddr[x >> 1]]; };
+    s[0] = s[1] = (float4v){};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) read(x);
+    keep_order();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+        if (x + 4 < 8) read(x + 4);
+        keep_order();
+        s[x & 1] = mfma16(ka[x], w.qb[x >> 1], s[x & 1]);
+        keep_order();
+    }
+}
+__device__ __forceinline__ void slice_weights(Few& w, float4v (&s)[2], int k0, bool mask, uint32_t hidden, half8v (&pb)[1]) {
+    if (mask) {
+        const int last = w.qpos - k0 - 4 * w.g;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j >> 2][j & 3] = 16 * (j >> 2) + (j & 3) > last ? kNegInf : s[j >> 2][j & 3];
+    }
+    if (rarely(hidden)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j >> 2][j & 3] = hidden >> (j >> 2) & 1 ? kNegInf : s[j >> 2][j & 3];
+    }
+    float mx = kNegInf;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, s[j >> 2][j & 3]);
+    mx = quarters_max(mx) * w.scale_log2;
+    const bool up = mx > w.m + kRescaleSlack;
+    if (__ballot(up)) {
+        if (rarely(__ballot(up && w.m != kNegInf))) {
+            const float alpha = !up ? 1.0f : w.m == kNegInf ? 0.0f : fast_exp2(w.m - mx);
+#pragma unroll
+            for (int db = 0; db < 8; ++db) w.o[db] *= alpha;
+            w.l *= alpha;
+        }
+        w.m = up ? mx : w.m;
+    }
+    const float mu = w.m == kNegInf ? 0.0f : w.m;
+    float ps[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        pb[0][j] = (f16)softmax_w_raw(s[j >> 2][j & 3], w.scale_log2, mu);
+        ps[j & 1] += (float)pb[0][j];
+    }
+    w.l += quarters_sum(ps[0] + ps[1]);
+}
+__device__ __forceinline__ void slice_product(Few& w, const f16* vt, const half8v (&pb)[1]) {
+    half4v lo[8], hi[8];
+    auto read = [&](int x) {
+        const f16* vp = vt + w.vbase + (x >> 1) * (kSlice * 32) + (x & 1) * 16;
+        lo[x] = read_tr(vp);
+        hi[x] = read_tr(vp + 16 * 32);
+    };
+#pragma unroll
+    for (int x = 0; x < 4; ++x) read(x);
+    keep_order();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+        if (x + 4 < 8) read(x + 4);
+        keep_order();
+        w.o[x] = mfma16(__builtin_shufflevector(lo[x], hi[x], 0, 1, 2, 3, 4, 5, 6, 7), pb[0], w.o[x]);
+        keep_order();
+    }
+}
+template <int NW>
+__device__ __forceinline__ void leave_all(Shared<NW>& sh, const Few& w, int wave, int lane) {
+    float4* dst = reinterpret_cast<float4*>(sh.buf) + wave * 1024 + lane;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) dst[db * 64] = make_float4(w.o[db][0], w.o[db][1], w.o[db][2], w.o[db][3]);
+}
+__device__ __forceinline__ void put_dims(const PagedAttnArgs& a, const Item& it, const float (&o)[8], float l, int wave,
+                                         int g, int r, int h) {
+    put_block<1>(a, it, o, l, wave, g >> 1, g & 1, r, h);
+    put_block<1>(a, it, o + 4, l, wave, 2 + (g >> 1), g & 1, r, h);
+}
+
+// And of up to 16 rows.
+struct Many : Wave {
+    static constexpr int kRows = kNarrowRows;
+};
+__device__ __forceinline__ void slice_scores(const Many& w, const f16* kt, float16v (&s)[1]) { scores<1>(w, kt, s); }
+__device__ __forceinline__ void slice_weights(Many& w, float16v (&s)[1], int k0, bool mask, uint32_t hidden, half8v (&pb)[2]) {
+    if (mask) mask_scores<1>(w, s, k0);
+    if (rarely(hidden)) hide_scores<1>(s, hidden);
+    move_max<1>(w, s);
+    weights<1>(w, s, pb);
+}
+__device__ __forceinline__ void slice_product(Many& w, const f16* vt, const half8v (&pb)[2]) { product<kSlice, 1>(w, vt, pb); }
+template <int NW>
+__device__ __forceinline__ void leave_all(Shared<NW>& sh, const Many& w, int wave, int lane) { leave<4>(sh, w, wave, 0, lane); }
+__device__ __forceinline__ void put_dims(const PagedAttnArgs& a, const Item& it, const float (&o)[16], float l, int wave,
+                                         int g, int r, int h) {
+    put_block<4>(a, it, o, l, wave, 0, g, r, h);
+}
+
+template <class W, class S, int NS, int NP>
+__device__ __forceinline__ void run_narrow(const PagedAttnArgs& a, const Item& it, Pages pg, Shared<kNarrowWaves>& sh) {
     const int tid = thread_id(), lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int n = lane & 31, h = n >> 4, rin = n & 15;
+    constexpr int kCols = kRep * W::kRows, kElems = kCols / 2;
+    const int n = lane & (kCols - 1), h = n / W::kRows, rin = n % W::kRows;
     f16* kbuf = sh.buf + wave * (2 * kSlice * kHeadDim);
     f16* vbuf = kbuf + kSlice * kHeadDim;
     const Offsets whole = group_offsets(lane, 0, 15, (uint32_t)a.kv_stride * 2);
@@ -629,7 +779,7 @@ __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it,
             copy_group(a, it, group_base(a, it, pg, key), whole, key, v, lds, v ? kSlice * 64 : 1024);
         }
     };
-    Wave w;
+    W w;
     init_wave(w, a, it, rin, h, lane);
     if (it.tile0 < it.tile1) {
         copy_slice(it.tile0, false);
@@ -646,22 +796,19 @@ __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it,
             break;
         }
         WAIT_VM(8);  // K landed, V in flight
-        float16v s[1];
-        half8v pb[2];
-        scores<1>(w, kbuf, s);
+        S s[NS];
+        half8v pb[NP];
+        slice_scores(w, kbuf, s);
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             copy_slice(t + 1, false);
         }
-        if (k0 + kSlice - 1 > it.pos0) mask_scores<1>(w, s, k0);
-        if (rarely(hidden)) hide_scores<1>(s, hidden);
-        move_max<1>(w, s);
-        weights<1>(w, s, pb);
+        slice_weights(w, s, k0, k0 + kSlice - 1 > it.pos0, hidden, pb);
         if (more)
             WAIT_VM(8);
         else
             WAIT_VM(0);
-        product<kSlice, 1>(w, vbuf, pb);
+        slice_product(w, vbuf, pb);
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             copy_slice(t + 1, true);
@@ -672,21 +819,29 @@ __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it,
     // wave's own (now free) slice buffer.
     const bool valid = rin < it.rows;
     if (valid) {
-        leave<4>(sh, w, wave, 0, lane);
+        leave_all(sh, w, wave, lane);
         sh.ml[wave][0][lane] = w.m;
         sh.ml[wave][1][lane] = w.l;
     }
     __syncthreads();
-    float o[16], M = 0.0f, L = 0.0f, t = 0.0f;
+    float o[kElems], M = 0.0f, L = 0.0f, t = 0.0f;
     if (valid) {
-        combine<kNarrowWaves, 16>(sh, 0, 1, 16 * wave, lane, o, M, L);
-        t = not_finite<16>(o) + 0.0f * L;
+        combine<kNarrowWaves, kElems>(sh, 0, 1, kElems * wave, lane, o, M, L);
+        t = not_finite<kElems>(o) + 0.0f * L;
     }
     if (rarely(__ballot(t != t)))
-        put_exact(a, it, it.tile0 * kNarrowTile, min(it.tile1 * kNarrowTile, it.kend), M, L, wave, rin, h, valid);
+        put_exact(a, it, it.tile0 * kNarrowTile, min(it.tile1 * kNarrowTile, it.kend), M, L, wave, rin, h, valid,
+                  kCols == 32 ? ~0u : 0xffffu);
     else if (valid)
-        put_block<4>(a, it, o, L, wave, 0, w.g, rin, h);
+        put_dims(a, it, o, L, wave, w.g, rin, h);
     if (it.splits > 1 && valid && wave == 0 && w.g == 0) store_dev2(range_ml(a, it, it.split) + column(it, rin, h) * 2, M, L);
+}
+
+__device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it, Pages pg, Shared<kNarrowWaves>& sh) {
+    if (it.planned <= kFewRows)
+        run_narrow<Few, float4v, 2, 1>(a, it, pg, sh);
+    else
+        run_narrow<Many, float16v, 1, 2>(a, it, pg, sh);
     if (it.splits > 1) arrive(a, it, sh);
 }
 
@@ -747,7 +902,7 @@ __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it,
         combine<2, 16>(sh, rw, 4, db * 16, lane, o, M, L);
         const float t = not_finite<16>(o) + 0.0f * L;
         if (rarely(__ballot(valid && t != t)))
-            put_exact(a, it, it.tile0 * kWideTile, min(it.tile1 * kWideTile, it.kend), M, L, db, rin, h, valid);
+            put_exact(a, it, it.tile0 * kWideTile, min(it.tile1 * kWideTile, it.kend), M, L, db, rin, h, valid, ~0u);
         else if (valid)
             put_block<4>(a, it, o, L, db, 0, w.g, rin, h);
     }
@@ -786,7 +941,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         it.kvh = kvh;
         const int shape = word(3);
         it.row0 = word(1);
-        it.rows = min(shape & 0xff, a.rows - it.row0);  // rows past the caller's q are left out
+        it.planned = shape & 0xff;
+        it.rows = min(it.planned, a.rows - it.row0);  // rows past the caller's q are left out
         it.pos0 = word(2);
         it.kend = it.pos0 + it.rows;
         it.tile0 = word(4);
