@@ -210,7 +210,8 @@ int qasr_prefill_layer(qasr_ctx* ctx, qasr_kv* kv, int layer, int slot, int kv_s
  * every call may be captured.  A context outlives its pools, a pool its plans.
  * Calls that share a plan must be ordered on one
  * stream (they share its arrays and split workspace); so must calls that
- * write pages of a pool and those that read them. */
+ * write pages of a pool and those that read them.  Plans share nothing, so calls
+ * of two plans may run side by side on two streams. */
 typedef struct qasr_pages qasr_pages;
 typedef struct qasr_paged_plan qasr_paged_plan;
 
@@ -282,9 +283,12 @@ int qasr_paged_plan_get_info(const qasr_paged_plan* plan, qasr_paged_plan_info* 
  * outputs are left as they were; so are those behind the last row.
  *
  * len_dev may be the plan's own lens_dev and cursor_dev its cursor_dev: then
- * each build goes on where the last one ended.  A table may list one page for
- * several requests (a shared prefix); a page given back twice corrupts the
- * ring.  The arrays must be distinct otherwise. */
+ * each build goes on where the last one ended.  The arrays must be distinct
+ * otherwise.  A table may list one page for several requests (a shared prefix),
+ * as long as none of them stores rows in it: a request's first new row goes
+ * into its last page while that has room, so a shared prefix is whole pages.  A
+ * page that two ended requests give back is twice in the ring: end all but the
+ * last of its requests with their shared entries set to -1. */
 int qasr_paged_plan_build(qasr_ctx* ctx, qasr_paged_plan* plan, int nreq, const int32_t* len_dev,
                           const int32_t* rows_dev, int32_t* table_dev, int table_stride,
                           int32_t* ring_dev, const int32_t* cursor_dev, void* stream);
@@ -300,7 +304,8 @@ int qasr_paged_append(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows,
  * [nqh*hd]; out_dev the same shape): a row at position p attends its request's
  * keys 0..p.  table_dev: the table of the build, unchanged since.  Keys of
  * entries outside the pool (an evicted page, say -1) are left out; a row that
- * sees no key gives zeros.  A request's output bits depend on its rows, length
+ * sees no key, or only scores of -inf, gives zeros.  Infinities and NaN in a key
+ * or value reach the rows that see it and no others.  A request's output bits depend on its rows, length
  * and keys alone, not on its batch mates or where its pages lie. */
 int qasr_paged_attn(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows,
                     const int32_t* table_dev, int table_stride, const void* q_dev, void* out_dev,

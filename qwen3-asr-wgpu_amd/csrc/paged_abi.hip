@@ -105,6 +105,7 @@ int qasr_pages_create(qasr_ctx* ctx, int pages, int page_rows, qasr_pages** out)
     if (e != hipSuccess) {
         if (p->base) (void)hipFree(p->base);
         delete p;
+        (void)hipGetLastError();  // the next launch must not report it
         return hip_fail(e, "page pool allocation");
     }
     *out = p;
@@ -182,6 +183,7 @@ int qasr_paged_plan_create(qasr_ctx* ctx, qasr_pages* pool, int max_requests, in
     if (e != hipSuccess) {
         if (p->mem) (void)hipFree(p->mem);
         delete p;
+        (void)hipGetLastError();  // the next launch must not report it
         return hip_fail(e, "paged plan allocation");
     }
     p->n_items = (int32_t*)(p->mem + o_ni);

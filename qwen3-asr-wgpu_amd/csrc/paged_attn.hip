@@ -2,24 +2,42 @@
 //
 // Row r at position p of a request attends keys 0..p of it: softmax(q.k_t /
 // sqrt(128)) . v, keys whose page lies outside the pool left out; a row that
-// sees no key is zero.  One launch takes any mix of single rows and chunks:
-// the work list (paged_plan.hip) is on the GPU, the workgroups walk it.
+// sees no key is zero.  A call takes any mix of single rows and chunks: the
+// work lists (paged_plan.hip) are on the GPU, the workgroups walk them; a
+// launch for narrow items and, where a step can have some, one for wide ones.
 //
-// Work item = (row block and key range of a request, kv head), kv head minor:
-// with 8 kv heads workgroup i runs kv head i mod 8 on XCD i mod 8, and the
-// row blocks of a kv head share its keys in that XCD's L2.  A workgroup is 4
-// waves; a wave's 32 MFMA columns are 16 rows x the 2 q heads of the kv head
-// (mfma_attn.hpp), so both heads use each key read.
-//  - narrow items, up to 16 rows: every 128-key tile is cut into the waves'
-//    slices of 32 keys.  A wave copies its own slice into its own LDS (16
-//    KB), so the loop has no barrier; K of the next tile is requested when
+// Work item = (row block and key range of a request), for one kv head: with 8
+// kv heads workgroup i runs kv head i mod 8 on XCD i mod 8, and the row blocks
+// of a kv head share its keys in that XCD's L2.  Both q heads of a kv head are
+// columns of one matrix product, so each key read serves both: S^T = K Q^T, the
+// softmax of a column in the registers of its lanes, O^T += V^T P^T.
+//  - narrow items, up to 16 rows, 4 waves: every 128-key tile is cut into the
+//    waves' slices of 32 keys.  A wave copies its own slice into its own LDS
+//    (16 KB), so the loop has no barrier; K of the next tile is requested when
 //    the scores are done with this one, V when its product is.  The waves'
-//    states combine through LDS at the end.
-//  - wide items, up to 64 rows: wave w takes rows 16 w .. +16 against whole
-//    64-key tiles, copied by all waves into two 32 KB buffers in turn, one
-//    barrier a tile.
-// Both fit 66 KB of LDS and 256 registers: two workgroups a CU, so one's
-// softmax and latencies run under the other's MFMAs and copies.
+//    states combine through LDS at the end.  68 KB of LDS: two workgroups a CU,
+//    one's softmax and latencies run under the other's products and copies.
+//    Blocks of up to 8 rows (decode) run on products of 16 columns.
+//  - wide items, up to 64 rows, 8 waves: 4 waves of 16 rows (32 columns) take
+//    the first 64 keys of a 128-key tile and 4 the others; a tile is copied by
+//    all into one of two buffers while the other is worked on, one barrier a
+//    tile, 135 KB of LDS.  Each key is read once for 64 rows.
+//
+// What bounds it.  Decode: bytes, and below some 100 MB the chain of one item:
+// a tile takes a wave 0.8 us (16 columns; 0.96 with 32) however early its copy
+// was asked for (two tiles in flight a wave: no gain), launch, item and first
+// tile 3.5 us, the end 1.3 us.  us a layer of 16 q and 8 kv heads:
+//   1 row of 512 keys 7.7, of 8192 (33.6 MB) 14.4, 16 rows of 400-2400 24.1
+//   (93.8 MB, 3.9 TB/s; a large copy reaches 5.2).
+// Chunks: MFMA and VALU work, which share the issue slots of a SIMD (two waves
+// overlap about half of the smaller part), at a clock that falls to 1.9 GHz:
+//   2 x 2048 rows at 4096 206 (172 GFLOP, 0.83 PFLOP/s; a large f16 product
+//   reaches 1.1-1.3), 512 at 7680 52 (0.64), 8 chunks of 7-45 rows at 200-1700
+//   17.2, 24 single rows of 100-2400 with 4 chunks of 100-450 rows 45.
+// Also measured: 64-row items of 4 waves 223 us for the first of these, the
+// key groups half a tile apart 223; narrow items of 8 waves 5.7 against 4.8 us
+// for a single row's loop; 64-row blocks for every chunk 85 us for the last
+// step.
 //
 // Copies are 1 KB global -> LDS instructions of 4 K rows or 16 V rows of 32
 // dims: with pages of at least 16 rows each stays in one page, whose address

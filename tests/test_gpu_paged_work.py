@@ -238,6 +238,63 @@ def test_wide_bits_do_not_depend_on_the_batch_or_the_pages(gpu):
     p.close()
 
 
+@pytest.mark.parametrize("batch", [[(300, 5)], [(300, 14)], [(1800, 8)], [(2500, 530)]])
+def test_a_broken_query_reaches_only_its_own_row_and_head(gpu, batch):
+    """NaN in one (row, q head): the other columns of its block are finite and
+    right."""
+    ps, (c, r) = 32, batch[0]
+    need = needed(batch, ps)
+    table, _ = shuffled_table(random.Random(4), need, need[0], need[0])
+    p = Paged(need[0], ps, 1, r, rope=False)
+    pool = p.pool.tensor()
+    pool.copy_(randn(5, *pool.shape))
+    q = randn(6, r, QDIM)
+    row, head = r // 2, 4
+    good = q.clone()
+    q[row, head * HD + 17] = float("nan")
+    out = run_attn(p, batch, i32(table), q)
+    v = out.view(r, NQH, HD)
+    assert bool(torch.isnan(v[row, head]).all())
+    v[row, head] = 0
+    assert bool(torch.isfinite(v).all())
+    clean = run_attn(p, batch, i32(table), good)
+    v[row, head] = clean.view(r, NQH, HD)[row, head]
+    check_rows(p, batch, table, good, out, heads=(head, head + 1, 0))
+    p.close()
+
+
+def test_scores_of_minus_infinity(gpu):
+    """Keys whose scores are -inf weigh nothing; a row with no other is zero."""
+    batch, ps = [(40, 1), (40, 3), (700, 12)], 16
+    need = needed(batch, ps)
+    table, _ = shuffled_table(random.Random(4), need, sum(need), max(need))
+    p = Paged(sum(need), ps, 3, 16, rope=False)
+    pool = p.pool.tensor()
+    pool.copy_(randn(5, *pool.shape))
+    q = randn(6, 16, QDIM).abs()  # so that a key of -inf scores -inf
+    pool[:, table[0][:need[0]], 0] = float("-inf")        # every key of request 0
+    pool[:, table[1][0], 0, :, 3:9] = float("-inf")       # some of request 1
+    pool[:, table[2][:20], 0] = float("-inf")             # whole tiles of request 2
+    out = run_attn(p, batch, i32(table), q)
+    assert bool((out[0] == 0).all())
+    # the definition over the keys that weigh something
+    r0 = 1
+    for i in (1, 2):
+        c, r = batch[i]
+        ids = torch.tensor(table[i][:need[i]]).cuda()
+        for h in (0, 9):
+            kv = pool[0][ids][:, :, h // 2].double().cpu().numpy()
+            k, v = (kv[:, s].reshape(-1, HD)[:c + r] for s in (0, 1))
+            seen = np.isfinite(k).all(axis=1)
+            cols = slice(h * HD, (h + 1) * HD)
+            want, bound = M.attend(q[r0:r0 + r, cols].double().cpu().numpy(), np.where(seen[:, None], k, 0), v,
+                                   range(c, c + r), seen)
+            d = np.abs(out[r0:r0 + r, cols].double().cpu().numpy() - want)
+            assert (d <= bound).all(), (i, h, float((d / bound).max()))
+        r0 += r
+    p.close()
+
+
 # ---- more items than workgroups --------------------------------------------
 
 @pytest.mark.parametrize("nkvh", [1, 8])
@@ -369,6 +426,45 @@ def test_creates_refuse(gpu):
     pool.close()
     other.close()
     ctx.close()
+
+
+def test_a_failed_allocation_is_not_the_next_calls_error(gpu):
+    """A pool far larger than the card: refused, and what follows runs."""
+    ctx = Q.Context(NQH, NKVH, HD, 28, 1e-6, 512, 0)
+    refused(Q.QASR_ENOMEM, lambda: Q.PagePool(ctx, (1 << 27) - 1, 16))
+    pool = Q.PagePool(ctx, 4, 16)
+    plan = Q.PagedPlan(ctx, pool, 1, 1)
+    table = i32([[2]])
+    Q.paged_plan(ctx, plan, i32([3]), i32([1]), table)
+    q = randn(3, 1, QDIM)
+    out = torch.full_like(q, 7.0)
+    Q.paged_attn(ctx, plan, 5, table, q, out)
+    torch.cuda.synchronize()
+    assert bool((out == 0).all())  # a zeroed pool
+    plan.close()
+    pool.close()
+    ctx.close()
+
+
+def test_a_shared_prefix_is_given_back_once(gpu):
+    """Two requests over one prefix of whole pages; the first to end leaves the
+    shared entries out, the last gives them back."""
+    p = Paged(8, 16, 2, 4, rope=False)
+    ring, cursor = i32([5, 6, 7, 0, 0, 0, 0, 0]), i32([0, 3])
+    table = i32([[0, 1, -1, -1], [0, 1, -1, -1]])
+    p.plan.lens.copy_(i32([32, 32]))
+    p.plan.cursor.copy_(cursor)
+    step = lambda rows: Q.paged_plan(p.ctx, p.plan, p.plan.lens, i32(rows), table, ring, p.plan.cursor)  # noqa: E731
+    step([1, 2])
+    assert table.tolist() == [[0, 1, 5, -1], [0, 1, 6, -1]] and p.plan.cursor.tolist() == [2, 1]
+    table[0, :2] = -1
+    step([-1, 1])
+    assert p.plan.status.tolist() == [0, 0] and p.plan.lens.tolist() == [0, 35]
+    assert p.plan.cursor.tolist() == [2, 2]
+    step([0, -1])
+    head, free = p.plan.cursor.tolist()
+    assert sorted(ring[(head + k) % 8].item() for k in range(free)) == [0, 1, 5, 6, 7]
+    p.close()
 
 
 def test_calls_refuse(gpu):
