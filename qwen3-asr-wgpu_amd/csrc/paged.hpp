@@ -23,9 +23,11 @@ constexpr int kPagedMaxShift = 8;
 // a request's bits do not depend on its batch mates.
 constexpr int kNarrowRows = 16, kNarrowTile = 128;
 constexpr int kWideRows = 64, kWideTile = 128;
-constexpr int kPagedMaxSplits = 32;     // row blocks x splits of a split request
-constexpr int kPagedRangeKeys = 512;
-constexpr int64_t kWideWork = 5 << 18;  // rows x mean keys from which on row blocks are wide
+constexpr int kPagedMaxSplits = 32;     // row blocks x ranges of a split request
+constexpr int kPagedManyBlocks = 16;    // but of one of more narrow row blocks than this
+constexpr int kPagedMaxItems = 64;      // (those)
+constexpr int kPagedRangeKeys = 512, kPagedManyRangeKeys = 2048;
+constexpr int64_t kWideWork = 1 << 21;  // rows x mean keys from which on row blocks are wide
 
 struct PagedShape {
     int32_t wide;    // row blocks of kWideRows rows
@@ -35,19 +37,25 @@ struct PagedShape {
 
 // Wide row blocks read each key once for 64 rows, narrow ones for 16, but
 // narrow ones are four times as many, start sooner and combine for less: us a
-// layer, narrow against wide, 128 rows at 4000 22.4 / 30.6, 1000 at 0 18 / 23.5,
-// 256 at 4000 29 / 32, 512 at 2000 28.8 / 28.1, 2048 at 0 43 / 38.6, 1024 at
-// 4000 65 / 55.5, 512 at 7680 74 / 51.  Ranges: one row at 1024, 2048, 8192 keys
-// 9.2, 9.6, 17.2 in ranges of 256 keys, 10.9, 11.3, 15.9 of 512, 12.9, 15.5, 19.4
-// of 1024; 16 rows at 2000 keys each 32.9, 29.6, 29.5.
+// layer, narrow against wide (each without a launch for the other kind), 1000
+// rows at 0 17.2 / 24.1, 512 at 2000 26.9 / 28.4, 1024 at 1000 27.2 / 31.9, 4
+// requests of 256 at 6000 108 / 125, 2048 at 0 40.9 / 39.8, 512 at 4000 43.4 /
+// 36.7, 1024 at 4000 64 / 57, 3000 at 0 71 / 58.  A launch that finds no wide
+// items takes 4.6 us.
+// Ranges, up to 16 row blocks: one row at 512, 8192 keys in ranges of 256 keys
+// 8.2, 13.4, of 512 7.7, 14.4; 16 rows of 400-2400 each 28.1, 24.1.  Of more row
+// blocks, 300 rows at 5000 not split 49, in 3 ranges 33; 4 requests of 300 rows
+// at 1200 not split 38, in ranges of 512 53: longer ranges, of 2048 keys.
 __host__ __device__ inline PagedShape paged_shape(int len, int rows) {
     PagedShape s;
     s.wide = (int64_t)rows * (len + rows / 2) >= kWideWork;
     const int rb = s.wide ? kWideRows : kNarrowRows;
     s.blocks = (rows + rb - 1) / rb;
     const int first = len + (rows < rb ? rows : rb);  // keys of the first row block
-    const int most = s.blocks < kPagedMaxSplits ? kPagedMaxSplits / s.blocks : 1;
-    const int want = (first + kPagedRangeKeys - 1) / kPagedRangeKeys;
+    const bool many = !s.wide && s.blocks > kPagedManyBlocks;
+    const int cap = many ? kPagedMaxItems : kPagedMaxSplits, range = many ? kPagedManyRangeKeys : kPagedRangeKeys;
+    const int most = s.blocks < cap ? cap / s.blocks : 1;
+    const int want = (first + range - 1) / range;
     s.splits = want < most ? want : most;
     return s;
 }
@@ -74,12 +82,15 @@ struct PagedItem {  // one row block and key range, for every kv head: 64 words,
 static_assert(sizeof(PagedItem) == 64 * 4, "a word a lane");
 
 // Capacities for max_requests requests and max_rows rows together.  A
-// request has at most max(kPagedMaxSplits, blocks) items and, split, rows *
+// request has at most max(kPagedMaxItems, blocks) items and, split, rows *
 // splits records: at most kPagedMaxSplits a row and kPagedMaxSplits *
 // kWideRows in all.
+static_assert(kPagedMaxItems * kNarrowRows <= kPagedMaxSplits * kWideRows && kPagedMaxItems >= kPagedMaxSplits &&
+                  kPagedMaxItems / (kPagedManyBlocks + 1) <= kPagedMaxSplits,
+              "splits and records of a request");
 inline int64_t paged_max_blocks(int64_t requests, int64_t rows) { return requests + rows / kNarrowRows; }
 inline int64_t paged_max_items(int64_t requests, int64_t rows, int64_t rows_a_block) {
-    return requests * kPagedMaxSplits + requests + rows / rows_a_block;
+    return requests * kPagedMaxItems + requests + rows / rows_a_block;
 }
 inline int64_t paged_max_records(int64_t requests, int64_t rows) {
     const int64_t a = rows * kPagedMaxSplits, b = requests * kPagedMaxSplits * kWideRows;

@@ -63,9 +63,9 @@ def assert_wide(batch):
 
 
 WIDE = [
-    [(2500, 512)], [(700, 1100)], [(0, 2048)], [(5000, 300)], [(2049, 575)], [(0, 1621)],
-    [(16000, 97)],  # every range of a wide row block
-    [(900, 1), (2500, 512), (40, 20), (0, 0), (1000, 1090), (3000, 1)],
+    [(4000, 512)], [(1500, 1100)], [(0, 2048)], [(7000, 300)], [(3600, 575)], [(0, 2051)],
+    [(16000, 135)],
+    [(900, 1), (4000, 512), (40, 20), (0, 0), (1600, 1090), (3000, 1)],
 ]
 
 
@@ -88,9 +88,29 @@ def test_wide_row_blocks_against_64_bits(gpu, ps, batch):
     p.close()
 
 
+@pytest.mark.parametrize("batch", [[(5000, 300)], [(4200, 272)], [(6000, 257), (3, 1), (4100, 400)]],
+                         ids=lambda b: "+".join(f"{r}@{c}" for c, r in b))
+def test_many_narrow_row_blocks_in_ranges(gpu, batch):
+    """More than 16 row blocks of 16 rows, each in two or three ranges."""
+    for c, r in batch:
+        block, blocks, splits = Q.plan_paged(c, r)
+        assert block == 16 and (r == 1 or (blocks > 16 and splits > 1))
+    ps, need = 32, needed(batch, 32)
+    table, _ = shuffled_table(random.Random(1), need, sum(need) + 1, max(need))
+    rows = sum(r for _, r in batch)
+    p = Paged(sum(need) + 1, ps, len(batch), rows, rope=False)
+    pool = p.pool.tensor()
+    pool.copy_(randn(5, *pool.shape))
+    q = randn(6, rows, QDIM)
+    out = run_attn(p, batch, i32(table), q).clone()
+    check_rows(p, batch, table, q, out, heads=(2, 15))
+    assert torch.equal(run_attn(p, batch, i32(table), q), out)
+    p.close()
+
+
 @pytest.mark.parametrize("nkvh", [1, 3, 16])
 def test_wide_other_head_counts(gpu, nkvh):
-    batch, ps = [(4000, 401), (100, 30), (700, 1)], 32
+    batch, ps = [(5200, 401), (100, 30), (700, 1)], 32
     assert_wide(batch)
     need = needed(batch, ps)
     table, _ = shuffled_table(random.Random(1), need, sum(need) + 1, max(need))
@@ -106,7 +126,7 @@ def test_wide_other_head_counts(gpu, nkvh):
 
 def test_wide_peaked_scores(gpu):
     """Scores of hundreds, and the running maximum moving late."""
-    batch, ps = [(2400, 600)], 64
+    batch, ps = [(3300, 600)], 64
     assert_wide(batch)
     need = needed(batch, ps)
     table, _ = shuffled_table(random.Random(1), need, sum(need), max(need))
@@ -120,7 +140,7 @@ def test_wide_peaked_scores(gpu):
 
 @pytest.mark.parametrize("bad", [float("nan"), float("-inf"), -65504.0])
 def test_wide_ignores_what_lies_behind_the_keys(gpu, bad):
-    batch, ps = [(2500, 513), (12, 1700), (30, 1)], 128
+    batch, ps = [(4000, 513), (12, 2100), (30, 1)], 128
     assert_wide(batch)
     need = needed(batch, ps)
     pages = sum(need) + 3
@@ -141,7 +161,7 @@ def test_wide_ignores_what_lies_behind_the_keys(gpu, bad):
 
 
 @pytest.mark.parametrize("what", ["k", "v"])
-@pytest.mark.parametrize("batch,at", [([(2500, 520)], 2777), ([(0, 1700)], 901), ([(8000, 200)], 8063)])
+@pytest.mark.parametrize("batch,at", [([(4000, 520)], 4277), ([(0, 2100)], 901), ([(10500, 200)], 10563)])
 def test_wide_infinities_reach_only_the_rows_that_see_them(gpu, batch, at, what):
     """A bad key of the new rows: the rows before it keep their values (within
     both runs' bounds), those that see it take what the definition gives."""
@@ -184,7 +204,7 @@ def test_wide_infinities_reach_only_the_rows_that_see_them(gpu, batch, at, what)
 
 def test_wide_leaves_evicted_pages_out(gpu):
     """Entries outside the pool, whole ranges of them and at a range's end."""
-    batch, ps = [(5000, 400), (0, 1800)], 16
+    batch, ps = [(5200, 400), (0, 2100)], 16
     assert_wide(batch)
     need = needed(batch, ps)
     pages = sum(need)
@@ -192,11 +212,11 @@ def test_wide_leaves_evicted_pages_out(gpu):
     gone = [x for t in (table[0][4:200], table[1][0:9]) for x in t]
     table[0][4:200] = [-1] * 196
     table[1][0:9] = [pages, 2 ** 31 - 1, -2 ** 31] * 3
-    p = Paged(pages, ps, 2, 2200, rope=False)
+    p = Paged(pages, ps, 2, 2500, rope=False)
     pool = p.pool.tensor()
     pool.copy_(randn(5, *pool.shape))
     pool[:, gone] = float("nan")
-    q = randn(6, 2200, QDIM)
+    q = randn(6, 2500, QDIM)
     d_table = i32(table)
     # The second request's own new rows lie on entries outside the pool: with
     # a given table such a request is refused, so it is planned on whole ones.
@@ -215,7 +235,7 @@ def test_wide_leaves_evicted_pages_out(gpu):
 
 
 def test_wide_bits_do_not_depend_on_the_batch_or_the_pages(gpu):
-    batch, ps = [(2500, 512), (900, 1), (5000, 300), (700, 1100)], 64
+    batch, ps = [(4000, 512), (900, 1), (7000, 300), (1500, 1100)], 64
     assert_wide(batch)
     need = needed(batch, ps)
     pages = 2 * sum(need)
@@ -238,7 +258,7 @@ def test_wide_bits_do_not_depend_on_the_batch_or_the_pages(gpu):
     p.close()
 
 
-@pytest.mark.parametrize("batch", [[(300, 5)], [(300, 14)], [(1800, 8)], [(2500, 530)]])
+@pytest.mark.parametrize("batch", [[(300, 5)], [(300, 14)], [(1800, 8)], [(4000, 530)]])
 def test_a_broken_query_reaches_only_its_own_row_and_head(gpu, batch):
     """NaN in one (row, q head): the other columns of its block are finite and
     right."""
@@ -367,7 +387,7 @@ def test_replayed_graph_of_changing_work(gpu):
     with torch.cuda.graph(graph):
         step(p.plan, out)
     for batch in ([(900, 1)] * 8, [(2000, 900), (1, 1), (3000, 1), (5, 0), (0, 16)], [(0, 0)],
-                  [(2100, 1)] * 5, [(2500, 700), (40, 40)], [(2500, 700), (40, 40)], [(0, 1)]):
+                  [(2100, 1)] * 5, [(2450, 750), (40, 40)], [(2450, 750), (40, 40)], [(0, 1)]):
         batch = batch + [(0, 0)] * (n - len(batch))
         lens.copy_(i32([c for c, _ in batch]))
         rows.copy_(i32([r for _, r in batch]))
@@ -384,7 +404,7 @@ def test_replayed_graph_of_changing_work(gpu):
 
 def test_on_another_stream(gpu):
     """Torch's current stream is the one that the calls run on."""
-    batch, ps = [(2500, 512), (900, 1)], 64
+    batch, ps = [(4000, 512), (900, 1)], 64
     need = needed(batch, ps)
     table, _ = shuffled_table(random.Random(2), need, sum(need), max(need))
     p = Paged(sum(need), ps, 2, 513, rope=False)
@@ -396,7 +416,7 @@ def test_on_another_stream(gpu):
         pool.copy_(randn(5, *pool.shape))  # ordered before the calls by the stream alone
         q.copy_(randn(6, 513, QDIM))
         d_table = i32(table)
-        Q.paged_plan(p.ctx, p.plan, i32([2500, 900]), i32([512, 1]), d_table)
+        Q.paged_plan(p.ctx, p.plan, i32([4000, 900]), i32([512, 1]), d_table)
         out = torch.zeros_like(q)
         Q.paged_attn(p.ctx, p.plan, 0, d_table, q, out)
         out2 = out.clone()
