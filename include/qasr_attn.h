@@ -296,7 +296,8 @@ int qasr_paged_plan_build(qasr_ctx* ctx, qasr_paged_plan* plan, int nreq, const 
 /* Stage (a) of the planned step's first `rows` rows (qkv_dev [rows][(nqh +
  * 2*nkvh)*hd]): roped Q -> q_out_dev [rows][nqh*hd], roped K and raw V -> row
  * row_slot[r] of the layer's pages.  The bits of qasr_qk_norm_rope_append.  A
- * row without a place is left out. */
+ * row without a place is left out.  All 16-byte aligned; q_out_dev apart from
+ * qkv_dev. */
 int qasr_paged_append(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows, const void* qkv_dev,
                       const void* q_gain_dev, const void* k_gain_dev, void* q_out_dev, void* stream);
 
@@ -305,8 +306,9 @@ int qasr_paged_append(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows,
  * keys 0..p.  table_dev: the table of the build, unchanged since.  Keys of
  * entries outside the pool (an evicted page, say -1) are left out; a row that
  * sees no key, or only scores of -inf, gives zeros.  Infinities and NaN in a key
- * or value reach the rows that see it and no others.  A request's output bits depend on its rows, length
- * and keys alone, not on its batch mates or where its pages lie. */
+ * or value reach the rows that see it and no others.  A request's output bits
+ * depend on its rows, length and keys alone, not on its batch mates or where its
+ * pages lie.  q_dev and out_dev are 16-byte aligned and do not overlap. */
 int qasr_paged_attn(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows,
                     const int32_t* table_dev, int table_stride, const void* q_dev, void* out_dev,
                     void* stream);

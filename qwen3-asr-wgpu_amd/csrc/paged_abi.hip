@@ -75,6 +75,15 @@ int check_layer_rows(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows) 
     return QASR_OK;
 }
 
+// Rows in and out: 16-byte loads and stores, and workgroups that read `in`
+// after others have written `out`.
+int check_arrays(const void* in, int64_t in_bytes, const void* out, int64_t out_bytes) {
+    const uintptr_t i = (uintptr_t)in, o = (uintptr_t)out;
+    if ((i | o) & 15) return fail(QASR_EINVAL, "rows must be 16-byte aligned");
+    if (i < o + out_bytes && o < i + in_bytes) return fail(QASR_EINVAL, "the output overlaps the input");
+    return QASR_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -274,6 +283,11 @@ int qasr_paged_append(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows,
     if (rc) return rc;
     if (rows == 0) return QASR_OK;
     if (!qkv_dev || !q_gain_dev || !k_gain_dev || !q_out_dev) return fail(QASR_EINVAL, "null device pointer");
+    const int nqh = ctx->cfg.num_attention_heads, heads = nqh + 2 * ctx->cfg.num_key_value_heads;
+    const int64_t head_bytes = (int64_t)rows * qasr::kHeadDim * sizeof(f16);
+    const int io = check_arrays(qkv_dev, heads * head_bytes, q_out_dev, nqh * head_bytes);
+    if (io) return io;
+    if (((uintptr_t)q_gain_dev | (uintptr_t)k_gain_dev) & 15) return fail(QASR_EINVAL, "gains must be 16-byte aligned");
     if (!ctx->cos) return fail(QASR_ESTATE, "RoPE tables not set (qasr_set_rope_tables)");
     DeviceScope ds(ctx->device);
     if (ds.err != hipSuccess) return hip_fail(ds.err, "hipSetDevice");
@@ -300,6 +314,9 @@ int qasr_paged_attn(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows, c
         return fail(QASR_EINVAL, "table_stride %d, the plan was built with %d", table_stride, plan->stride);
     if (rows == 0) return QASR_OK;
     if (!table_dev || !q_dev || !out_dev) return fail(QASR_EINVAL, "null device pointer");
+    const int64_t bytes = (int64_t)rows * ctx->cfg.num_attention_heads * qasr::kHeadDim * sizeof(f16);
+    const int io = check_arrays(q_dev, bytes, out_dev, bytes);
+    if (io) return io;
     DeviceScope ds(ctx->device);
     if (ds.err != hipSuccess) return hip_fail(ds.err, "hipSetDevice");
     const qasr::CacheGeom g = page_geom(plan->pool);

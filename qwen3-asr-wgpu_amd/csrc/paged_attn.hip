@@ -31,9 +31,9 @@
 //   (93.8 MB, 3.9 TB/s; a large copy reaches 5.2).
 // Chunks: MFMA and VALU work, which share the issue slots of a SIMD (two waves
 // overlap about half of the smaller part), at a clock that falls to 1.9 GHz:
-//   2 x 2048 rows at 4096 206 (172 GFLOP, 0.83 PFLOP/s; a large f16 product
+//   2 x 2048 rows at 4096 185-206 (172 GFLOP, 0.83-0.93 PFLOP/s; a large f16 product
 //   reaches 1.1-1.3), 512 at 7680 52 (0.64), 8 chunks of 7-45 rows at 200-1700
-//   17.2, 24 single rows of 100-2400 with 4 chunks of 100-450 rows 45.
+//   17-18, 24 single rows of 100-2400 with 4 chunks of 100-450 rows 45.
 // Also measured: 64-row items of 4 waves 223 us for the first of these, the
 // key groups half a tile apart 223; narrow items of 8 waves 5.7 against 4.8 us
 // for a single row's loop; 64-row blocks for every chunk 85 us for the last

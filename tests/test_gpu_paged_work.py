@@ -360,6 +360,66 @@ def test_most_requests(gpu):
     p.close()
 
 
+def test_largest_step(gpu):
+    """65536 rows of 1024 requests, some requests of one row, some large."""
+    rnd = random.Random(9)
+    rows = [1] * 300 + [700, 1500, 2100, 4000] + [rnd.randint(2, 130) for _ in range(719)]
+    rows.append(65536 - sum(rows))
+    rnd.shuffle(rows)
+    assert len(rows) == 1024 and min(rows) > 0
+    batch = [(rnd.choice([0, 1, rnd.randint(0, 700)]), r) for r in rows]
+    ps = 64
+    need = needed(batch, ps)
+    table, _ = shuffled_table(rnd, need, sum(need), max(need))
+    p = Paged(sum(need), ps, 1024, 65536, nkvh=1, rope=False)
+    pool = p.pool.tensor()
+    pool.copy_(randn(5, *pool.shape))
+    q = randn(6, 65536, 2 * HD)
+    out = run_attn(p, batch, i32(table), q)
+    assert p.plan.status.tolist() == [M.OK] * 1024
+    starts = p.plan.row_start.tolist()
+    assert starts[-1] == 65536
+    big = sorted(range(1024), key=lambda i: -rows[i])[:4]
+    for i in big + rnd.sample(range(1024), 24) + [0, 1023]:
+        r0, r1 = starts[i], starts[i + 1]
+        check_rows(p, batch[i:i + 1], table[i:i + 1], q[r0:r1], out[r0:r1], heads=(i % 2,))
+    p.close()
+
+
+@pytest.mark.parametrize("ps", [16, 64])
+def test_long_contexts_find_their_keys(gpu, ps):
+    """100000 keys on shuffled pages, ranges of many pages: a row whose query is
+    a multiple of one key gives that key's value.  Its score is 4 |k|^2 /
+    sqrt(128), 45 +- 6, the others' are normal with deviation s = 4 |k| /
+    sqrt(128), about 4, whose exponentials average e^(s^2/2), about e^8: 20 below
+    it and more, so all of them weigh less than 100000 e^-20."""
+    n, nkvh = 100000, 2
+    need = -(-(n + 1) // ps)
+    at = [0, 5, 511, 1700, 1791, 1792, 3124, 3125, 30000, 77777, n - 3, n - 1]
+    p = Paged(need, ps, len(at), len(at), nkvh=nkvh, max_seq=1 << 17, rope=False)
+    pool = p.pool.tensor()
+    pool.copy_(randn(5, *pool.shape))
+    ids = random.Random(1).sample(range(need), need)
+    q = torch.empty((len(at), 2 * nkvh, HD), dtype=torch.float16, device="cuda")
+    want = torch.empty_like(q)
+    for i, t in enumerate(at):
+        kv = pool[0, ids[t // ps], :, :, t % ps]
+        for h in range(2 * nkvh):
+            q[i, h], want[i, h] = 4 * kv[0, h // 2], kv[1, h // 2]
+    out = run_attn(p, [(n, 1)] * len(at), i32([ids] * len(at)), q.view(len(at), -1))
+    # two f16 roundings (the weight's and the result's) of values below 8, and
+    # the other keys
+    d = (out.view_as(want).double() - want.double()).abs().max().item()
+    assert d <= 2 * 2.0 ** -11 * 8 + 2 * 100000 * np.exp(-20.0) * 8, d
+    # not so when its page is gone
+    gone = list(ids)
+    gone[77777 // ps] = -1
+    out2 = run_attn(p, [(n, 1)], i32([gone]), q[9:10].view(1, -1))
+    assert bool(torch.isfinite(out2).all())
+    assert float((out2.view(-1).double() - want[9].view(-1).double()).abs().max()) > 0.5
+    p.close()
+
+
 def test_replayed_graph_of_changing_work(gpu):
     """One captured [plan, attention] over lengths and row counts that change
     between the replays: wide, split, single and no work at all, with eager
@@ -511,6 +571,13 @@ def test_calls_refuse(gpu):
     refused(Q.QASR_ERANGE, lambda: Q.paged_attn(ctx, plan, 0, table, q, out))
     refused(Q.QASR_EINVAL, lambda: Q.paged_attn(ctx, plan, 0, wide, q[:2], out))  # another stride
     refused(Q.QASR_EINVAL, lambda: Q.paged_attn(other.ctx, plan, 0, table, q[:2], out))
+    # outputs over inputs, and rows that 16-byte accesses cannot take
+    refused(Q.QASR_EINVAL, lambda: Q.paged_attn(ctx, plan, 0, table, q[:2], q[:2]))
+    refused(Q.QASR_EINVAL, lambda: Q.paged_attn(ctx, plan, 0, table, q[:2], q[1:3]))
+    refused(Q.QASR_EINVAL, lambda: Q.paged_append(ctx, plan, 0, qkv[:2], g, g, qkv.view(-1)[:2 * QDIM]))
+    odd = q.view(-1)[1:1 + 2 * QDIM].view(2, QDIM)
+    refused(Q.QASR_EINVAL, lambda: Q.paged_attn(ctx, plan, 0, table, odd, out))
+    refused(Q.QASR_EINVAL, lambda: Q.paged_append(ctx, plan, 0, qkv[:2], randn(2, HD + 1)[1:], g, q))
     # tensors of other types, devices and layouts
     for bad in (one[:2].long(), one[:2].cpu(), i32([1, 0, 1, 0])[::2]):
         with pytest.raises((Q.QasrError, ValueError, TypeError)):
