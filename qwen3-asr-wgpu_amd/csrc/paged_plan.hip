@@ -17,6 +17,8 @@
 // by a binary search of the prefix sums in LDS.  What may alias an input
 // (lengths and the cursor, updated in place by a replayed graph) is written
 // by the workgroup that arrives last, when every other has read it.
+// us a launch: 16 single rows 7.3, 256 requests of 220 single rows and 20 chunks
+// 15.8; with three scans and items by the row blocks' workgroups 43.
 
 #include "paged.hpp"
 
