@@ -242,8 +242,8 @@ __device__ __forceinline__ void merge_pairs(const float* src, int cols, int spli
         for (int k = 0; k < kUnits; ++k) {
             const int u = u0 + k * THREADS, p = u / cols, c = u - p * cols;
             if (u < units) {
-                const float inv = sums[c * splits];
-                const half2v y = {(f16)(o[k][0] * inv), (f16)(o[k][1] * inv)};
+                const float inv = sums[c * splits];  // 0: no key weighs anything, whatever o is
+                const half2v y = {(f16)(inv == 0.0f ? 0.0f : o[k][0] * inv), (f16)(inv == 0.0f ? 0.0f : o[k][1] * inv)};
                 res[c * pad + p] = __builtin_bit_cast(uint32_t, y);
             }
         }
@@ -373,7 +373,8 @@ __device__ __forceinline__ float not_finite(const float* o) {
 // states that are not finite.  The MFMA product weighs a hidden key with 0,
 // and 0 * inf is NaN: here hidden keys are left out, so infinities and NaN
 // reach only the rows that see them.  The weights are taken against the max
-// that the state has; lane l < 32 returns dim 32 db + l of row r, q head h.
+// that the state has (-inf: they are 0); lane l < 32 returns dim 32 db + l of
+// row r, q head h.
 __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& it, int key0, int key1, float M, int r,
                                             int h, int db, int lane) {
     const int pos = it.pos0 + r;
@@ -393,7 +394,7 @@ __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& 
 #pragma unroll
             for (int e = 0; e < 8; ++e) s = fmaf(h2f(x.e[e]), h2f(y.e[e]), s);
         }
-        const float p = fast_exp2(s * a.scale_log2 - M);
+        const float p = M == kNegInf ? 0.0f : fast_exp2(s * a.scale_log2 - M);  // (-inf) - (-inf): weighs nothing
         uint64_t todo = __ballot(seen);
         while (todo) {
             const int j = __builtin_ctzll(todo);
