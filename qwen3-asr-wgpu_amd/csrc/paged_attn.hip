@@ -373,13 +373,13 @@ __device__ __forceinline__ float not_finite(const float* o) {
 // states that are not finite.  The MFMA product weighs a hidden key with 0,
 // and 0 * inf is NaN: here hidden keys are left out, so infinities and NaN
 // reach only the rows that see them.  The weights are taken against the max
-// that the state has (-inf: they are 0); lane l < 32 returns dim 32 db + l of
-// row r, q head h.
+// that the state has (-inf: they are 0).  Lane l < 32 returns dim 32 db + l of
+// row r, q head h; `sum`: the sum of the weights.
 __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& it, int key0, int key1, float M, int r,
-                                            int h, int db, int lane) {
+                                            int h, int db, int lane, float& sum) {
     const int pos = it.pos0 + r;
     const f16* q = a.q + ((int64_t)(it.row0 + r) * a.nkvh + it.kvh) * (kRep * kHeadDim) + h * kHeadDim;
-    float o = 0.0f;
+    float o = 0.0f, l = 0.0f;
     for (int k0 = key0; k0 < min(key1, pos + 1); k0 += 64) {
         const int key = k0 + lane;
         const int id = it.table[min(key, it.kend - 1) >> a.page_shift];
@@ -395,6 +395,7 @@ __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& 
             for (int e = 0; e < 8; ++e) s = fmaf(h2f(x.e[e]), h2f(y.e[e]), s);
         }
         const float p = M == kNegInf ? 0.0f : fast_exp2(s * a.scale_log2 - M);  // (-inf) - (-inf): weighs nothing
+        l += seen ? p : 0.0f;
         uint64_t todo = __ballot(seen);
         while (todo) {
             const int j = __builtin_ctzll(todo);
@@ -404,10 +405,16 @@ __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& 
             o = fmaf(__shfl(p, j), h2f(it.base[at + a.kv_stride + 32 * db + (lane & 31)]), o);
         }
     }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+    sum = l;
     return o;
 }
 // Puts the columns of a wave whose dim block db (32 dims) is not finite.
-// every lane: its column's max and sum; valid columns only.
+// every lane: its column's max and sum; valid columns only.  The sum that the
+// state has is of weights rounded to f16 (weights()), those here are not: the
+// dims are divided by their own sum, and a range's state holds them times the
+// state's sum over theirs.
 __device__ __forceinline__ void put_exact(const PagedAttnArgs& a, const Item& it, int key0, int key1, float M, float L,
                                           int db, int r, int h, bool valid, uint32_t cols) {
     const int lane = thread_id() & 63;
@@ -417,15 +424,18 @@ __device__ __forceinline__ void put_exact(const PagedAttnArgs& a, const Item& it
         todo &= todo - 1;
         const int rj = __shfl(r, j), hj = __shfl(h, j);
         const float l = __shfl(L, j);
-        const float o = exact_dims(a, it, key0, key1, __shfl(M, j), rj, hj, db, lane);
+        float sum;
+        float o = exact_dims(a, it, key0, key1, __shfl(M, j), rj, hj, db, lane, sum);
         if (lane >= 32) continue;
-        if (it.splits == 1)
-            a.out[((int64_t)(it.row0 + rj) * a.nkvh + it.kvh) * (kRep * kHeadDim) + hj * kHeadDim + db * 32 + lane] =
-                f2h(l == 0.0f ? 0.0f : o / l);
-        else
+        if (it.splits == 1) {
+            o = l == 0.0f ? 0.0f : o / sum;
+            a.out[((int64_t)(it.row0 + rj) * a.nkvh + it.kvh) * (kRep * kHeadDim) + hj * kHeadDim + db * 32 + lane] = f2h(o);
+        } else {
+            o = l == 0.0f ? o : o * (l / sum);
             store_dev(range_o(a, it, it.split) + (db * 16 + (lane >> 1)) * it.rows * kRep * 2 +
                           column(it, rj, hj) * 2 + (lane & 1),
                       o);
+        }
     }
 }
 

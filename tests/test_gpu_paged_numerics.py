@@ -127,3 +127,90 @@ def test_only_scores_of_minus_infinity_give_zeros(gpu, c, r, bad):
     out = run_attn(p, [(c, r)], i32(table), q)
     assert bool((out == 0).all())
     p.close()
+
+
+# ---- columns computed again -------------------------------------------------
+
+def half_weight(lo=0.5, hi=0.51):
+    """f16 numbers (a, b) whose product as a score, a b / sqrt(128), has a
+    weight p = exp(score) in [lo, hi] that lies as far from an f16 number as
+    can be found, above it; and p."""
+    a = np.arange(1.0, 2.0, 2.0 ** -10)
+    b = -np.arange(6.0, 8.0, 2.0 ** -8)
+    assert np.array_equal(a.astype(np.float16), a) and np.array_equal(b.astype(np.float16), b)
+    p = np.exp(a[:, None] * b[None] * HD ** -0.5)
+    off = np.where((p >= lo) & (p <= hi), (p - p.astype(np.float16).astype(float)) / p, 0)
+    i, j = np.unravel_index(off.argmax(), off.shape)
+    assert off[i, j] > 4.5e-4
+    return float(a[i]), float(b[j]), float(p[i, j])
+
+
+def two_weights(pool, table, ps, n, every=8):
+    """Keys of one dim: every 8th has weight 1, the others half_weight()'s p.
+    Returns the query and p."""
+    a, b, w = half_weight()
+    set_keys(pool, table, ps, range(n), 0, 0.0)
+    keys = [k for k in range(n) if k % every]
+    pages, rows = at(table, ps, np.asarray(keys))
+    pool[0, pages, 0, :, rows, 0] = b
+    return a, w
+
+
+AGAIN = [(20, 5), (20, 12), (1500, 6), (1500, 12), (0, 2100), (10500, 200)]
+
+
+@pytest.mark.parametrize("c,r", AGAIN)
+def test_columns_computed_again_keep_a_constant_value(gpu, c, r):
+    """Every value is 2 - 2^-10, but one of the last row's is not finite: the
+    32 dims of it are computed again for all rows of the last row block.  A
+    weighted mean of a constant is the constant, however the weights are
+    rounded, as long as the mean divides by the sum of the same weights: the
+    longest f32 sum has 2100 terms (its divisor's 2100 / 64 a lane), which moves
+    the result by less than 2 * (2100 + 33 + 40) * 2^-24 = 2.6e-4, and half a step
+    of f16 below 2 is 4.9e-4."""
+    ps, value = 16, 2.0 - 2.0 ** -10
+    p, pool, table = one(c, r, ps)
+    a, _ = two_weights(pool, table, ps, c + r)
+    q = torch.zeros((r, QDIM), dtype=torch.float16, device="cuda")
+    q.view(r, NQH, HD)[:, :, 0] = a
+    set_keys(pool, table, ps, range(c + r), 1, value)
+    page, off = at(table, ps, c + r - 1)
+    pool[0, page, 1, :, off, 5] = INF
+    out = run_attn(p, [(c, r)], i32(table), q).view(r, NQH, HD)
+    assert bool(torch.isinf(out[-1, :, 5]).all())
+    out[-1, :, 5] = value
+    assert bool((out == value).all()), out[out != value][:4]
+    p.close()
+
+
+@pytest.mark.parametrize("c,r", [(30, 7), (900, 8), (2000, 5), (900, 14), (2500, 13), (300, 90)])
+@pytest.mark.parametrize("what", ["k", "v"])
+def test_columns_computed_again_against_64_bits(gpu, c, r, what):
+    """A bad key in the middle of the new rows: the rows before it, and where
+    its value is bad the other dims of the rows after it, are within the bound
+    of the definition."""
+    ps, row = 32, r // 2
+    p, pool, table = one(c, r, ps)
+    page, off = at(table, ps, c + row)
+    kept = pool[0, page, :, :, off].clone()
+    if what == "k":
+        pool[0, page, 0, :, off, 3] = NAN
+    else:
+        pool[0, page, 1, :, off, 5] = INF
+    q = randn(6, r, QDIM)
+    out = run_attn(p, [(c, r)], i32(table), q)
+    pool[0, page, :, :, off] = kept
+    check_rows(p, table, q, out, c, list(range(row)), heads=range(0, NQH, 3))
+    seers = out[row:].view(-1, NQH, HD)
+    if what == "k":
+        assert bool(torch.isnan(seers).all())
+    else:
+        assert bool(torch.isinf(seers[:, :, 5]).all())
+        pool[0, page, 1, :, off, 5] = 0.0  # a dim of its own: set alike on both sides
+        seers[:, :, 5] = 0
+        rows = list(range(row, r))
+        keep = pool.clone()
+        pool[:, :, 1, :, :, 5] = 0
+        check_rows(p, table, q, out, c, rows, heads=range(0, NQH, 3))
+        pool.copy_(keep)
+    p.close()
