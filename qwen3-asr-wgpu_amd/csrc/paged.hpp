@@ -5,7 +5,8 @@
 // d) is at base + layer*layer_stride + page*page_stride + kv*kv_stride +
 // head*head_stride + row*kHeadDim + d, so a (page, K or V, head) is one
 // contiguous block.  A request's position p lives in row p % rows of page
-// table[p / rows].
+// table[p / rows].  Behind the last layer lies one page of zeros, which stands
+// for table entries outside the pool.
 #pragma once
 
 #include "kernels.hpp"
@@ -146,6 +147,7 @@ struct PagedAttnArgs {
     int64_t page_stride, kv_stride, head_stride;
     const int32_t* table;
     int32_t stride, pages, page_shift, nkvh, rows;
+    int32_t zero_page;  // page of zeros behind the pool, counted from `base`
     float scale_log2;
     const int32_t* n_items;
     const PagedItem *narrow, *wide;

@@ -21,8 +21,8 @@ struct qasr_pages {
     int device;
     int32_t pages;
     int32_t shift;  // log2 of a page's rows
-    f16* base = nullptr;
-    size_t bytes = 0;
+    f16* base = nullptr;  // the layers' pages, then the zero page
+    size_t bytes = 0;     // without the zero page
 };
 
 struct qasr_paged_plan {
@@ -99,6 +99,8 @@ int qasr_pages_create(qasr_ctx* ctx, int pages, int page_rows, qasr_pages** out)
     if (pages <= 0) return fail(QASR_EINVAL, "pages must be > 0");
     if ((int64_t)pages << shift > std::numeric_limits<int32_t>::max())
         return fail(QASR_EINVAL, "%d pages of %d rows pass 2^31 rows", pages, page_rows);
+    if ((int64_t)pages * ctx->cfg.num_hidden_layers > std::numeric_limits<int32_t>::max())
+        return fail(QASR_ENOMEM, "%d pages of %d layers: more than a card holds", pages, ctx->cfg.num_hidden_layers);
     qasr_pages* p = new (std::nothrow) qasr_pages();
     if (!p) return fail(QASR_ENOMEM, "out of host memory");
     p->ctx = ctx;
@@ -106,10 +108,11 @@ int qasr_pages_create(qasr_ctx* ctx, int pages, int page_rows, qasr_pages** out)
     p->pages = pages;
     p->shift = shift;
     p->bytes = (size_t)page_geom(p).layer_stride * ctx->cfg.num_hidden_layers * sizeof(f16);
+    const size_t all = p->bytes + (size_t)page_geom(p).slot_stride * sizeof(f16);
     DeviceScope ds(ctx->device);
     hipError_t e = ds.err;
-    if (e == hipSuccess) e = hipMalloc(&p->base, p->bytes);
-    if (e == hipSuccess) e = hipMemset(p->base, 0, p->bytes);
+    if (e == hipSuccess) e = hipMalloc(&p->base, all);
+    if (e == hipSuccess) e = hipMemset(p->base, 0, all);
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) {
         if (p->base) (void)hipFree(p->base);
@@ -330,6 +333,7 @@ int qasr_paged_attn(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows, c
     a.table = table_dev;
     a.stride = table_stride;
     a.pages = plan->pool->pages;
+    a.zero_page = a.pages * (ctx->cfg.num_hidden_layers - layer);
     a.page_shift = plan->pool->shift;
     a.nkvh = g.nkvh;
     a.rows = rows;

@@ -131,7 +131,9 @@ __device__ __forceinline__ Offsets group_offsets(int lane, int add, int last, ui
 // + lo + l of the table, of the second the 64 after them.  The work item
 // brings the first 48 ids (lanes 16 .. 63, lo = -16), so that the first copies
 // wait for one load; longer ranges read on from the table.  An id outside the
-// pool sets its lane's bit in `bad` and reads page 0; its keys are hidden.
+// pool sets its lane's bit in `bad`, which hides its keys, and reads the zero
+// page: page 0, say, is another request's, whose infinities times a weight of 0
+// would be NaN here.
 struct PageRun {
     int id;
     uint64_t bad;
@@ -145,7 +147,7 @@ __device__ __forceinline__ int load_pages(const Item& it, int rel) {
 }
 __device__ __forceinline__ PageRun check_pages(const PagedAttnArgs& a, int id) {
     const bool bad = (uint32_t)id >= (uint32_t)a.pages;
-    return {bad ? 0 : id, __ballot(bad)};
+    return {bad ? a.zero_page : id, __ballot(bad)};
 }
 __device__ __forceinline__ int page_rel(const PagedAttnArgs& a, const Item& it, int key) {
     return (min(key, it.kend - 1) >> a.page_shift) - it.page0;

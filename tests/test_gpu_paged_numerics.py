@@ -214,3 +214,25 @@ def test_columns_computed_again_against_64_bits(gpu, c, r, what):
         check_rows(p, table, q, out, c, rows, heads=range(0, NQH, 3))
         pool.copy_(keep)
     p.close()
+
+
+# ---- what others hold -------------------------------------------------------
+
+@pytest.mark.parametrize("c,r,evicted", [(1000, 1, (4, 40)), (1000, 6, (0, 60)), (700, 12, (1, 30)),
+                                         (300, 100, (0, 18)), (5200, 400, (10, 300)), (0, 2100, (0, 0))])
+def test_bits_do_not_depend_on_the_pages_of_others(gpu, c, r, evicted):
+    """A request with evicted pages, beside one that holds page 0: whatever
+    page 0 holds, the first one's bits are the same."""
+    ps = 16
+    p, pool, table = one(c, r, ps, mate=1)
+    table[0][evicted[0]:evicted[1]] = [(-1, p.pool.pages, 2 ** 31 - 1)[i % 3] for i in range(*evicted)]
+    both = i32([table[0], [0] + [-1] * (len(table[0]) - 1)])
+    q = randn(6, r + 1, QDIM)
+    outs = []
+    for value in (0.5, NAN, INF, -INF, 65504.0):
+        pool[0, 0] = value
+        outs.append(run_attn(p, [(c, r), (7, 1)], both, q)[:r].clone())
+    for out in outs:
+        assert torch.equal(out, outs[0])
+    check_rows(p, table, q, outs[0], c, some_rows(r, random.Random(1)))
+    p.close()
