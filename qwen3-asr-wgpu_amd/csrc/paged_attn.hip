@@ -527,9 +527,12 @@ __device__ __forceinline__ void move_max(Wave& w, const float16v (&s)[NB]) {
     }
 }
 
-// The weights of a step's scores, as P^T (f16, B-operand layout), and their
-// row sum: of the rounded values, so that a rounding shifts weight between
-// keys and does not scale the row.  Four sums of v_fma_mix_f32, which runs
+// The weights of a step's scores, as P^T (B-operand layout), and their row sum.
+// They are rounded to f16, as in the slot pool's prefill: the product takes f16,
+// and two of them for each weight (Few) would be half as many MFMAs again where
+// MFMAs bound the time.  The sum is of the rounded values, so that a rounding
+// shifts weight between keys and does not scale the row: an output moves by at
+// most 2^-11 of the values' mean distance from it.  Four sums of v_fma_mix_f32, which runs
 // beside another wave's MFMAs; v_dot2_f32_f16 does not (MFMA and VALU work of
 // two waves a SIMD: no overlap with it, about half of the smaller part
 // without).
@@ -658,14 +661,25 @@ __device__ __forceinline__ void leave(Shared<NW>& sh, const Wave& w, int wave, i
 
 // Narrow items of up to 8 rows: their 16 columns on v_mfma_f32_16x16x32_f16,
 // whose products take half the time, with half the scores a lane.  us a layer
-// on 32 columns against 16: 1 row of 512 keys 8.4 / 7.7, of 8192 14.8 / 14.4, 16 rows
+// on 32 columns against 16 (f16 weights on both): 1 row of 512 keys 8.4 / 7.7, of 8192 14.8 / 14.4, 16 rows
 // of 400-2400 24.7 / 24.1.
+//
+// Their weights are held to 22 bits, as the slot pool's decode step holds them
+// in f32: a weight is a sum of two f16 numbers, hi and its remainder lo, each
+// with a product of its own.  (One f16 number moves an output by up to 2^-11 of
+// the values' spread, about as much again as its own rounding.)  Exponents are
+// taken against the running maximum less 7, so that the largest weight is 2^7
+// to 2^15 and lo holds down to 2^-32 of it; f16 ends at 65504.  us a layer with
+// one product and with two: 1 row of 512 keys 7.6 / 7.9, of 8192 14.4 / 14.6, 16
+// rows of 400-2400 24.2 / 24.3.
 constexpr int kFewRows = 8;
+constexpr float kFewBase = 7.0f;
+static_assert(kFewBase + kRescaleSlack < 16.0f, "weights fit f16");
 struct Few {
     static constexpr int kRows = kFewRows;
     half8v qb[4];  // Q^T of k-step ks: dims 32*ks + 8*g .. +8 of query n
     float4v o[8];  // O^T: o[db][i] = dim db*16 + 4*g + i of query n
-    float m, l;
+    float m, l;    // the running maximum less kFewBase, and the sum of weights
     int kaddr[4];  // K operand of k-step ks, rows 0..15 (halves)
     int vbase;
     int g, qpos;  // g: the lane's quarter
@@ -705,8 +719,8 @@ __device__ __forceinline__ void wait_q(Few& w) {
     for (int ks = 0; ks < 4; ++ks) asm volatile("" : "+v"(w.qb[ks]));
 }
 // P^T of a slice: S^T of keys 16 kb + 4 g + i, masked, the running maximum,
-// the weights (B operand: its k 8 g + j is key 16 (j / 4) + 4 g + j % 4) and
-// their sum.
+// the weights (B operand: its k 8 g + j is key 16 (j / 4) + 4 g + j % 4), hi and
+// lo, and their sum.
 __device__ __forceinline__ void slice_scores(const Few& w, const f16* kt, float4v (&s)[2]) {
     half8v ka[8];
     auto read = [&](int x) { ka[x] = *(const half8v*)&kt[(x & 1) * 16 * kHeadDim + w.kaddr[x >> 1]]; };
@@ -722,7 +736,7 @@ __device__ __forceinline__ void slice_scores(const Few& w, const f16* kt, float4
         keep_order();
     }
 }
-__device__ __forceinline__ void slice_weights(Few& w, float4v (&s)[2], int k0, bool mask, uint32_t hidden, half8v (&pb)[1]) {
+__device__ __forceinline__ void slice_weights(Few& w, float4v (&s)[2], int k0, bool mask, uint32_t hidden, half8v (&pb)[2]) {
     if (mask) {
         const int last = w.qpos - k0 - 4 * w.g;
 #pragma unroll
@@ -735,7 +749,7 @@ __device__ __forceinline__ void slice_weights(Few& w, float4v (&s)[2], int k0, b
     float mx = kNegInf;
 #pragma unroll
     for (int j = 0; j < 8; ++j) mx = fmaxf(mx, s[j >> 2][j & 3]);
-    mx = quarters_max(mx) * w.scale_log2;
+    mx = quarters_max(mx) * w.scale_log2 - kFewBase;
     const bool up = mx > w.m + kRescaleSlack;
     if (__ballot(up)) {
         if (rarely(__ballot(up && w.m != kNegInf))) {
@@ -750,13 +764,19 @@ __device__ __forceinline__ void slice_weights(Few& w, float4v (&s)[2], int k0, b
     float ps[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        pb[0][j] = (f16)softmax_w_raw(s[j >> 2][j & 3], w.scale_log2, mu);
-        ps[j & 1] += (float)pb[0][j];
+        const float p = softmax_w_raw(s[j >> 2][j & 3], w.scale_log2, mu);
+        pb[0][j] = (f16)p;
+        pb[1][j] = (f16)(p - (float)pb[0][j]);
+        ps[j & 1] += p;
     }
     w.l += quarters_sum(ps[0] + ps[1]);
 }
-__device__ __forceinline__ void slice_product(Few& w, const f16* vt, const half8v (&pb)[1]) {
-    half4v lo[8], hi[8];
+__device__ __forceinline__ void slice_product(Few& w, const f16* vt, const half8v (&pb)[2]) {
+    half4v lo[8], hi[8];  // keys 0..15 and 16..31
+    auto add = [&](int x, int part) {
+        w.o[x] = mfma16(__builtin_shufflevector(lo[x], hi[x], 0, 1, 2, 3, 4, 5, 6, 7), pb[part], w.o[x]);
+        keep_order();
+    };
     auto read = [&](int x) {
         const f16* vp = vt + w.vbase + (x >> 1) * (kSlice * 32) + (x & 1) * 16;
         lo[x] = read_tr(vp);
@@ -769,9 +789,11 @@ __device__ __forceinline__ void slice_product(Few& w, const f16* vt, const half8
     for (int x = 0; x < 8; ++x) {
         if (x + 4 < 8) read(x + 4);
         keep_order();
-        w.o[x] = mfma16(__builtin_shufflevector(lo[x], hi[x], 0, 1, 2, 3, 4, 5, 6, 7), pb[0], w.o[x]);
-        keep_order();
+        add(x, 0);
+        if (x >= 2) add(x - 2, 1);  // not right behind the product it adds to
     }
+    add(6, 1);
+    add(7, 1);
 }
 template <int NW>
 __device__ __forceinline__ void leave_all(Shared<NW>& sh, const Few& w, int wave, int lane) {
@@ -884,7 +906,7 @@ __device__ __forceinline__ void run_narrow(const PagedAttnArgs& a, const Item& i
 
 __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it, Pages pg, Shared<kNarrowWaves>& sh, Draw& next) {
     if (it.planned <= kFewRows)
-        run_narrow<Few, float4v, 2, 1>(a, it, pg, sh, next);
+        run_narrow<Few, float4v, 2, 2>(a, it, pg, sh, next);
     else
         run_narrow<Many, float16v, 1, 2>(a, it, pg, sh, next);
     if (it.splits > 1) arrive(a, it, sh);

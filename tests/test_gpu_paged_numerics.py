@@ -236,3 +236,75 @@ def test_bits_do_not_depend_on_the_pages_of_others(gpu, c, r, evicted):
         assert torch.equal(out, outs[0])
     check_rows(p, table, q, outs[0], c, some_rows(r, random.Random(1)))
     p.close()
+
+
+# ---- the weights' bits --------------------------------------------------------
+
+@pytest.mark.parametrize("c,r", [(300, 1), (250, 8), (767, 1), (760, 3), (2000, 2), (40, 24)])
+def test_few_rows_hold_their_weights_to_22_bits(gpu, c, r):
+    """Items of up to 8 rows, a lone row's among them, weigh keys as the slot
+    pool's decode step does: not rounded to f16.  Every 8th key has weight 1
+    and value 1, the others weight p, just above an f16 number by 4.8e-4 of
+    it, and value -1/4: the mean of n1 keys and n2 others is (n1 - n2 p / 4) /
+    (n1 + n2 p), and f16 weights move it by about 1e-4, while it is about 0.03
+    and its own f16 rounding 1.5e-5.
+    Scores are single products: 3 roundings of an exponent near 1, exp2's error
+    and the split of a weight (2^-22) are below 2^-20 of it together.  A wave
+    adds the two products of each key of its quarter of the keys (n / 2 f32
+    sums), then the waves and up to 32 ranges join; the weights' own sum has n /
+    16 terms a lane: (0.6 n + 80) 2^-24 of the mean |v|."""
+    ps = 16
+    p, pool, table = one(c, r, ps)
+    a, w = two_weights(pool, table, ps, c + r)
+    q = torch.zeros((r, QDIM), dtype=torch.float16, device="cuda")
+    q.view(r, NQH, HD)[:, :, 0] = a
+    ones = range(0, c + r, 8)
+    set_keys(pool, table, ps, range(c + r), 1, -0.25)
+    set_keys(pool, table, ps, ones, 1, 1.0)
+    out = run_attn(p, [(c, r)], i32(table), q).double().cpu().numpy()
+    rows = range(r) if r <= 8 else range(16, r)  # the last row block of a chunk
+    for row in rows:
+        n = c + row + 1
+        n1 = len(range(0, n, 8))
+        n2 = n - n1
+        want = (n1 - 0.25 * n2 * w) / (n1 + n2 * w)
+        f16 = float(np.float16(w))
+        moved = abs((n1 - 0.25 * n2 * f16) / (n1 + n2 * f16) - want)
+        mean = (n1 + 0.25 * n2 * w) / (n1 + n2 * w)
+        allow = (2.0 ** -20 + (0.6 * n + 80) * 2.0 ** -24) * mean + 2.0 ** -11 * abs(want) + 2.0 ** -25
+        assert moved > 2 * allow, "f16 weights would pass"
+        assert np.abs(out[row] - want).max() <= allow, (row, np.abs(out[row] - want).max(), allow, moved)
+    p.close()
+
+
+@pytest.mark.parametrize("c,r", [(500, 1), (500, 8), (1500, 2)])
+def test_few_rows_keep_small_weights(gpu, c, r):
+    """Weights of about 2^-16 of the largest, which f16 holds to 9 bits, and
+    values of 1000 on them: one key of weight 1 and value 1 a slice, the others
+    b.  The result's f16 rounding is 2^-11 of it, the exponent of 16 is off by
+    2^-20 and exp2 by less (2^-19), a weight below 2^-21 is held to 2^-32 of the
+    largest, and the f32 sums move it by (0.6 n + 80) 2^-24."""
+    ps = 16
+    a = 1.0
+    b = float(np.float16(-16.56 * np.log(2.0) * HD ** 0.5))
+    w = float(np.exp(a * b * HD ** -0.5))
+    near = float(np.float16(w))
+    assert abs(near - w) / w > 2.5e-3
+    p, pool, table = one(c, r, ps)
+    set_keys(pool, table, ps, range(c + r), 0, 0.0)
+    small = [k for k in range(c + r) if k % 16]
+    pages, rows = at(table, ps, np.asarray(small))
+    pool[0, pages, 0, :, rows, 0] = b
+    set_keys(pool, table, ps, range(c + r), 1, 0.0)
+    set_keys(pool, table, ps, small, 1, 1000.0)
+    q = torch.zeros((r, QDIM), dtype=torch.float16, device="cuda")
+    q.view(r, NQH, HD)[:, :, 0] = a
+    out = run_attn(p, [(c, r)], i32(table), q).double().cpu().numpy()
+    for row in range(r):
+        n = c + row + 1
+        n1 = len(range(0, n, 16))
+        n2 = n - n1
+        want = 1000 * n2 * w / (n1 + n2 * w)
+        allow = want * (2.0 ** -11 + 2.0 ** -19 + 2.0 ** -32 / w + (0.6 * n + 80) * 2.0 ** -24)
+        assert np.abs(out[row] - want).max() <= allow, (row, out[row][:2], want, allow)
+    p.close()
