@@ -27,17 +27,19 @@ constexpr int kPad = kHeadDim + 8;    // f16 raw heads: padded rows
 constexpr int kSqPad = kHeadDim + 4;  // f32 squares: lanes reading head h at the same j sit 4 banks apart
 
 // Where row `row` of a paged step goes: its position, page and row within the
-// page.  A row that the plan gave no place, or whose map entries lie outside
-// the pool or the tables, gets a readable place and false: nothing of it is
-// stored.
-__device__ __forceinline__ bool map_row(const RowMap& P, int row, int& pos, int& slot, int& at) {
+// page.  A row that the plan gave no position, or one outside the tables, gets
+// a readable one and placed = false: nothing of it is stored.  Without a slot
+// in the pool (its page came as an id outside it) it has no K and V, stored =
+// false, but it attends the keys before it, so its Q is roped.
+__device__ __forceinline__ void map_row(const RowMap& P, int row, int& pos, int& slot, int& at, bool& placed,
+                                        bool& stored) {
     pos = P.pos[row];
     const int s = P.slot[row];
-    const bool ok = (uint32_t)pos < (uint32_t)P.rope_rows && (uint32_t)s < (uint32_t)P.slots;
-    pos = ok ? pos : 0;
-    slot = ok ? s >> P.page_shift : 0;
-    at = ok ? s & ((1 << P.page_shift) - 1) : 0;
-    return ok;
+    placed = (uint32_t)pos < (uint32_t)P.rope_rows;
+    stored = placed && (uint32_t)s < (uint32_t)P.slots;
+    pos = placed ? pos : 0;
+    slot = stored ? s >> P.page_shift : 0;
+    at = stored ? s & ((1 << P.page_shift) - 1) : 0;
 }
 
 // Per row, one memory round trip and one serial chain: the raw q/k heads go
@@ -83,14 +85,14 @@ __global__ __launch_bounds__(kRowThreads) void norm_rope_append_kernel(
     }
     // Then the row's segment (position, slot) and the gains and cos/sin row.
     int pos, slot, at;
-    bool ok = true;
+    bool placed = true, stored = true;
     if constexpr (std::is_same_v<Rows, SegPlan>) {
         int sg = 0;
         while (sg + 1 < P.nseg && P.row_base[sg + 1] <= row) ++sg;
         at = pos = P.pos0[sg] + (row - P.row_base[sg]);
         slot = P.slot[sg];
     } else {
-        ok = map_row(P, row, pos, slot, at);
+        map_row(P, row, pos, slot, at, placed, stored);
     }
     f16* kdst = g.base + slot * g.slot_stride + layer * g.layer_stride + (int64_t)at * kHeadDim;
     f16* vdst = kdst + g.kv_stride;
@@ -128,7 +130,7 @@ __global__ __launch_bounds__(kRowThreads) void norm_rope_append_kernel(
         }
     }
     if (tid < 64) *(uint4*)&s_aux[(tid >> 4) * kHeadDim + (tid & 15) * 8] = a;
-    if (vt >= 0 && ok) *(uint4*)(vdst + (vt >> 4) * g.head_stride + (vt & 15) * 8) = v;
+    if (vt >= 0 && stored) *(uint4*)(vdst + (vt >> 4) * g.head_stride + (vt & 15) * 8) = v;
     __syncthreads();
     if (tid < nh) s_inv[tid] = head_inv_rms_squares_all(&s_sq[tid * kSqPad], P.eps);
     __syncthreads();
@@ -141,7 +143,7 @@ __global__ __launch_bounds__(kRowThreads) void norm_rope_append_kernel(
         const f16* gain = is_q ? &s_aux[0] : &s_aux[kHeadDim];
         const float inv = s_inv[h];
         const uint4 o = rope8(&s_raw[h * kPad], gain, crow, srow, inv, j0);
-        if (!ok) continue;
+        if (!(is_q ? placed : stored)) continue;
         if (is_q)
             *(uint4*)(q_out + (int64_t)row * nqh * kHeadDim + h * kHeadDim + j0) = o;
         else
@@ -188,7 +190,7 @@ __global__ __launch_bounds__(64) void norm_rope_many_kernel(
     // The row's segment: the number of later segment starts at or before it
     // (lane i reads segment i's fields; the arrays hold 64).
     int pos, slot, at;
-    bool ok = true;
+    bool placed = true, stored = true;
     if constexpr (std::is_same_v<Rows, SegPlan>) {
         static_assert(kMaxBatch == 64, "one lane per segment");
         const int e_slot = P.slot[lane], e_pos = P.pos0[lane], e_r0 = P.row_base[lane], e_r1 = P.row_base[lane + 1];
@@ -196,7 +198,7 @@ __global__ __launch_bounds__(64) void norm_rope_many_kernel(
         at = pos = __builtin_amdgcn_readlane(e_pos, sg) + row - __builtin_amdgcn_readlane(e_r0, sg);
         slot = __builtin_amdgcn_readlane(e_slot, sg);
     } else {
-        ok = map_row(P, row, pos, slot, at);
+        map_row(P, row, pos, slot, at, placed, stored);
     }
     f16* kdst = g.base + slot * g.slot_stride + layer * g.layer_stride + (int64_t)at * kHeadDim;
     f16* vdst = kdst + g.kv_stride;
@@ -219,7 +221,7 @@ __global__ __launch_bounds__(64) void norm_rope_many_kernel(
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const int it = lane + 64 * k;
-        if (it < nv && ok) *(uint4*)(vdst + (it >> 4) * g.head_stride + (it & 15) * 8) = v[k].u;
+        if (it < nv && stored) *(uint4*)(vdst + (it >> 4) * g.head_stride + (it & 15) * 8) = v[k].u;
     }
     __syncthreads();  // one wave: its LDS writes have completed
     float inv = 0.0f;
@@ -229,7 +231,7 @@ __global__ __launch_bounds__(64) void norm_rope_many_kernel(
         const int h = h0 + 8 * k;
         H8 o[2];
         rope16(x[k], gn[k], c, sn, __shfl(inv, h), o);
-        if (h < nh && ok) {
+        if (h < nh && (h < nqh ? placed : stored)) {
             f16* dst = h < nqh ? q_out + ((int64_t)row * nqh + h) * kHeadDim : kdst + (h - nqh) * g.head_stride;
             *(uint4*)(dst + 8 * w) = o[0].u;
             *(uint4*)(dst + 8 * w + kHeadDim / 2) = o[1].u;
