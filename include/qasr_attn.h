@@ -271,11 +271,14 @@ int qasr_paged_plan_get_info(const qasr_paged_plan* plan, qasr_paged_plan_info* 
  * cursor_dev[0] on (the ring wraps), in request order, and are entered in the
  * table; pages of ended requests go to the ring's end and are free from the
  * next step on.  ring_dev and cursor_dev NULL: the table holds the new rows'
- * pages already.
+ * pages already.  The ring's ids are entered as they are: rows on one that is
+ * outside the pool have a position but no slot, are stored nowhere and seen by
+ * none.
  *
  * The step's rows are the requests' new rows one after the other.  A request
  * is placed whole or not at all: status_dev[i] is QASR_EINVAL for a negative
- * length, rows below -1, or a page of the new rows outside the pool;
+ * length, rows below -1, or a page of the new rows that the table holds and
+ * that is outside the pool;
  * QASR_ERANGE for positions past max_seq, the RoPE tables or table_stride *
  * page_rows, or rows past max_rows; QASR_ENOMEM when the free pages do not
  * reach (nor for any later request that needs one).  Rows of refused requests
@@ -296,8 +299,8 @@ int qasr_paged_plan_build(qasr_ctx* ctx, qasr_paged_plan* plan, int nreq, const 
 /* Stage (a) of the planned step's first `rows` rows (qkv_dev [rows][(nqh +
  * 2*nkvh)*hd]): roped Q -> q_out_dev [rows][nqh*hd], roped K and raw V -> row
  * row_slot[r] of the layer's pages.  The bits of qasr_qk_norm_rope_append.  A
- * row without a place is left out.  All 16-byte aligned; q_out_dev apart from
- * qkv_dev. */
+ * row without a position is left out, of one without a slot only Q is written.
+ * All 16-byte aligned; q_out_dev apart from qkv_dev. */
 int qasr_paged_append(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows, const void* qkv_dev,
                       const void* q_gain_dev, const void* k_gain_dev, void* q_out_dev, void* stream);
 
