@@ -278,20 +278,23 @@ int qasr_paged_plan_get_info(const qasr_paged_plan* plan, qasr_paged_plan_info* 
  * The step's rows are the requests' new rows one after the other.  A request
  * is placed whole or not at all: status_dev[i] is QASR_EINVAL for a negative
  * length, rows below -1, or a page of the new rows that the table holds and
- * that is outside the pool;
- * QASR_ERANGE for positions past max_seq, the RoPE tables or table_stride *
- * page_rows, or rows past max_rows; QASR_ENOMEM when the free pages do not
- * reach (nor for any later request that needs one).  Rows of refused requests
- * keep their places in the step, are neither stored nor attended, and their
- * outputs are left as they were; so are those behind the last row.
+ * that is outside the pool; QASR_ERANGE for positions past max_seq, the RoPE
+ * tables or table_stride * page_rows, or rows past max_rows; QASR_ENOMEM when
+ * the free pages do not reach (nor for any later request that needs one).  Rows
+ * of refused requests keep their places in the step, are neither stored nor
+ * attended, and their outputs are left as they were; so are those behind the
+ * last row.
  *
  * len_dev may be the plan's own lens_dev and cursor_dev its cursor_dev: then
- * each build goes on where the last one ended.  The arrays must be distinct
- * otherwise.  A table may list one page for several requests (a shared prefix),
- * as long as none of them stores rows in it: a request's first new row goes
- * into its last page while that has room, so a shared prefix is whole pages.  A
- * page that two ended requests give back is twice in the ring: end all but the
- * last of its requests with their shared entries set to -1. */
+ * each build goes on where the last one ended.  Arrays that lie in the plan's
+ * memory otherwise, and a ring, or a table with a ring, that overlaps another
+ * array, are refused.
+ *
+ * A table may list one page for several requests (a shared prefix), as long as
+ * none of them stores rows in it: a request's first new row goes into its last
+ * page while that has room, so a shared prefix is whole pages.  A page that two
+ * ended requests give back is twice in the ring: end all but the last of its
+ * requests with their shared entries set to -1. */
 int qasr_paged_plan_build(qasr_ctx* ctx, qasr_paged_plan* plan, int nreq, const int32_t* len_dev,
                           const int32_t* rows_dev, int32_t* table_dev, int table_stride,
                           int32_t* ring_dev, const int32_t* cursor_dev, void* stream);

@@ -84,6 +84,34 @@ int check_arrays(const void* in, int64_t in_bytes, const void* out, int64_t out_
     return QASR_OK;
 }
 
+// What a build's workgroups all read, none of them may write before the last
+// has read it: they would plan different requests, and one count work items
+// that another never wrote.  Only the plan's lens and cursor are written by the
+// workgroup that arrives last.  Fresh table entries are written, and pages given
+// back to the ring, where no one reads them: only with a ring.
+struct Range {
+    uintptr_t at;
+    int64_t bytes;
+    bool meets(const Range& o) const {
+        return at && o.at && bytes > 0 && o.bytes > 0 && at < o.at + o.bytes && o.at < at + bytes;
+    }
+};
+int check_build_arrays(const qasr_paged_plan* p, int nreq, const int32_t* len, const int32_t* rows, const int32_t* table,
+                       int stride, const int32_t* ring, const int32_t* cursor) {
+    if (((uintptr_t)len | (uintptr_t)rows | (uintptr_t)table | (uintptr_t)ring | (uintptr_t)cursor) & 3)
+        return fail(QASR_EINVAL, "an array of 32-bit numbers is not 4-byte aligned");
+    const Range own{(uintptr_t)p->mem, (int64_t)p->bytes}, t{(uintptr_t)table, (int64_t)nreq * stride * 4},
+        g{(uintptr_t)ring, (int64_t)p->pool->pages * 4}, l{(uintptr_t)len, (int64_t)nreq * 4},
+        r{(uintptr_t)rows, (int64_t)nreq * 4}, c{(uintptr_t)cursor, 8};
+    if (t.meets(own) || g.meets(own) || r.meets(own) || (len != p->lens && l.meets(own)) ||
+        (cursor != p->cursor && c.meets(own)))
+        return fail(QASR_EINVAL, "an array lies in the plan's own (only its lens and cursor may)");
+    if (!ring) return QASR_OK;
+    if (t.meets(g) || t.meets(l) || t.meets(r) || t.meets(c) || g.meets(l) || g.meets(r) || g.meets(c))
+        return fail(QASR_EINVAL, "the table or the ring overlaps another array");
+    return QASR_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -249,6 +277,8 @@ int qasr_paged_plan_build(qasr_ctx* ctx, qasr_paged_plan* plan, int nreq, const 
     if (table_stride < 1) return fail(QASR_EINVAL, "table_stride must be > 0");
     if (!len_dev || !rows_dev || !table_dev) return fail(QASR_EINVAL, "null device pointer");
     if (!ring_dev != !cursor_dev) return fail(QASR_EINVAL, "ring and cursor go together");
+    const int ar = check_build_arrays(plan, nreq, len_dev, rows_dev, table_dev, table_stride, ring_dev, cursor_dev);
+    if (ar) return ar;
     DeviceScope ds(ctx->device);
     if (ds.err != hipSuccess) return hip_fail(ds.err, "hipSetDevice");
     qasr::PagedPlanArgs a;

@@ -1,4 +1,5 @@
-"""Paged steps at their edges: pages that the pool does not have."""
+"""Paged steps at their edges: pages that the pool does not have, arrays that
+overlap."""
 from __future__ import annotations
 
 import random
@@ -54,4 +55,56 @@ def test_rows_on_a_page_outside_the_pool_attend_what_is_before_them(gpu, rows):
     assert torch.equal(pool, want)
     check_attn(p, [(start, rows)], table, q, out, heads=(0, 15))
     ref.close()
+    p.close()
+
+
+# ---- what a build takes -----------------------------------------------------
+
+def refused(fn):
+    with pytest.raises(Q.QasrError) as e:
+        fn()
+    assert e.value.code == Q.QASR_EINVAL, e.value
+
+
+def test_build_refuses_arrays_that_overlap(gpu):
+    """What one workgroup of a build writes and another reads, save the plan's
+    lens and cursor in their own places."""
+    n, pages, width = 4, 16, 3
+    p = Paged(pages, 16, n, 16, rope=False)
+    c, plan = p.ctx, p.plan
+    lens, rows, cursor = i32([3] * n), i32([1] * n), i32([0, pages])
+    ring, table = i32(list(range(pages))), i32([[i, -1, -1] for i in range(n)])
+    build = lambda *a: refused(lambda: Q.paged_plan(c, plan, *a))  # noqa: E731
+    # in the plan's own memory
+    build(plan.lens, plan.lens, table, ring, cursor)
+    build(lens, plan.status, table, ring, cursor)
+    build(plan.row_pos, rows, table, ring, cursor)
+    build(plan.row_start[1:], rows, table, ring, cursor)
+    build(lens, rows, plan.row_slot[:n * width].view(n, width), ring, cursor)
+    build(lens, rows, plan.row_slot[:n * width].view(n, width))
+    build(lens, rows, table, plan.row_pos, cursor)
+    build(lens, rows, table, ring, plan.row_start[:2])
+    # each other's
+    a = i32([0] * 64)
+    view = lambda at: a[at:at + n * width].view(n, width)  # noqa: E731
+    build(lens, rows, view(0), a[n * width - 1:n * width - 1 + pages], cursor)
+    build(a[n * width - 1:][:n], rows, view(0), ring, cursor)
+    build(lens, a[:n], view(n - 1), ring, cursor)
+    build(lens, rows, view(0), ring, a[1:3])
+    build(a[pages - 1:pages - 1 + n], rows, table, a[:pages], cursor)
+    build(lens, a[4:4 + n], table, a[:pages], cursor)
+    build(lens, rows, table, a[:pages], a[pages - 1:pages + 1])
+    lib = Q.load()
+    assert lib.qasr_paged_plan_build(c.handle, plan.handle, n, lens.data_ptr() + 2, rows.data_ptr(), table.data_ptr(),
+                                     width, None, None, None) == Q.QASR_EINVAL
+    # side by side in one allocation, lens and rows the same array, and in place
+    a[:n * width] = table.view(-1)
+    a[12:28], a[28:30], a[30:34], a[34:38] = ring, i32([4, 12]), lens, rows
+    Q.paged_plan(c, plan, a[30:34], a[34:38], view(0), a[12:28], a[28:30])
+    assert plan.status.tolist() == [0] * n and plan.lens.tolist() == [4] * n
+    Q.paged_plan(c, plan, rows, rows, table)
+    assert plan.status.tolist() == [0] * n and plan.lens.tolist() == [2] * n
+    plan.cursor.copy_(i32([4, 12]))
+    Q.paged_plan(c, plan, plan.lens, rows, table, ring, plan.cursor)
+    assert plan.status.tolist() == [0] * n and plan.lens.tolist() == [3] * n
     p.close()
