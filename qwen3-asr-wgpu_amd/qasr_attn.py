@@ -495,6 +495,8 @@ class PagePool:
         self.pages, self.page_rows = pages, page_rows
 
     def info(self) -> PagesInfo:
+        if not self.ctx.handle:
+            raise QasrError(QASR_ESTATE, "the context is closed")
         inf = PagesInfo()
         _check(load().qasr_pages_get_info(self.handle, ctypes.byref(inf)))
         return inf
@@ -584,7 +586,8 @@ class PagedPlan:
 
     @property
     def handle(self):
-        return self._mem.handle
+        """None once the plan or its pool is closed: calls on it are refused."""
+        return self._mem.handle if self.pool.handle else None
 
     def close(self):
         """Free the plan now; its views must not be used any more."""

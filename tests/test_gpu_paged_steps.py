@@ -1,5 +1,5 @@
 """Paged steps at their edges: pages that the pool does not have, arrays that
-overlap."""
+overlap, closed objects."""
 from __future__ import annotations
 
 import random
@@ -11,7 +11,7 @@ torch = pytest.importorskip("torch")
 import qasr_attn as Q  # noqa: E402
 from gpu_helpers import Gpu  # noqa: E402
 from test_gpu_paged import Paged, check_attn, i32, randn  # noqa: E402
-from workloads import HD, QDIM, TOT  # noqa: E402
+from workloads import HD, NKVH, NQH, QDIM, TOT  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +108,40 @@ def test_build_refuses_arrays_that_overlap(gpu):
     Q.paged_plan(c, plan, plan.lens, rows, table, ring, plan.cursor)
     assert plan.status.tolist() == [0] * n and plan.lens.tolist() == [3] * n
     p.close()
+
+
+def test_calls_on_a_closed_pool_are_refused(gpu):
+    """A plan whose pool or context is closed: its calls are refused, and it can
+    still be closed."""
+    def make():
+        ctx = Q.Context(NQH, NKVH, HD, 1, 1e-6, 128, 0)
+        pool = Q.PagePool(ctx, 4, 16)
+        plan = Q.PagedPlan(ctx, pool, 2, 4)
+        table = i32([[0], [1]])
+        Q.paged_plan(ctx, plan, i32([3, 3]), i32([1, 1]), table)
+        torch.cuda.synchronize()
+        q, out = randn(1, 2, QDIM), torch.zeros((2, QDIM), dtype=torch.float16, device="cuda")
+        qkv, g = randn(2, 2, TOT), randn(3, HD)
+
+        def calls():
+            refused(lambda: Q.paged_plan(ctx, plan, i32([3, 3]), i32([1, 1]), table))
+            refused(lambda: Q.paged_attn(ctx, plan, 0, table, q, out))
+            refused(lambda: Q.paged_append(ctx, plan, 0, qkv, g, g, out))
+
+        return ctx, pool, plan, calls
+
+    ctx, pool, plan, calls = make()
+    pool.close()
+    calls()
+    refused(lambda: pool.info())
+    refused(lambda: Q.PagedPlan(ctx, pool, 1, 1))
+    plan.close()
+    ctx.close()
+    ctx, pool, plan, calls = make()
+    ctx.close()
+    calls()
+    with pytest.raises(Q.QasrError):
+        pool.tensor()
+    plan.close()
+    calls()
+    pool.close()
