@@ -256,9 +256,11 @@ typedef struct qasr_paged_plan_info {
 
 /* A plan for up to max_requests (<= QASR_PAGED_MAX_REQUESTS) requests and
  * max_rows (<= QASR_PAGED_MAX_ROWS) new rows together in a step.  Its memory
- * is mostly the attention's split workspace: min(32 * max_rows, 2048 *
- * max_requests) records of (128 + 2) floats per q head (67 MB for 256 rows and
- * 16 q heads). */
+ * is mostly the attention's split workspace: min(S * max_rows, 2048 *
+ * max_requests) records of (128 + 2) floats per q head, S = min(32, ceil(max_seq
+ * / 512)) of the context, none for S = 1.  With 16 q heads and S = 32 that is 68
+ * MB for 256 rows, 1.1 GB for 4096 rows of 256 requests, 17 GB for the largest
+ * plan; a context of 2048 positions takes an eighth. */
 int qasr_paged_plan_create(qasr_ctx* ctx, qasr_pages* pool, int max_requests, int max_rows,
                            qasr_paged_plan** out);
 void qasr_paged_plan_destroy(qasr_paged_plan* plan);

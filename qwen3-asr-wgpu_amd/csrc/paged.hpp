@@ -84,8 +84,8 @@ static_assert(sizeof(PagedItem) == 64 * 4, "a word a lane");
 
 // Capacities for max_requests requests and max_rows rows together.  A
 // request has at most max(kPagedMaxItems, blocks) items and, split, rows *
-// splits records: at most kPagedMaxSplits a row and kPagedMaxSplits *
-// kWideRows in all.
+// splits records: at most kPagedMaxSplits a row, no more than a context of
+// max_seq positions has ranges, and kPagedMaxSplits * kWideRows in all.
 static_assert(kPagedMaxItems * kNarrowRows <= kPagedMaxSplits * kWideRows && kPagedMaxItems >= kPagedMaxSplits &&
                   kPagedMaxItems / (kPagedManyBlocks + 1) <= kPagedMaxSplits,
               "splits and records of a request");
@@ -93,8 +93,12 @@ inline int64_t paged_max_blocks(int64_t requests, int64_t rows) { return request
 inline int64_t paged_max_items(int64_t requests, int64_t rows, int64_t rows_a_block) {
     return requests * kPagedMaxItems + requests + rows / rows_a_block;
 }
-inline int64_t paged_max_records(int64_t requests, int64_t rows) {
-    const int64_t a = rows * kPagedMaxSplits, b = requests * kPagedMaxSplits * kWideRows;
+static_assert(kPagedRangeKeys <= kPagedManyRangeKeys, "the shorter range bounds the splits");
+inline int64_t paged_max_records(int64_t requests, int64_t rows, int64_t max_seq) {
+    const int64_t ranges = (max_seq + kPagedRangeKeys - 1) / kPagedRangeKeys;
+    if (ranges <= 1) return 0;  // nothing is split
+    const int64_t a = rows * (ranges < kPagedMaxSplits ? ranges : kPagedMaxSplits);
+    const int64_t b = requests * kPagedMaxSplits * kWideRows;
     return a < b ? a : b;
 }
 

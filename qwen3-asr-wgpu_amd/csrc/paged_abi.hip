@@ -196,7 +196,7 @@ int qasr_paged_plan_create(qasr_ctx* ctx, qasr_pages* pool, int max_requests, in
     p->max_narrow = (int32_t)qasr::paged_max_items(max_requests, max_rows, qasr::kNarrowRows);
     p->max_wide = (int32_t)qasr::paged_max_items(max_requests, max_rows, qasr::kWideRows);
     const int64_t blocks = qasr::paged_max_blocks(max_requests, max_rows) * nkvh;
-    const int64_t recs = qasr::paged_max_records(max_requests, max_rows) * nkvh * qasr::kRep;
+    const int64_t recs = qasr::paged_max_records(max_requests, max_rows, ctx->cfg.max_seq) * nkvh * qasr::kRep;
     // One allocation, each part from a multiple of 256 bytes; the parts up to
     // `clear` start at zero (counters, and a plan that was never built has no
     // items).

@@ -1,5 +1,5 @@
 """Paged steps at their edges: pages that the pool does not have, arrays that
-overlap, closed objects."""
+overlap, closed objects, the size of a plan."""
 from __future__ import annotations
 
 import random
@@ -10,7 +10,7 @@ torch = pytest.importorskip("torch")
 
 import qasr_attn as Q  # noqa: E402
 from gpu_helpers import Gpu  # noqa: E402
-from test_gpu_paged import Paged, check_attn, i32, randn  # noqa: E402
+from test_gpu_paged import Paged, check_attn, i32, randn, run_attn, shuffled_table  # noqa: E402
 from workloads import HD, NKVH, NQH, QDIM, TOT  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -145,3 +145,37 @@ def test_calls_on_a_closed_pool_are_refused(gpu):
     plan.close()
     calls()
     pool.close()
+
+
+@pytest.mark.parametrize("max_seq,ranges", [(400, 0), (512, 0), (513, 2), (2048, 4), (5000, 10), (16384, 32), (1 << 20, 32)])
+def test_a_plan_holds_no_more_split_state_than_its_context_needs(gpu, max_seq, ranges):
+    """Records of 130 floats a q head: a key range of 512 keys or more a record
+    for each row, at most 32 ranges a row and 2048 records a request.  Beside
+    them a plan has items, counters and row maps, below 5 MB here."""
+    ctx = Q.Context(NQH, NKVH, HD, 1, 1e-6, max_seq, 0)
+    pool = Q.PagePool(ctx, 4, 16)
+    for n, rows in ((1, 1), (64, 64), (3, 4096), (64, 2048)):
+        plan = Q.PagedPlan(ctx, pool, n, rows)
+        state = min(rows * ranges, n * 2048 if ranges else 0) * NQH * 130 * 4
+        assert state <= plan.bytes <= state + 5e6, (n, rows, state, plan.bytes)
+        plan.close()
+    pool.close()
+    ctx.close()
+
+
+@pytest.mark.parametrize("max_seq,batch", [(513, [(512, 1), (0, 513), (505, 8)]), (1024, [(1023, 1), (1000, 24), (900, 124)]),
+                                           (2048, [(2047, 1), (1800, 248), (0, 2048), (1500, 548)])])
+def test_positions_up_to_the_last_of_a_short_context(gpu, max_seq, batch):
+    """The split state of a plan for exactly these rows is as short as it gets."""
+    ps = 16
+    need = [-(-(c + r) // ps) for c, r in batch]
+    table, _ = shuffled_table(random.Random(1), need, sum(need), max(need))
+    rows = sum(r for _, r in batch)
+    p = Paged(sum(need), ps, len(batch), rows, max_seq=max_seq, rope=False)
+    pool = p.pool.tensor()
+    pool.copy_(randn(5, *pool.shape))
+    q = randn(6, rows, QDIM)
+    out = run_attn(p, batch, i32(table), q)
+    assert p.plan.status.tolist() == [0] * len(batch)
+    check_attn(p, batch, i32(table), q, out, heads=(0, 13))
+    p.close()

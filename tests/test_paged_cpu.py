@@ -106,3 +106,13 @@ def test_shapes_fit_the_workspaces():
 def test_plan_paged_refuses():
     for length, rows in ((-1, 1), (0, 0), (0, -3), ((1 << 24) + 1, 1), (0, 65537)):
         _refused(lambda: Q.plan_paged(length, rows))
+
+
+def test_ranges_of_a_short_context():
+    """A plan's split state counts on it: no request of a context of max_seq
+    positions has more than ceil(max_seq / 512) ranges."""
+    for max_seq in (1, 511, 512, 513, 1024, 1025, 2048, 5000, 16384):
+        for rows in {1, 2, 15, 16, 17, 64, 65, 255, 256, 257, 300, 513, 1000, 4000, max_seq}:
+            for length in {0, 1, 500, max_seq // 2, max_seq - rows - 1, max_seq - rows}:
+                if length >= 0 and length + rows <= max_seq:
+                    assert Q.plan_paged(length, rows)[2] <= -(-max_seq // 512)
