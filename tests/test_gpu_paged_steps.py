@@ -1,5 +1,6 @@
 """Paged steps at their edges: pages that the pool does not have, arrays that
-overlap, closed objects, the size of a plan."""
+overlap, closed objects, the size of a plan, other head counts, fewer rows than
+planned."""
 from __future__ import annotations
 
 import random
@@ -55,6 +56,71 @@ def test_rows_on_a_page_outside_the_pool_attend_what_is_before_them(gpu, rows):
     assert torch.equal(pool, want)
     check_attn(p, [(start, rows)], table, q, out, heads=(0, 15))
     ref.close()
+    p.close()
+
+
+@pytest.mark.parametrize("nkvh", [1, 5, 9, 16])
+@pytest.mark.parametrize("batch", [[(20, 1), (0, 37), (15, 2)], [(3, 300), (1000, 1), (0, 640)]])
+def test_append_of_other_head_counts_has_the_bits_of_stage_a(gpu, nkvh, batch):
+    """Up to 24 heads and more, few rows and many."""
+    ps, tot, qd = 32, 4 * nkvh * HD, 2 * nkvh * HD
+    lens, rows = [c for c, _ in batch], [r for _, r in batch]
+    total = sum(rows)
+    need = [-(-(c + r) // ps) for c, r in batch]
+    table, _ = shuffled_table(random.Random(3), need, sum(need) + 2, max(need))
+    p = Paged(sum(need) + 2, ps, len(batch), total + 3, nkvh=nkvh)
+    pool = p.pool.tensor()
+    pool.copy_(randn(1, *pool.shape))
+    want = pool.clone()
+    qkv, g = randn(2, total + 3, tot), randn(3, 2, HD) + 1
+    q = torch.full((total + 3, qd), 7.0, dtype=torch.float16, device="cuda")
+    Q.paged_plan(p.ctx, p.plan, i32(lens), i32(rows), i32(table))
+    Q.paged_append(p.ctx, p.plan, 0, qkv, g[0], g[1], q)
+    kv = Q.KVPool(p.ctx, len(batch), max(c + r for c, r in batch))
+    q_ref = torch.empty((total, qd), dtype=torch.float16, device="cuda")
+    Q.qk_norm_rope_append(p.ctx, kv, 0, [(i, c, r) for i, (c, r) in enumerate(batch)], qkv, g[0], g[1], q_ref)
+    assert torch.equal(q[:total], q_ref) and bool((q[total:] == 7).all())
+    slots = kv.tensor()
+    for i, (c, r) in enumerate(batch):
+        for pos in range(c, c + r):
+            want[0, table[i][pos // ps], :, :, pos % ps] = slots[i, 0, :, :, pos]
+    assert torch.equal(pool, want)
+    kv.close()
+    p.close()
+
+
+# ---- attention --------------------------------------------------------------
+
+@pytest.mark.parametrize("batch,cuts", [([(1500, 12)], (1, 5, 8, 9, 11)), ([(1500, 8)], (1, 3)),
+                                        ([(5000, 300)], (17, 160, 289)), ([(10500, 200)], (1, 63, 64, 65, 190)),
+                                        ([(0, 2100)], (1, 100, 2099)),
+                                        ([(900, 1), (4000, 512), (40, 20)], (1, 2, 200, 513, 520))])
+def test_fewer_rows_than_planned(gpu, batch, cuts):
+    """Row blocks and key ranges cut short by the caller's rows, wide and
+    split: the rows there are come out, those behind stay, and the plan serves
+    the whole step afterwards."""
+    ps = 16
+    need = [-(-(c + r) // ps) for c, r in batch]
+    table, _ = shuffled_table(random.Random(1), need, sum(need), max(need))
+    rows = sum(r for _, r in batch)
+    p = Paged(sum(need), ps, len(batch), rows, rope=False)
+    pool = p.pool.tensor()
+    pool.copy_(randn(5, *pool.shape))
+    q = randn(6, rows, QDIM)
+    d_table = i32(table)
+    whole = run_attn(p, batch, d_table, q).clone()
+    check_attn(p, batch, d_table, q, whole, heads=(3,))
+    for cut in cuts:
+        out = torch.full_like(q, 7.0)
+        Q.paged_attn(p.ctx, p.plan, 0, d_table, q[:cut], out)
+        assert bool((out[cut:] == 7).all())
+        left, part = cut, []
+        for c, r in batch:
+            part.append((c, min(r, left)))
+            left -= part[-1][1]
+        check_attn(p, part, d_table, q[:cut], out[:cut], heads=(3,))
+        Q.paged_attn(p.ctx, p.plan, 0, d_table, q, out)
+        assert torch.equal(out, whole)
     p.close()
 
 
