@@ -158,6 +158,99 @@ __device__ __forceinline__ void dma_q(u32x4v qr, int row0, int last_row, int ldq
     }
 }
 
+// First half of a step over NB * 32 keys: S^T from K rows kt[0 .. 32 NB - 1]
+// (first key k0), row max, the running-max update, P^T (f16, B-operand
+// layout) and its row sum.  MASK: some key is past some row's position.
+template <bool MASK, int NB>
+__device__ __forceinline__ void step_s(Wave& w, const f16* kt, int k0, half8v (&pb)[2 * NB]) {
+    // S^T: keys kb*32 + (8*(i/4) + 4*g + i%4) x query n, accumulated over dims.
+    float16v s[NB];
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb) s[kb] = (float16v){};
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb) {
+            const half8v ka = *(const half8v*)&kt[kb * 32 * kHeadDim + w.kaddr[ks]];
+            s[kb] = mfma32(ka, w.qb[ks], s[kb]);
+        }
+    // Operand reads run at most two k-steps ahead of the MFMAs (bounded
+    // register lifetime; 8 NB reads + 8 NB MFMAs).
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * NB, 0);
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NB, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, NB, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2 * NB, 0);
+    float mx = kNegInf;
+#pragma unroll
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (MASK) {
+                const int key = k0 + kb * 32 + 8 * (i >> 2) + 4 * w.g + (i & 3);
+                s[kb][i] = key > w.qpos ? kNegInf : s[kb][i];
+            }
+            mx = fmaxf(mx, s[kb][i]);
+        }
+    mx = halves_max(mx) * w.scale_log2;
+    // Move the running max when a row max passed it by more than the slack.
+    {
+        const bool up = mx > w.m + kRescaleSlack;
+        if (__ballot(up)) {
+            const float mn = up ? mx : w.m;
+            const float alpha = w.m == kNegInf ? 0.0f : fast_exp2(w.m - mn);
+#pragma unroll
+            for (int db = 0; db < 4; ++db) w.o[db] *= alpha;
+            w.l *= alpha;
+            w.m = mn;
+        }
+    }
+    const float mu = w.m == kNegInf ? 0.0f : w.m;
+    // P^T = 2^(s*scale_log2 - m), k-step w4 covering keys 16*w4 + 4*g +
+    // {0..3, 8..11}; the row sum from the same f16 values (v_dot2, f32 sum).
+#pragma unroll
+    for (int w4 = 0; w4 < 2 * NB; ++w4)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            pb[w4][j] = (f16)softmax_w_raw(s[w4 >> 1][8 * (w4 & 1) + j], w.scale_log2, mu);
+    const half2v ones2 = {(f16)1.0f, (f16)1.0f};
+    float ps = 0.0f;
+#pragma unroll
+    for (int w4 = 0; w4 < 2 * NB; ++w4)
+#pragma unroll
+        for (int q2 = 0; q2 < 4; ++q2) {
+            const half2v pr = {pb[w4][2 * q2], pb[w4][2 * q2 + 1]};
+            ps = __builtin_amdgcn_fdot2(pr, ones2, ps, false);
+        }
+    w.l += halves_sum(ps);
+}
+
+// Second half: O^T += V^T P^T with V rows vt[0 .. 32 NB - 1] (slab stride
+// kTileKeys*32 halves).
+template <int NB>
+__device__ __forceinline__ void step_pv(Wave& w, const f16* vt, const half8v (&pb)[2 * NB]) {
+#pragma unroll
+    for (int w4 = 0; w4 < 2 * NB; ++w4)
+#pragma unroll
+        for (int db = 0; db < 4; ++db) {
+            const f16* vp = vt + w.vbase + db * (kTileKeys * 32) + w4 * 16 * 32;
+            const half4v lo = read_tr(vp);
+            const half4v hi = read_tr(vp + 8 * 32);
+            const half8v va = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            w.o[db] = mfma32(va, pb[w4], w.o[db]);
+        }
+    // Two transposing reads per MFMA, at most two MFMAs ahead.
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < 8 * NB - 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+}
+
 // Merge of the nsp split-K partials of one wave's 32 rows (lane = query row),
 // for accumulator element chunks C0 .. C0+NC-1 (chunk k = elements 8k .. 8k+7
 // = o[k / 2][8 (k % 2) .. +8]): returns the merged row sum and leaves the
@@ -645,7 +738,7 @@ __global__ __launch_bounds__(NW * 64, 1) void prefill_attn_kernel(
                 step_s<false, NB>(w, kh, k0, pb);
             else
                 step_s<true, NB>(w, kh, k0, pb);
-            step_pv<kTileKeys, NB>(w, vh, pb);
+            step_pv<NB>(w, vh, pb);
         }
         if constexpr (SLICE) {
             if (t + 2 < t_end) {
