@@ -374,20 +374,22 @@ __device__ __forceinline__ float not_finite(const float* o) {
 // One column's output dims again, in f32 and key by key, by one wave: for
 // states that are not finite.  The MFMA product weighs a hidden key with 0,
 // and 0 * inf is NaN: here hidden keys are left out, so infinities and NaN
-// reach only the rows that see them.  The weights are taken against the max
-// that the state has (-inf: they are 0).  Lane l < 32 returns dim 32 db + l of
-// row r, q head h; `sum`: the sum of the weights.
-__device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& it, int key0, int key1, float M, int r,
-                                            int h, int db, int lane, float& sum) {
-    const int pos = it.pos0 + r;
+// reach only the rows that see them.  Lane l < 32 returns dim 32 db + l of row
+// r, q head h; `sum`: the sum of the weights, which are taken against these
+// scores' own maximum (-inf: they are 0), as the sums of the MFMA round
+// otherwise.
+__device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& it, int key0, int key1, int r, int h,
+                                            int db, int lane, float& sum) {
+    const int pos = it.pos0 + r, end = min(key1, pos + 1);
     const f16* q = a.q + ((int64_t)(it.row0 + r) * a.nkvh + it.kvh) * (kRep * kHeadDim) + h * kHeadDim;
-    float o = 0.0f, l = 0.0f;
-    for (int k0 = key0; k0 < min(key1, pos + 1); k0 += 64) {
+    // This lane's key of the 64 from k0 on: its row, whether it is seen, and its
+    // score.
+    auto score = [&](int k0, uint64_t& row, bool& seen) {
         const int key = k0 + lane;
         const int id = it.table[min(key, it.kend - 1) >> a.page_shift];
-        const bool seen = key < key1 && key <= pos && (uint32_t)id < (uint32_t)a.pages;
-        const uint64_t row = (uint64_t)(uint32_t)(seen ? id : 0) * (uint32_t)a.page_stride +
-                             (key & ((1 << a.page_shift) - 1)) * kHeadDim;
+        seen = key < end && (uint32_t)id < (uint32_t)a.pages;
+        row = (uint64_t)(uint32_t)(seen ? id : 0) * (uint32_t)a.page_stride +
+              (key & ((1 << a.page_shift) - 1)) * kHeadDim;
         float s = 0.0f;
         for (int d = 0; d < kHeadDim; d += 8) {
             H8 x, y;
@@ -396,7 +398,20 @@ __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& 
 #pragma unroll
             for (int e = 0; e < 8; ++e) s = fmaf(h2f(x.e[e]), h2f(y.e[e]), s);
         }
-        const float p = M == kNegInf ? 0.0f : fast_exp2(s * a.scale_log2 - M);  // (-inf) - (-inf): weighs nothing
+        return s * a.scale_log2;
+    };
+    uint64_t row;
+    bool seen;
+    float M = kNegInf, l = 0.0f, o = 0.0f;
+    for (int k0 = key0; k0 < end; k0 += 64) {
+        const float s = score(k0, row, seen);
+        M = fmaxf(M, seen ? s : kNegInf);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d));
+    for (int k0 = key0; k0 < end; k0 += 64) {
+        const float s = score(k0, row, seen);
+        const float p = M == kNegInf ? 0.0f : softmax_w_scaled(s, M);  // (-inf) - (-inf): weighs nothing
         l += seen ? p : 0.0f;
         uint64_t todo = __ballot(seen);
         while (todo) {
@@ -413,12 +428,12 @@ __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& 
     return o;
 }
 // Puts the columns of a wave whose dim block db (32 dims) is not finite.
-// every lane: its column's max and sum; valid columns only.  The sum that the
-// state has is of weights rounded to f16 (weights()), those here are not: the
-// dims are divided by their own sum, and a range's state holds them times the
+// every lane: its column's sum; valid columns only.  The sum that the state has
+// is of weights against another maximum, rounded to f16 (weights()): the dims
+// are divided by their own sum, and a range's state holds them times the
 // state's sum over theirs.
-__device__ __forceinline__ void put_exact(const PagedAttnArgs& a, const Item& it, int key0, int key1, float M, float L,
-                                          int db, int r, int h, bool valid, uint32_t cols) {
+__device__ __forceinline__ void put_exact(const PagedAttnArgs& a, const Item& it, int key0, int key1, float L, int db,
+                                          int r, int h, bool valid, uint32_t cols) {
     const int lane = thread_id() & 63;
     uint64_t todo = __ballot(valid) & cols;  // a lane a column: those of g = 0
     while (todo) {
@@ -427,7 +442,7 @@ __device__ __forceinline__ void put_exact(const PagedAttnArgs& a, const Item& it
         const int rj = __shfl(r, j), hj = __shfl(h, j);
         const float l = __shfl(L, j);
         float sum;
-        float o = exact_dims(a, it, key0, key1, __shfl(M, j), rj, hj, db, lane, sum);
+        float o = exact_dims(a, it, key0, key1, rj, hj, db, lane, sum);
         if (lane >= 32) continue;
         if (it.splits == 1) {
             o = l == 0.0f ? 0.0f : o / sum;
@@ -506,9 +521,17 @@ __device__ __forceinline__ void hide_scores(float16v (&s)[NB], uint32_t hidden) 
             for (int i = 0; i < 8; ++i) s[j >> 1][8 * (j & 1) + i] = kNegInf;
 }
 
-// The running maximum moves when a score passes it by more than the slack.
+// The running maximum moves when a score passes it by more than the slack.  A
+// weight is then 2^(s * e.scale - e.base).  The scale is fused into the
+// subtraction, which leaves the rounding of the scaled maximum in it: next to
+// nothing, but 1 and more for maxima past 2^24, and the weights would pass f16.
+// Scores that large are scaled and reduced here, one rounding after the other.
+constexpr float kLargeScore = 1 << 20;
+struct Exponent {
+    float scale, base;
+};
 template <int NB>
-__device__ __forceinline__ void move_max(Wave& w, const float16v (&s)[NB]) {
+__device__ __forceinline__ Exponent move_max(Wave& w, float16v (&s)[NB]) {
     float mx = kNegInf;
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb)
@@ -516,7 +539,8 @@ __device__ __forceinline__ void move_max(Wave& w, const float16v (&s)[NB]) {
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[kb][i]);
     mx = halves_max(mx) * w.scale_log2;
     const bool up = mx > w.m + kRescaleSlack;
-    if (__ballot(up)) {
+    Exponent e{w.scale_log2, w.m};
+    if (__ballot(up || !(fabsf(mx) < kLargeScore))) {
         if (rarely(__ballot(up && w.m != kNegInf))) {  // not at the first keys
             const float alpha = !up ? 1.0f : w.m == kNegInf ? 0.0f : fast_exp2(w.m - mx);
 #pragma unroll
@@ -524,7 +548,19 @@ __device__ __forceinline__ void move_max(Wave& w, const float16v (&s)[NB]) {
             w.l *= alpha;
         }
         w.m = up ? mx : w.m;
+        e.base = w.m;
+        if (rarely(__ballot(fabsf(mx) >= kLargeScore && mx != kNegInf))) {
+#pragma clang fp contract(off)
+            const float base = w.m == kNegInf ? 0.0f : w.m;
+#pragma unroll
+            for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[kb][i] = s[kb][i] * w.scale_log2 - base;
+            e = {1.0f, 0.0f};
+        }
     }
+    e.base = e.base == kNegInf ? 0.0f : e.base;
+    return e;
 }
 
 // The weights of a step's scores, as P^T (B-operand layout), and their row sum.
@@ -537,8 +573,7 @@ __device__ __forceinline__ void move_max(Wave& w, const float16v (&s)[NB]) {
 // two waves a SIMD: no overlap with it, about half of the smaller part
 // without).
 template <int NB>
-__device__ __forceinline__ void weights(Wave& w, const float16v (&s)[NB], half8v (&pb)[2 * NB]) {
-    const float mu = w.m == kNegInf ? 0.0f : w.m;
+__device__ __forceinline__ void weights(Wave& w, const float16v (&s)[NB], const Exponent& e, half8v (&pb)[2 * NB]) {
     float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w4 = 0; w4 < 2 * NB; ++w4) {
@@ -547,7 +582,7 @@ __device__ __forceinline__ void weights(Wave& w, const float16v (&s)[NB], half8v
             uint32_t u[4];
         } p;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p.h[j] = (f16)softmax_w_raw(s[w4 >> 1][8 * (w4 & 1) + j], w.scale_log2, mu);
+        for (int j = 0; j < 8; ++j) p.h[j] = (f16)softmax_w_raw(s[w4 >> 1][8 * (w4 & 1) + j], e.scale, e.base);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             asm("v_fma_mix_f32 %0, 1.0, %1, %0 op_sel_hi:[0,1,0]" : "+v"(ps[j]) : "v"(p.u[j]));
@@ -737,6 +772,7 @@ __device__ __forceinline__ void slice_scores(const Few& w, const f16* kt, float4
     }
 }
 __device__ __forceinline__ void slice_weights(Few& w, float4v (&s)[2], int k0, bool mask, uint32_t hidden, half8v (&pb)[2]) {
+#pragma clang fp contract(off)
     if (mask) {
         const int last = w.qpos - k0 - 4 * w.g;
 #pragma unroll
@@ -746,10 +782,16 @@ __device__ __forceinline__ void slice_weights(Few& w, float4v (&s)[2], int k0, b
 #pragma unroll
         for (int j = 0; j < 8; ++j) s[j >> 2][j & 3] = hidden >> (j >> 2) & 1 ? kNegInf : s[j >> 2][j & 3];
     }
+    // (Scaled first: a largest score minus itself is 0 then.  A fused multiply
+    // and subtract leaves the rounding of the maximum, which past 2^24 is 1 and
+    // more, and the weights would pass f16.)
     float mx = kNegInf;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, s[j >> 2][j & 3]);
-    mx = quarters_max(mx) * w.scale_log2 - kFewBase;
+    for (int j = 0; j < 8; ++j) {
+        s[j >> 2][j & 3] *= w.scale_log2;
+        mx = fmaxf(mx, s[j >> 2][j & 3]);
+    }
+    mx = quarters_max(mx) - kFewBase;
     const bool up = mx > w.m + kRescaleSlack;
     if (__ballot(up)) {
         if (rarely(__ballot(up && w.m != kNegInf))) {
@@ -764,7 +806,7 @@ __device__ __forceinline__ void slice_weights(Few& w, float4v (&s)[2], int k0, b
     float ps[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float p = softmax_w_raw(s[j >> 2][j & 3], w.scale_log2, mu);
+        const float p = softmax_w_scaled(s[j >> 2][j & 3], mu);
         pb[0][j] = (f16)p;
         pb[1][j] = (f16)(p - (float)pb[0][j]);
         ps[j & 1] += p;
@@ -815,8 +857,8 @@ __device__ __forceinline__ void slice_scores(const Many& w, const f16* kt, float
 __device__ __forceinline__ void slice_weights(Many& w, float16v (&s)[1], int k0, bool mask, uint32_t hidden, half8v (&pb)[2]) {
     if (mask) mask_scores<1>(w, s, k0);
     if (rarely(hidden)) hide_scores<1>(s, hidden);
-    move_max<1>(w, s);
-    weights<1>(w, s, pb);
+    const Exponent e = move_max<1>(w, s);
+    weights<1>(w, s, e, pb);
 }
 __device__ __forceinline__ void slice_product(Many& w, const f16* vt, const half8v (&pb)[2]) { product<kSlice, 1>(w, vt, pb); }
 template <int NW>
@@ -897,7 +939,7 @@ __device__ __forceinline__ void run_narrow(const PagedAttnArgs& a, const Item& i
         t = not_finite<kElems>(o) + 0.0f * L;
     }
     if (rarely(__ballot(t != t)))
-        put_exact(a, it, it.tile0 * kNarrowTile, min(it.tile1 * kNarrowTile, it.kend), M, L, wave, rin, h, valid,
+        put_exact(a, it, it.tile0 * kNarrowTile, min(it.tile1 * kNarrowTile, it.kend), L, wave, rin, h, valid,
                   kCols == 32 ? ~0u : 0xffffu);
     else if (valid)
         put_dims(a, it, o, L, wave, w.g, rin, h);
@@ -951,8 +993,8 @@ __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it,
         scores<2>(w, kt, s);
         if (k0 + kGroup - 1 > first_pos) mask_scores<2>(w, s, k0);
         if (rarely(hidden)) hide_scores<2>(s, hidden);
-        move_max<2>(w, s);
-        weights<2>(w, s, pb);
+        const Exponent e = move_max<2>(w, s);
+        weights<2>(w, s, e, pb);
         product<kWideTile, 2>(w, sh.buf + (t & 1) * 2 * kTile + kTile + kg * kGroup * 32, pb);
     }
     draw(next);
@@ -970,7 +1012,7 @@ __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it,
         combine<2, 16>(sh, rw, 4, db * 16, lane, o, M, L);
         const float t = not_finite<16>(o) + 0.0f * L;
         if (rarely(__ballot(valid && t != t)))
-            put_exact(a, it, it.tile0 * kWideTile, min(it.tile1 * kWideTile, it.kend), M, L, db, rin, h, valid, ~0u);
+            put_exact(a, it, it.tile0 * kWideTile, min(it.tile1 * kWideTile, it.kend), L, db, rin, h, valid, ~0u);
         else if (valid)
             put_block<4>(a, it, o, L, db, 0, w.g, rin, h);
     }

@@ -308,3 +308,39 @@ def test_few_rows_keep_small_weights(gpu, c, r):
         allow = want * (2.0 ** -11 + 2.0 ** -19 + 2.0 ** -32 / w + (0.6 * n + 80) * 2.0 ** -24)
         assert np.abs(out[row] - want).max() <= allow, (row, out[row][:2], want, allow)
     p.close()
+
+
+# ---- scores past 2^24 -------------------------------------------------------
+
+@pytest.mark.parametrize("c,r", [(20, 1), (20, 7), (20, 12), (1500, 1), (1500, 6), (1500, 12), (0, 2100), (10500, 200)])
+@pytest.mark.parametrize("again", [False, True])
+def test_scores_of_millions_pick_their_key(gpu, c, r, again):
+    """Scores of 10^8, where a step of f32 is 8 to 64: a row's largest score
+    leads by more than any rounding (128 products of f32: 2^-17 sum |q k|, 10^4
+    here), so its key's value is the result, to the bit.  `again`: and the last
+    row's value is not finite, so that the columns of its block are computed
+    again."""
+    if again and r == 1:
+        pytest.skip("a lone row sees its own value")
+    ps = 16
+    p, pool, table = one(c, r, ps)
+    pool[:, :, 0] = randn(8, *pool[:, :, 0].shape, std=1e4)
+    q = randn(6, r, QDIM, std=1e4)
+    if again:
+        page, off = at(table, ps, c + r - 1)
+        pool[0, page, 1, :, off, 5] = INF
+    out = run_attn(p, [(c, r)], i32(table), q).view(r, NQH, HD)
+    rows = [x for x in some_rows(r, random.Random(1)) if x < r - 1 or not again]
+    kv = pool[0, torch.tensor(table[0]).cuda()]
+    checked = 0
+    for h in (0, 15):
+        k, v = (kv[:, s, h // 2].reshape(-1, HD)[:c + r] for s in (0, 1))
+        s = (q.view(r, NQH, HD)[rows, h].double().cpu() @ k.double().cpu().T) * HD ** -0.5
+        s[torch.arange(c + r)[None] > torch.tensor([c + x for x in rows])[:, None]] = -INF
+        top = s.topk(2, dim=1)
+        lead = (top.values[:, 0] - top.values[:, 1]) > 2e4
+        checked += int(lead.sum())
+        want = v[top.indices[:, 0].cuda()][lead.cuda()]
+        assert torch.equal(out[rows, h][lead.cuda()], want), (h, (out[rows, h][lead.cuda()] != want).sum())
+    assert checked >= len(rows)
+    p.close()
