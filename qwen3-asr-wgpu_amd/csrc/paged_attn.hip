@@ -362,13 +362,14 @@ __device__ __forceinline__ void put_block(const PagedAttnArgs& a, const Item& it
     }
 }
 
-// NaN if some element is not finite.
+// NaN if some element is not finite and has to be computed again: not if the
+// weights' sum is NaN, which all dims of the column are then anyway.
 template <int N>
-__device__ __forceinline__ float not_finite(const float* o) {
+__device__ __forceinline__ float not_finite(const float* o, float l) {
     float t = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) t = fmaf(o[i], 0.0f, t);
-    return t;
+    return l == l ? t : 0.0f;
 }
 
 // One column's output dims again, in f32 and key by key, by one wave: for
@@ -936,7 +937,7 @@ __device__ __forceinline__ void run_narrow(const PagedAttnArgs& a, const Item& i
     float o[kElems], M = 0.0f, L = 0.0f, t = 0.0f;
     if (valid) {
         combine<kNarrowWaves, kElems>(sh, 0, 1, kElems * wave, lane, o, M, L);
-        t = not_finite<kElems>(o) + 0.0f * L;
+        t = not_finite<kElems>(o, L);
     }
     if (rarely(__ballot(t != t)))
         put_exact(a, it, it.tile0 * kNarrowTile, min(it.tile1 * kNarrowTile, it.kend), L, wave, rin, h, valid,
@@ -1010,7 +1011,7 @@ __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it,
 #pragma unroll 1
     for (int db = 2 * kg; db < 2 * kg + 2; ++db) {
         combine<2, 16>(sh, rw, 4, db * 16, lane, o, M, L);
-        const float t = not_finite<16>(o) + 0.0f * L;
+        const float t = not_finite<16>(o, L);
         if (rarely(__ballot(valid && t != t)))
             put_exact(a, it, it.tile0 * kWideTile, min(it.tile1 * kWideTile, it.kend), L, db, rin, h, valid, ~0u);
         else if (valid)
