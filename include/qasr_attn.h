@@ -202,7 +202,8 @@ int qasr_prefill_layer(qasr_ctx* ctx, qasr_kv* kv, int layer, int slot, int kv_s
  * waits for the host and a captured graph of [plan, layers] that updates the
  * lengths in place can be replayed token after token.  The reference's caches
  * are one buffer per slot (decoder.rs:1270-1271, 2453-2457): these entry points
- * have no counterpart in it; their arithmetic is that of the stages above.
+ * have no counterpart in it; their arithmetic is that of the stages above
+ * (qasr_paged_attn says which).
  *
  * A step: qasr_paged_plan_build once, then per layer qasr_paged_append (stage
  * (a)) and qasr_paged_attn (stages (b) and (c): single rows, chunks and any
@@ -314,9 +315,19 @@ int qasr_paged_append(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows,
  * keys 0..p.  table_dev: the table of the build, unchanged since.  Keys of
  * entries outside the pool (an evicted page, say -1) are left out; a row that
  * sees no key, or only scores of -inf, gives zeros.  Infinities and NaN in a key
- * or value reach the rows that see it and no others.  A request's output bits
- * depend on its rows, length and keys alone, not on its batch mates or where its
- * pages lie.  q_dev and out_dev are 16-byte aligned and do not overlap. */
+ * or value reach the rows that see it (also with a weight of 0, as 0 * inf is
+ * NaN) and no others; a value that is not finite is slow, its columns are
+ * computed again key by key.  A request's output bits depend on its rows, length
+ * and keys alone, not on its batch mates or where its pages lie.
+ *
+ * Scores, sums and states are f32.  Rows are attended in blocks of 16 or 64
+ * (qasr_plan_paged): a block of up to 8 rows, a single row among them, weighs
+ * keys to 22 bits, as stage (b) does in f32; larger ones in f16, as stage (c).
+ *
+ * A plan whose max_rows and table could hold a large chunk (rows * mean keys >=
+ * 2^21) launches a kernel for such chunks at every call, 1.4-2 us a layer: a
+ * step of single rows alone is faster on a plan of its own, of as many rows as
+ * requests.  q_dev and out_dev are 16-byte aligned and do not overlap. */
 int qasr_paged_attn(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows,
                     const int32_t* table_dev, int table_stride, const void* q_dev, void* out_dev,
                     void* stream);

@@ -284,8 +284,8 @@ hipError_t launch_norm_rope_append(const CacheGeom& g, int layer, const SegPlan&
 
 // The same kernels with a row map instead of segments: a row's page and place
 // come with its position, in the same round trip.  Bound as they are: us a
-// layer, 1 row 3.0 (a launch), 16 prompts of 150-450 rows (5185 rows, 85 MB)
-// 19.4-20, 4.3 TB/s.
+// layer, 1 row 3.1 (a launch), 16 prompts of 150-450 rows (5185 rows, 85 MB)
+// 19-20.5, 4.1-4.5 TB/s.
 hipError_t launch_paged_append(const CacheGeom& g, int layer, const RowMap& P, int rows,
                                const f16* qkv, const f16* q_gain, const f16* k_gain,
                                const f16* cos_tab, const f16* sin_tab, f16* q_out,

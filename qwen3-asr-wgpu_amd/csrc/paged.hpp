@@ -42,10 +42,10 @@ struct PagedShape {
 // rows at 0 17.2 / 24.1, 512 at 2000 26.9 / 28.4, 1024 at 1000 27.2 / 31.9, 4
 // requests of 256 at 6000 108 / 125, 2048 at 0 40.9 / 39.8, 512 at 4000 43.4 /
 // 36.7, 1024 at 4000 64 / 57, 3000 at 0 71 / 58.  A launch that finds no wide
-// items takes 4.6 us.
+// items takes 4.6 us on its own and adds 1.4-2 to a layer of a graph.
 // Ranges, up to 16 row blocks: one row at 512, 8192 keys in ranges of 256 keys
-// 8.2, 13.4, of 512 7.7, 14.4; 16 rows of 400-2400 each 28.1, 24.1.  Of more row
-// blocks, 300 rows at 5000 not split 49, in 3 ranges 33; 4 requests of 300 rows
+// 8.3, 13.4, of 512 7.9, 14.0; 16 rows of 400-2400 27.4, 24.1; 8 chunks of 7-45
+// rows 22.7, 17.1.  Of more row blocks, 300 rows at 5000 not split 49, in 3 ranges 33; 4 requests of 300 rows
 // at 1200 not split 38, in ranges of 512 53: longer ranges, of 2048 keys.
 __host__ __device__ inline PagedShape paged_shape(int len, int rows) {
     PagedShape s;

@@ -24,16 +24,18 @@
 //    tile, 135 KB of LDS.  Each key is read once for 64 rows.
 //
 // What bounds it.  Decode: bytes, and below some 100 MB the chain of one item:
-// a tile takes a wave 0.8 us (16 columns; 0.96 with 32) however early its copy
+// a tile takes a wave 0.87 us (16 columns; 0.96 with 32) however early its copy
 // was asked for (two tiles in flight a wave: no gain), launch, item and first
-// tile 3.5 us, the end 1.3 us.  us a layer of 16 q and 8 kv heads:
-//   1 row of 512 keys 7.7, of 8192 (33.6 MB) 14.4, 16 rows of 400-2400 24.1
-//   (93.8 MB, 3.9 TB/s; a large copy reaches 5.2).
+// tile 3.5 us, the end 1.3 us.  us a layer of 16 q and 8 kv heads (ranges: over
+// runs, warm and cold inputs):
+//   1 row of 512 keys 7.9-8.1, of 8192 (33.6 MB) 14.0-14.7, 16 rows of 400-2400
+//   23.6-24.3 (93.8 MB, 3.9 TB/s; a large copy reaches 5.2).
 // Chunks: MFMA and VALU work, which share the issue slots of a SIMD (two waves
 // overlap about half of the smaller part), at a clock that falls to 1.9 GHz:
-//   2 x 2048 rows at 4096 185-206 (172 GFLOP, 0.83-0.93 PFLOP/s; a large f16 product
-//   reaches 1.1-1.3), 512 at 7680 52 (0.64), 8 chunks of 7-45 rows at 200-1700
-//   17-18, 24 single rows of 100-2400 with 4 chunks of 100-450 rows 45.
+//   2 x 2048 rows at 4096 182-200 (172 GFLOP, 0.86-0.95 PFLOP/s; a large f16 product
+//   reaches 1.1-1.3), 512 at 7680 52-55 (0.60-0.64), 8 chunks of 7-45 rows at
+//   200-1700 17-20.7, 24 single rows of 100-2400 with 4 chunks of 100-450 rows
+//   44.5-45.2.
 // Also measured: 64-row items of 4 waves 223 us for the first of these, the
 // key groups half a tile apart 223; narrow items of 8 waves 5.7 against 4.8 us
 // for a single row's loop; 64-row blocks for every chunk 85 us for the last

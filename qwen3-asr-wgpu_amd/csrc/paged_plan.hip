@@ -17,8 +17,12 @@
 // by a binary search of the prefix sums in LDS.  What may alias an input
 // (lengths and the cursor, updated in place by a replayed graph) is written
 // by the workgroup that arrives last, when every other has read it.
-// us a launch: 16 single rows 7.3, 256 requests of 220 single rows and 20 chunks
-// 15.8; with three scans and items by the row blocks' workgroups 43.
+// us a launch: 16 single rows 7.3, 256 requests of 220 single rows and 20 chunks,
+// 16 of them ended, 15.8-17; with three scans and items by the row blocks'
+// workgroups 43.  A given table is checked by each request's own thread, entry
+// by entry: 2048 new rows of one request on pages of 256 rows 6.1, of 16 14.2.
+// Pages go back in the last workgroup alone, a workgroup's threads of them at a
+// time.
 
 #include "paged.hpp"
 

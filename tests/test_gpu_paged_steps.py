@@ -245,3 +245,33 @@ def test_positions_up_to_the_last_of_a_short_context(gpu, max_seq, batch):
     assert p.plan.status.tolist() == [0] * len(batch)
     check_attn(p, batch, i32(table), q, out, heads=(0, 13))
     p.close()
+
+
+def test_two_plans_take_turns_over_one_pool(gpu):
+    """Single rows on a plan of their own, chunks on a larger one: each build
+    goes on from the lens and the cursor of the other plan."""
+    ps, pages, n = 16, 60, 4
+    p = Paged(pages, ps, n, n)
+    large = Q.PagedPlan(p.ctx, p.pool, n, 100)
+    ring, cursor = p.pool.free_ring()
+    table = torch.full((n, 14), -1, dtype=torch.int32, device="cuda")
+    g = randn(3, 2, HD) + 1
+    lens, at, cur = [0] * n, i32([0] * n), cursor
+    for t, rows in enumerate([[20, 30, 15, 1], [1] * n, [1, 0, 1, 1], [40, 1, 1, 20], [1] * n, [0, 33, 0, 1], [1] * n]):
+        plan = p.plan if max(rows) <= 1 else large
+        total = sum(rows)
+        qkv = randn(50 + t, total, TOT)
+        q, out = (torch.empty((total, QDIM), dtype=torch.float16, device="cuda") for _ in range(2))
+        Q.paged_plan(p.ctx, plan, at, i32(rows), table, ring, cur)
+        Q.paged_append(p.ctx, plan, 0, qkv, g[0], g[1], q)
+        Q.paged_attn(p.ctx, plan, 0, table, q, out)
+        at, cur = plan.lens, plan.cursor
+        assert plan.status.tolist() == [0] * n
+        check_attn(p, list(zip(lens, rows)), table, q, out, heads=(0, 7))
+        lens = [a + b for a, b in zip(lens, rows)]
+        assert at.tolist() == lens
+    held = [x for i in range(n) for x in table[i, :-(-lens[i] // ps)].tolist()]
+    head, free = cur.tolist()
+    assert sorted(held + [ring[(head + k) % pages].item() for k in range(free)]) == list(range(pages))
+    large.close()
+    p.close()
