@@ -521,6 +521,8 @@ class PagePool:
                 torch.tensor([0, self.pages], dtype=torch.int32, device=dev))
 
     def close(self):
+        """Free the pages now; their views must not be used any more, calls of
+        the pool's plans are refused."""
         if self.handle:
             load().qasr_pages_destroy(self.handle)
             self.handle = None
