@@ -242,6 +242,36 @@ int qasr_pages_create(qasr_ctx* ctx, int pages, int page_rows, qasr_pages** out)
 void qasr_pages_destroy(qasr_pages* pool);
 int qasr_pages_get_info(const qasr_pages* pool, qasr_pages_info* out);
 
+/* A pool in 8 bits: element (layer, page, kv, head, row, d) is the e4m3 byte at
+ * the same place times the power of two that its block, 16 rows of a head of a
+ * page, has: 2^(scale byte - 127) (e8m0), byte layer*layer_stride +
+ * page*page_stride + kv*kv_stride + head*head_stride + row/block_rows at
+ * base_dev.  Zeroed, the scales 2^0.  Half the memory of an f16 pool and an
+ * eighth of a per cent.  All paged calls take such a pool:
+ *  - qasr_paged_append rounds K and V, once they are f16 as in an f16 pool, to
+ *    the nearest e4m3 number (ties to even) in units of the smallest power of two
+ *    from 2^-15 on of which the block's largest finite value is at most 448; with a
+ *    unit of 2^8 magnitudes end at 240.  Rows that a block holds already keep
+ *    their values if they fit; where a new row needs a larger unit they are
+ *    rounded to it (exact but for values below 2^-6 of the unit).  Infinities and
+ *    NaN become NaN.
+ *  - qasr_paged_attn gives the bits that it gives over an f16 pool of the values
+ *    that the bytes stand for.  Each of these is an f16 number, as scales lie in
+ *    2^-15 .. 2^8; with others, stored by the caller, a value is rounded to f16.
+ * qasr_pages_get_info counts elements; its bytes are those of the elements. */
+typedef struct qasr_pages_scales {
+    uint8_t* base_dev;
+    int32_t block_rows; /* 16 */
+    int32_t head_stride;
+    int32_t kv_stride;
+    int32_t page_stride;
+    int64_t layer_stride;
+    size_t bytes;
+} qasr_pages_scales;
+int qasr_pages_create_e4m3(qasr_ctx* ctx, int pages, int page_rows, qasr_pages** out);
+/* QASR_EINVAL for an f16 pool. */
+int qasr_pages_get_scales(const qasr_pages* pool, qasr_pages_scales* out);
+
 /* A step's plan: device arrays of its own, written by each build. */
 typedef struct qasr_paged_plan_info {
     int32_t max_requests;

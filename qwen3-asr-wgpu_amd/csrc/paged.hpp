@@ -7,6 +7,9 @@
 // contiguous block.  A request's position p lives in row p % rows of page
 // table[p / rows].  Behind the last layer lies one page of zeros, which stands
 // for table entries outside the pool.
+// e4m3 pools hold bytes in the same places, and a byte for each 16 rows of a
+// (layer, page, kv, head), the exponent of an f32 power of two: [layer][page]
+// [2][nkvh][rows / 16], the zero page's behind the last layer's.
 #pragma once
 
 #include "kernels.hpp"
@@ -16,6 +19,7 @@ namespace qasr {
 constexpr int kPagedMaxRequests = 1024;  // one thread of the plan kernel each
 constexpr int kPagedMinShift = 4;        // pages of 16 rows: one copy instruction stays in a page
 constexpr int kPagedMaxShift = 8;
+constexpr int kPagedScaleRows = 16;  // e4m3: rows of a scale
 
 // Attention work items.  A request's new rows are cut into row blocks of
 // kNarrowRows rows (whose waves share the keys) or kWideRows rows (whose waves
@@ -138,6 +142,21 @@ hipError_t launch_paged_append(const CacheGeom& g, int layer, const RowMap& P, i
                                const f16* cos_tab, const f16* sin_tab, f16* q_out,
                                hipStream_t stream);
 
+// And into e4m3 pages (paged_append8.hip): the layer's pages and scale bytes.
+struct PagedAppend8Args {
+    const f16 *qkv, *q_gain, *k_gain, *cos_tab, *sin_tab;
+    f16* q_out;
+    const int32_t* pos;
+    const int32_t* slot;
+    int32_t rows, slots, page_shift, rope_rows, nqh, nkvh;
+    float eps;
+    uint8_t* base;
+    int64_t page_stride, kv_stride, head_stride;
+    uint8_t* scales;  // exponents of f32 powers of two, one for 16 rows of a head
+    int32_t page_scales, kv_scales, head_scales;
+};
+hipError_t launch_paged_append8(const PagedAppend8Args& a, hipStream_t stream);
+
 // Attention.  Split state, `records` rows of it (a row of a range): nqh * 128
 // unnormalised f32 outputs and nqh (max, sum) pairs each, laid out per (row
 // block, kv head, range) (paged_attn.hip); one arrival counter per (row block,
@@ -147,7 +166,7 @@ constexpr int kPagedDrawWords = 17 * kPagedCounterStep;  // 16 kv heads and one,
 struct PagedAttnArgs {
     const f16* q;    // [rows][nqh*128], roped
     f16* out;        // [rows][nqh*128]
-    const f16* base; // the layer's pages
+    const void* base; // the layer's pages
     int64_t page_stride, kv_stride, head_stride;
     const int32_t* table;
     int32_t stride, pages, page_shift, nkvh, rows;
@@ -160,6 +179,8 @@ struct PagedAttnArgs {
     float* ws_ml;
     uint32_t* counters;
     uint32_t* drawn;  // [2][kPagedDrawWords], zero at rest: items drawn per kv head, workgroups gone
+    const uint8_t* scales;  // e4m3: the layer's scale bytes; NULL: f16
+    int32_t page_scales, kv_scales, head_scales;  // their strides
 };
 hipError_t launch_paged_attn(const PagedAttnArgs& a, int cus, hipStream_t stream);
 

@@ -21,8 +21,11 @@ struct qasr_pages {
     int device;
     int32_t pages;
     int32_t shift;  // log2 of a page's rows
-    f16* base = nullptr;  // the layers' pages, then the zero page
-    size_t bytes = 0;     // without the zero page
+    int32_t elem;         // bytes of an element: 2 (f16) or 1 (e4m3)
+    char* base = nullptr;  // the layers' pages, then the zero page; e4m3: then the scales
+    size_t bytes = 0;      // without the zero page and the scales
+    uint8_t* scales = nullptr;
+    size_t scale_bytes = 0;  // without the zero page's
 };
 
 struct qasr_paged_plan {
@@ -48,7 +51,7 @@ namespace {
 qasr::CacheGeom page_geom(const qasr_pages* p) {
     const qasr_attn_cfg& c = p->ctx->cfg;
     qasr::CacheGeom g;
-    g.base = p->base;
+    g.base = (f16*)p->base;
     g.head_stride = (int64_t)qasr::kHeadDim << p->shift;
     g.kv_stride = g.head_stride * c.num_key_value_heads;
     g.slot_stride = 2 * g.kv_stride;  // page
@@ -56,6 +59,18 @@ qasr::CacheGeom page_geom(const qasr_pages* p) {
     g.nkvh = c.num_key_value_heads;
     g.cap = 1 << p->shift;
     return g;
+}
+
+// Scale bytes of a page's head, of its K, of a page.
+struct ScaleGeom {
+    int32_t head, kv, page;
+};
+ScaleGeom scale_geom(const qasr_pages* p) {
+    ScaleGeom s;
+    s.head = (1 << p->shift) / qasr::kPagedScaleRows;
+    s.kv = s.head * p->ctx->cfg.num_key_value_heads;
+    s.page = 2 * s.kv;
+    return s;
 }
 
 int check_plan(qasr_ctx* ctx, qasr_paged_plan* plan) {
@@ -116,7 +131,7 @@ int check_build_arrays(const qasr_paged_plan* p, int nreq, const int32_t* len, c
 
 extern "C" {
 
-int qasr_pages_create(qasr_ctx* ctx, int pages, int page_rows, qasr_pages** out) {
+static int create_pages(qasr_ctx* ctx, int pages, int page_rows, int elem, qasr_pages** out) {
     if (!ctx || !out) return fail(QASR_EINVAL, "null argument");
     *out = nullptr;
     int shift = qasr::kPagedMinShift;
@@ -135,12 +150,17 @@ int qasr_pages_create(qasr_ctx* ctx, int pages, int page_rows, qasr_pages** out)
     p->device = ctx->device;
     p->pages = pages;
     p->shift = shift;
-    p->bytes = (size_t)page_geom(p).layer_stride * ctx->cfg.num_hidden_layers * sizeof(f16);
-    const size_t all = p->bytes + (size_t)page_geom(p).slot_stride * sizeof(f16);
+    p->elem = elem;
+    p->bytes = (size_t)page_geom(p).layer_stride * ctx->cfg.num_hidden_layers * elem;
+    const size_t data = p->bytes + (size_t)page_geom(p).slot_stride * elem;
+    const size_t zero_scales = elem == 1 ? scale_geom(p).page : 0;
+    p->scale_bytes = zero_scales * pages * ctx->cfg.num_hidden_layers;
+    const size_t all = data + p->scale_bytes + zero_scales;
     DeviceScope ds(ctx->device);
     hipError_t e = ds.err;
     if (e == hipSuccess) e = hipMalloc(&p->base, all);
-    if (e == hipSuccess) e = hipMemset(p->base, 0, all);
+    if (e == hipSuccess) e = hipMemset(p->base, 0, data);
+    if (e == hipSuccess && all > data) e = hipMemset(p->base + data, 127, all - data);  // 2^0
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) {
         if (p->base) (void)hipFree(p->base);
@@ -148,7 +168,30 @@ int qasr_pages_create(qasr_ctx* ctx, int pages, int page_rows, qasr_pages** out)
         (void)hipGetLastError();  // the next launch must not report it
         return hip_fail(e, "page pool allocation");
     }
+    if (elem == 1) p->scales = (uint8_t*)p->base + data;
     *out = p;
+    return QASR_OK;
+}
+
+int qasr_pages_create(qasr_ctx* ctx, int pages, int page_rows, qasr_pages** out) {
+    return create_pages(ctx, pages, page_rows, sizeof(f16), out);
+}
+
+int qasr_pages_create_e4m3(qasr_ctx* ctx, int pages, int page_rows, qasr_pages** out) {
+    return create_pages(ctx, pages, page_rows, 1, out);
+}
+
+int qasr_pages_get_scales(const qasr_pages* p, qasr_pages_scales* out) {
+    if (!p || !out) return fail(QASR_EINVAL, "null argument");
+    if (!p->scales) return fail(QASR_EINVAL, "the pool's pages are f16: they have no scales");
+    const ScaleGeom s = scale_geom(p);
+    out->base_dev = p->scales;
+    out->block_rows = qasr::kPagedScaleRows;
+    out->head_stride = s.head;
+    out->kv_stride = s.kv;
+    out->page_stride = s.page;
+    out->layer_stride = (int64_t)s.page * p->pages;
+    out->bytes = p->scale_bytes;
     return QASR_OK;
 }
 
@@ -324,6 +367,37 @@ int qasr_paged_append(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows,
     if (!ctx->cos) return fail(QASR_ESTATE, "RoPE tables not set (qasr_set_rope_tables)");
     DeviceScope ds(ctx->device);
     if (ds.err != hipSuccess) return hip_fail(ds.err, "hipSetDevice");
+    if (plan->pool->scales) {
+        const qasr::CacheGeom g = page_geom(plan->pool);
+        const ScaleGeom s = scale_geom(plan->pool);
+        qasr::PagedAppend8Args a;
+        a.qkv = (const f16*)qkv_dev;
+        a.q_gain = (const f16*)q_gain_dev;
+        a.k_gain = (const f16*)k_gain_dev;
+        a.cos_tab = ctx->cos;
+        a.sin_tab = ctx->sin;
+        a.q_out = (f16*)q_out_dev;
+        a.pos = plan->row_pos;
+        a.slot = plan->row_slot;
+        a.rows = rows;
+        a.slots = plan->pool->pages << plan->pool->shift;
+        a.page_shift = plan->pool->shift;
+        a.rope_rows = ctx->rope_rows;
+        a.nqh = nqh;
+        a.nkvh = g.nkvh;
+        a.eps = ctx->cfg.rms_norm_eps;
+        a.base = (uint8_t*)plan->pool->base + layer * g.layer_stride;
+        a.page_stride = g.slot_stride;
+        a.kv_stride = g.kv_stride;
+        a.head_stride = g.head_stride;
+        a.scales = plan->pool->scales + layer * (int64_t)s.page * plan->pool->pages;
+        a.page_scales = s.page;
+        a.kv_scales = s.kv;
+        a.head_scales = s.head;
+        const hipError_t e = qasr::launch_paged_append8(a, (hipStream_t)stream);
+        if (e != hipSuccess) return hip_fail(e, "paged append launch");
+        return QASR_OK;
+    }
     qasr::RowMap P;
     P.pos = plan->row_pos;
     P.slot = plan->row_slot;
@@ -356,10 +430,15 @@ int qasr_paged_attn(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows, c
     qasr::PagedAttnArgs a;
     a.q = (const f16*)q_dev;
     a.out = (f16*)out_dev;
-    a.base = g.base + layer * g.layer_stride;
+    const ScaleGeom s = scale_geom(plan->pool);
+    a.base = plan->pool->base + layer * g.layer_stride * plan->pool->elem;
     a.page_stride = g.slot_stride;
     a.kv_stride = g.kv_stride;
     a.head_stride = g.head_stride;
+    a.scales = plan->pool->scales ? plan->pool->scales + layer * (int64_t)s.page * plan->pool->pages : nullptr;
+    a.page_scales = s.page;
+    a.kv_scales = s.kv;
+    a.head_scales = s.head;
     a.table = table_dev;
     a.stride = table_stride;
     a.pages = plan->pool->pages;

@@ -53,6 +53,7 @@
 // who that is.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "mfma_attn.hpp"
 #include "paged.hpp"
@@ -97,34 +98,99 @@ struct Item {
     int row0, rows, planned, pos0, kend, tile0, tile1, splits, split, rec, block, kvh;
     int page0, last_page;  // first page of the range, last of the row block's keys (table places)
     const int32_t* table;  // the request's pages
-    const f16* base;       // the kv head's K in page 0
+    const char* base;      // the kv head's K in page 0
 };
 
-// Copies of one 16-key group, 1 KB an instruction (lane l's 16 bytes to m0 +
-// 16 l): K instruction j reads rows 4 j .. +4 with their 16-byte chunks
-// permuted (swz16: lane l's chunk is (l % 16) ^ (4 (l / 16) | j)), V
-// instruction j dims 32 j .. +32 of the 16 rows, `slab` bytes on in the LDS.
+// ---- the page formats -----------------------------------------------------
+
+// f16 rows of 256 bytes, or e4m3 rows of 128 with a power of two for each 16 of
+// them, which v_cvt_scalef32_pk_f16_fp8 multiplies by as it converts two values
+// at once.  What a stored pair of value and scale stands for is an f16 number
+// (kMinScale, kMaxScale), and a product takes the same numbers in the same
+// places as from f16 pages: the outputs have the same bits as over f16 pages
+// that hold these numbers.
+struct F16Pages {
+    static constexpr int kElem = 2;
+    static constexpr int kRow = kHeadDim * kElem;  // bytes
+    static constexpr int kCopies = 4;              // 1 KB each, of a 16-row group's K or V
+    static constexpr int kOrders = 1;              // of a group's V in the LDS
+};
+struct E4m3Pages {
+    static constexpr int kElem = 1;
+    static constexpr int kRow = kHeadDim * kElem;
+    static constexpr int kCopies = 2;
+    static constexpr int kOrders = 2;
+};
+template <class P>
+constexpr bool kScaled = P::kElem == 1;
+
+// Scales of the 16-key groups of a slice or key group, f32 powers of two.
+template <int N>
+struct Units {
+    float k[N], v[N];
+};
+// 8 e4m3 values as f16: the first four by `lo`, the others by `hi`.
+__device__ __forceinline__ half8v widen(uint2 x, float lo, float hi) {
+    union {
+        half8v h;
+        half2v h2[4];
+    } y;
+    y.h2[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x.x, lo, false);
+    y.h2[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x.x, lo, true);
+    y.h2[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x.y, hi, false);
+    y.h2[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x.y, hi, true);
+    return y.h;
+}
+// 8 keys of a dim: ds_read_b64_tr_b8 transposes bytes within each 16-lane group
+// (result lane 8 m + e, byte k <- source lane 2 k + m, byte e).
+typedef int int2v __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint2 read_tr8(const char* p) {
+    return __builtin_bit_cast(
+        uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) int2v*)p));
+}
+
+// Copies of one 16-key group, 1 KB an instruction.  f16: K instruction j reads
+// rows 4 j .. +4 with their 16-byte chunks permuted (swz16: lane l's chunk is
+// (l % 16) ^ (4 (l / 16) | j)), V instruction j dims 32 j .. +32 of the 16 rows,
+// `step` bytes on in the LDS.  e4m3: K instruction j rows 8 j .. +8, the chunks
+// of row r permuted by r / 2 % 8, so that 16 rows' reads of one chunk, 128 bytes
+// apart, meet every bank once; V instruction j dims 64 j .. +64, chunk by chunk
+// (16 dims), the 16 rows of a chunk 16 bytes apart, those of odd chunks 4 places
+// on and of odd groups 8 (`order`): a transposing read takes 4 rows of two chunks
+// or of two groups at once, on different banks so.
 // The group's address is scalar, a lane's offsets are registers of the kernel,
 // so a copy is an instruction and its LDS address (which m0 needs a cycle to
 // take).  Waited for by count.
+template <class P>
 struct Offsets {
-    uint32_t k[4], v[4];
+    uint32_t k[P::kCopies], v[P::kOrders][P::kCopies];
 };
-__device__ __forceinline__ void copy4(const f16* base, const uint32_t (&voff)[4], uint32_t lds, uint32_t step) {
+template <int N>
+__device__ __forceinline__ void copies(const char* base, const uint32_t (&voff)[N], uint32_t lds, uint32_t step) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < N; ++j)
         asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff[j]), "s"(base), "{m0}"(lds + j * step)
                      : "memory");
 }
 // Row r of the group reads row min(r + add, last): 0 and 15, but in the group
-// of the last key or past it.  `v_from_k`: bytes from a page's K to its V.
-__device__ __forceinline__ Offsets group_offsets(int lane, int add, int last, uint32_t v_from_k) {
-    Offsets o;
+// of the last key or past it.
+template <class P>
+__device__ __forceinline__ Offsets<P> group_offsets(const PagedAttnArgs& a, int lane, int add, int last) {
+    const uint32_t v_from_k = (uint32_t)a.kv_stride * P::kElem;  // bytes from a page's K to its V
+    Offsets<P> o;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int r = lane >> 4;
-        o.k[j] = min(4 * j + r + add, last) * 256 + (((lane & 15) ^ (r << 2) ^ j) * 16);
-        o.v[j] = v_from_k + min((lane >> 2) + add, last) * 256 + j * 64 + (lane & 3) * 16;
+    for (int j = 0; j < P::kCopies; ++j) {
+        if constexpr (kScaled<P>) {
+            const int r = 8 * j + (lane >> 3), c = lane >> 4;
+            o.k[j] = min(r + add, last) * P::kRow + (((lane & 7) ^ (r >> 1)) * 16);
+#pragma unroll
+            for (int order = 0; order < 2; ++order)
+                o.v[order][j] = v_from_k + min(((lane & 15) ^ 4 * (c & 1) ^ 8 * order) + add, last) * P::kRow + (4 * j + c) * 16;
+        } else {
+            const int r = lane >> 4;
+            o.k[j] = min(4 * j + r + add, last) * P::kRow + (((lane & 15) ^ (r << 2) ^ j) * 16);
+            o.v[0][j] = v_from_k + min((lane >> 2) + add, last) * P::kRow + j * 64 + (lane & 3) * 16;
+        }
     }
     return o;
 }
@@ -163,11 +229,36 @@ __device__ __forceinline__ void advance_pages(const PagedAttnArgs& a, const Item
     }
 }
 // Address of K of the 16-key group of `key` (past the end: of the last key).
-__device__ __forceinline__ const f16* group_base(const PagedAttnArgs& a, const Item& it, const Pages& p, int key) {
+template <class P>
+__device__ __forceinline__ const char* group_base(const PagedAttnArgs& a, const Item& it, const Pages& p, int key) {
     const int k = min(key, it.kend - 1), r = (k >> a.page_shift) - it.page0 - p.lo;
     const int id = __builtin_amdgcn_readlane(r < 64 ? p.cur.id : p.nxt.id, r & 63);
     const uint64_t page = (uint64_t)(uint32_t)id * (uint32_t)a.page_stride;  // a page is < 2^21 elements
-    return it.base + page + ((k & ((1 << a.page_shift) - 1)) & ~15) * kHeadDim;
+    return it.base + page * P::kElem + ((k & ((1 << a.page_shift) - 1)) & ~15) * P::kRow;
+}
+// Scales of the 64 16-key groups from that of `key` on, a lane each, K's byte
+// (an f32's exponent) and V's above it; past the end: of the last key's group.
+// A range has mostly no more groups than that.
+__device__ __forceinline__ uint32_t load_scales(const PagedAttnArgs& a, const Item& it, const Pages& p, int key) {
+    const int k = min(key + 16 * (thread_id() & 63), it.kend - 1), r = (k >> a.page_shift) - it.page0 - p.lo;
+    const int cur = __shfl(p.cur.id, r & 63), nxt = __shfl(p.nxt.id, r & 63);
+    const uint8_t* s = a.scales + (uint64_t)(uint32_t)(r < 64 ? cur : nxt) * (uint32_t)a.page_scales +
+                       it.kvh * a.head_scales + ((k & ((1 << a.page_shift) - 1)) >> 4);
+    return s[0] | (uint32_t)s[a.kv_scales] << 8;
+}
+constexpr int kScaleTiles = 64 / (kNarrowTile / 16);  // tiles that 64 groups last for
+static_assert(kNarrowTile == kWideTile, "");
+// Those of groups j .. j + N of a load.
+template <int N>
+__device__ __forceinline__ Units<N> units(uint32_t scales, int j) {
+    Units<N> u;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t s = __builtin_amdgcn_readlane(scales, j + i);
+        u.k[i] = __uint_as_float((s & 0xff) << 23);
+        u.v[i] = __uint_as_float((s >> 8) << 23);
+    }
+    return u;
 }
 // Bit j: the page of keys key + 16 j .. +16 lies outside the pool.
 template <int N>
@@ -182,16 +273,16 @@ __device__ __forceinline__ uint32_t hidden_groups(const PagedAttnArgs& a, const 
     }
     return bits;
 }
-// K and V of the 16-key group of `key` into kd (1 KB a step) and vd (`slab` a
-// step).
-__device__ __forceinline__ void copy_group(const PagedAttnArgs& a, const Item& it, const f16* base, const Offsets& whole,
-                                           int key, bool v, uint32_t lds, uint32_t step) {
+// K or V of the 16-key group of `key` to `lds`, `step` bytes an instruction.
+template <class P>
+__device__ __forceinline__ void copy_group(const PagedAttnArgs& a, const Item& it, const char* base, const Offsets<P>& whole,
+                                           int key, bool v, int order, uint32_t lds, uint32_t step) {
     if (key + 16 <= it.kend) {
-        copy4(base, v ? whole.v : whole.k, lds, step);
+        copies(base, v ? whole.v[order] : whole.k, lds, step);
     } else {
         const int gkey = min(key, (it.kend - 1) & ~15);
-        const Offsets o = group_offsets(thread_id() & 63, key - gkey, it.kend - 1 - gkey, (uint32_t)a.kv_stride * 2);
-        copy4(base, v ? o.v : o.k, lds, step);
+        const Offsets<P> o = group_offsets<P>(a, thread_id() & 63, key - gkey, it.kend - 1 - gkey);
+        copies(base, v ? o.v[order] : o.k, lds, step);
     }
 }
 
@@ -381,22 +472,33 @@ __device__ __forceinline__ float not_finite(const float* o, float l) {
 // r, q head h; `sum`: the sum of the weights, which are taken against these
 // scores' own maximum (-inf: they are 0), as the sums of the MFMA round
 // otherwise.
+template <class P>
 __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& it, int key0, int key1, int r, int h,
                                             int db, int lane, float& sum) {
     const int pos = it.pos0 + r, end = min(key1, pos + 1);
     const f16* q = a.q + ((int64_t)(it.row0 + r) * a.nkvh + it.kvh) * (kRep * kHeadDim) + h * kHeadDim;
-    // This lane's key of the 64 from k0 on: its row, whether it is seen, and its
-    // score.
+    // This lane's key of the 64 from k0 on: its row (and the unit of its V),
+    // whether it is seen, and its score.
+    float unit = 1.0f;
     auto score = [&](int k0, uint64_t& row, bool& seen) {
         const int key = k0 + lane;
         const int id = it.table[min(key, it.kend - 1) >> a.page_shift];
         seen = key < end && (uint32_t)id < (uint32_t)a.pages;
         row = (uint64_t)(uint32_t)(seen ? id : 0) * (uint32_t)a.page_stride +
               (key & ((1 << a.page_shift) - 1)) * kHeadDim;
-        float s = 0.0f;
+        float s = 0.0f, k_unit = 1.0f;
+        if constexpr (kScaled<P>) {
+            const uint8_t* u = a.scales + (uint64_t)(uint32_t)(seen ? id : 0) * (uint32_t)a.page_scales +
+                               it.kvh * a.head_scales + ((key & ((1 << a.page_shift) - 1)) >> 4);
+            k_unit = __uint_as_float((uint32_t)u[0] << 23);
+            unit = __uint_as_float((uint32_t)u[a.kv_scales] << 23);
+        }
         for (int d = 0; d < kHeadDim; d += 8) {
             H8 x, y;
-            x.u = *(const uint4*)(it.base + row + d);
+            if constexpr (kScaled<P>)
+                x.h = widen(*(const uint2*)(it.base + row + d), k_unit, k_unit);
+            else
+                x.u = *(const uint4*)(it.base + (row + d) * P::kElem);
             y.u = *(const uint4*)(q + d);
 #pragma unroll
             for (int e = 0; e < 8; ++e) s = fmaf(h2f(x.e[e]), h2f(y.e[e]), s);
@@ -422,7 +524,13 @@ __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& 
             todo &= todo - 1;
             const uint64_t at = (uint64_t)__shfl((int)(uint32_t)(row >> 32), j) << 32 |
                                 (uint32_t)__shfl((int)(uint32_t)row, j);
-            o = fmaf(__shfl(p, j), h2f(it.base[at + a.kv_stride + 32 * db + (lane & 31)]), o);
+            const char* v = it.base + (at + a.kv_stride + 32 * db + (lane & 31)) * P::kElem;
+            if constexpr (kScaled<P>) {
+                const float u = __shfl(unit, j);
+                o = fmaf(__shfl(p, j), h2f(widen(make_uint2(*(const uint8_t*)v, 0), u, u)[0]), o);
+            } else {
+                o = fmaf(__shfl(p, j), h2f(*(const f16*)v), o);
+            }
         }
     }
 #pragma unroll
@@ -435,6 +543,7 @@ __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& 
 // is of weights against another maximum, rounded to f16 (weights()): the dims
 // are divided by their own sum, and a range's state holds them times the
 // state's sum over theirs.
+template <class P>
 __device__ __forceinline__ void put_exact(const PagedAttnArgs& a, const Item& it, int key0, int key1, float L, int db,
                                           int r, int h, bool valid, uint32_t cols) {
     const int lane = thread_id() & 63;
@@ -445,7 +554,7 @@ __device__ __forceinline__ void put_exact(const PagedAttnArgs& a, const Item& it
         const int rj = __shfl(r, j), hj = __shfl(h, j);
         const float l = __shfl(L, j);
         float sum;
-        float o = exact_dims(a, it, key0, key1, rj, hj, db, lane, sum);
+        float o = exact_dims<P>(a, it, key0, key1, rj, hj, db, lane, sum);
         if (lane >= 32) continue;
         if (it.splits == 1) {
             o = l == 0.0f ? 0.0f : o / sum;
@@ -474,9 +583,29 @@ __device__ __forceinline__ void draw(Draw& d) {
 
 // ---- the two kinds of item ------------------------------------------------
 
+// A wave's state, and for V in e4m3 its operand source addresses: of even and odd
+// groups.
+template <class P>
+struct PageWave : Wave {
+    int vb[2];
+};
+// Operand addresses of a lane in e4m3 tiles (bytes): K operand of k-step ks: row
+// n, dims 16 ks + 8 g .. +8; V^T operand: source lane 16 q4 + 2 k + m reads the
+// bytes 8 m .. +8 of chunk 2 db + q4 % 2 in row 4 (q4 / 2) + k % 4 + 8 (k / 4),
+// the keys that the f16 operand has in the same places.
+__device__ __forceinline__ void operand_addrs8(PageWave<E4m3Pages>& w, int lane) {
+    const int n = lane & 31, g = lane >> 5;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) w.kaddr[ks] = n * E4m3Pages::kRow + ((ks ^ ((n >> 1) & 7)) * 16) + 8 * g;
+    const int c = (lane >> 4) & 1, k = (lane >> 1) & 7, row = 4 * g + (k & 3) + 8 * (k >> 2);
+#pragma unroll
+    for (int order = 0; order < 2; ++order) w.vb[order] = c * 256 + (row ^ 4 * c ^ 8 * order) * 16 + 8 * (lane & 1);
+}
+
 // This lane's query column (row rin of the block, q head h): its Q^T operand
 // straight from memory, its position and the empty softmax state.
-__device__ __forceinline__ void init_wave(Wave& w, const PagedAttnArgs& a, const Item& it, int rin, int h, int lane) {
+template <class P>
+__device__ __forceinline__ void init_wave(PageWave<P>& w, const PagedAttnArgs& a, const Item& it, int rin, int h, int lane) {
     const int r = min(rin, it.rows - 1);  // columns past the block repeat its last row
     const f16* q = a.q + ((int64_t)(it.row0 + r) * a.nkvh + it.kvh) * (kRep * kHeadDim) + h * kHeadDim + 8 * (lane >> 5);
 #pragma unroll
@@ -488,7 +617,10 @@ __device__ __forceinline__ void init_wave(Wave& w, const PagedAttnArgs& a, const
     for (int db = 0; db < 4; ++db) w.o[db] = (float16v){};
     w.m = kNegInf;
     w.l = 0.0f;
-    operand_addrs(w, lane);
+    if constexpr (kScaled<P>)
+        operand_addrs8(w, lane);
+    else
+        operand_addrs(w, lane);
 }
 // Every load and copy so far has landed, Q among them.  The registers are
 // named here, once: else the compiler, which does not count the copies, waits
@@ -597,6 +729,14 @@ __device__ __forceinline__ void weights(Wave& w, const float16v (&s)[NB], const 
 }
 
 #define WAIT_VM(n) asm volatile("s_waitcnt vmcnt(" #n ")" ::: "memory")
+template <int N>
+__device__ __forceinline__ void wait_copies() {  // all but the last N
+    static_assert(N == 8 || N == 4, "");
+    if constexpr (N == 8)
+        WAIT_VM(8);
+    else
+        WAIT_VM(4);
+}
 
 // The matrix products of a step.  Operand reads run kAhead products ahead of
 // their MFMA: reads and MFMAs stay in this order (vector and scalar work may
@@ -604,14 +744,23 @@ __device__ __forceinline__ void weights(Wave& w, const float16v (&s)[NB], const 
 constexpr int kAhead = 3;
 __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x406); }  // VALU, SALU, exp may cross
 
-// S^T of K rows kt[0 .. 32 NB - 1], keys kb*32 + (8*(i/4) + 4*g + i%4) x query
+// S^T of K rows 0 .. 32 NB - 1 at kt, keys kb*32 + (8*(i/4) + 4*g + i%4) x query
 // n.
-template <int NB>
-__device__ __forceinline__ void scores(const Wave& w, const f16* kt, float16v (&s)[NB]) {
+template <class P, int NB>
+__device__ __forceinline__ void scores(const PageWave<P>& w, const char* kt, const Units<2 * NB>& u, float16v (&s)[NB]) {
+    using Raw = std::conditional_t<kScaled<P>, uint2, half8v>;
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) s[kb] = (float16v){};
-    half8v ka[8 * NB];
-    auto read = [&](int x) { ka[x] = *(const half8v*)&kt[(x % NB) * 32 * kHeadDim + w.kaddr[x / NB]]; };
+    Raw ka[8 * NB];
+    auto read = [&](int x) {
+        ka[x] = *(const Raw*)(kt + (x % NB) * 32 * P::kRow + w.kaddr[x / NB] * (kScaled<P> ? 1 : 2));
+    };
+    float unit[NB];  // of this lane's row
+    if constexpr (kScaled<P>) {
+        const bool second = thread_id() & 16;
+#pragma unroll
+        for (int kb = 0; kb < NB; ++kb) unit[kb] = second ? u.k[2 * kb + 1] : u.k[2 * kb];
+    }
 #pragma unroll
     for (int x = 0; x < kAhead; ++x) read(x);
     keep_order();
@@ -619,19 +768,29 @@ __device__ __forceinline__ void scores(const Wave& w, const f16* kt, float16v (&
     for (int x = 0; x < 8 * NB; ++x) {
         if (x + kAhead < 8 * NB) read(x + kAhead);
         keep_order();
-        s[x % NB] = mfma32(ka[x], w.qb[x / NB], s[x % NB]);
+        half8v k;
+        if constexpr (kScaled<P>)
+            k = widen(ka[x], unit[x % NB], unit[x % NB]);
+        else
+            k = ka[x];
+        s[x % NB] = mfma32(k, w.qb[x / NB], s[x % NB]);
         keep_order();
     }
 }
 
-// O^T += V^T P^T with V rows vt[0 .. 32 NB - 1] of a tile of ROWS rows.
-template <int ROWS, int NB>
-__device__ __forceinline__ void product(Wave& w, const f16* vt, const half8v (&pb)[2 * NB]) {
+// O^T += V^T P^T with V rows 0 .. 32 NB - 1 at vt, f16 rows of a tile of ROWS.
+template <class P, int ROWS, int NB>
+__device__ __forceinline__ void product(PageWave<P>& w, const char* vt, const Units<2 * NB>& u, const half8v (&pb)[2 * NB]) {
     half4v lo[8 * NB], hi[8 * NB];
+    uint2 both[8 * NB];
     auto read = [&](int x) {
-        const f16* vp = vt + w.vbase + (x & 3) * (ROWS * 32) + (x >> 2) * 16 * 32;
-        lo[x] = read_tr(vp);
-        hi[x] = read_tr(vp + 8 * 32);
+        if constexpr (kScaled<P>) {
+            both[x] = read_tr8(vt + w.vb[(x >> 2) & 1] + (x >> 2) * 16 * P::kRow + (x & 3) * 512);
+        } else {
+            const f16* vp = (const f16*)vt + w.vbase + (x & 3) * (ROWS * 32) + (x >> 2) * 16 * 32;
+            lo[x] = read_tr(vp);
+            hi[x] = read_tr(vp + 8 * 32);
+        }
     };
 #pragma unroll
     for (int x = 0; x < kAhead; ++x) read(x);
@@ -640,7 +799,11 @@ __device__ __forceinline__ void product(Wave& w, const f16* vt, const half8v (&p
     for (int x = 0; x < 8 * NB; ++x) {
         if (x + kAhead < 8 * NB) read(x + kAhead);
         keep_order();
-        const half8v va = __builtin_shufflevector(lo[x], hi[x], 0, 1, 2, 3, 4, 5, 6, 7);
+        half8v va;
+        if constexpr (kScaled<P>)
+            va = widen(both[x], u.v[x >> 2], u.v[x >> 2]);
+        else
+            va = __builtin_shufflevector(lo[x], hi[x], 0, 1, 2, 3, 4, 5, 6, 7);
         w.o[x & 3] = mfma32(va, pb[x >> 2], w.o[x & 3]);
         keep_order();
     }
@@ -713,13 +876,16 @@ __device__ __forceinline__ void leave(Shared<NW>& sh, const Wave& w, int wave, i
 constexpr int kFewRows = 8;
 constexpr float kFewBase = 7.0f;
 static_assert(kFewBase + kRescaleSlack < 16.0f, "weights fit f16");
+template <class P>
 struct Few {
+    using Pages = P;
     static constexpr int kRows = kFewRows;
     half8v qb[4];  // Q^T of k-step ks: dims 32*ks + 8*g .. +8 of query n
     float4v o[8];  // O^T: o[db][i] = dim db*16 + 4*g + i of query n
     float m, l;    // the running maximum less kFewBase, and the sum of weights
-    int kaddr[4];  // K operand of k-step ks, rows 0..15 (halves)
+    int kaddr[4];  // K operand of k-step ks, rows 0..15 (bytes)
     int vbase;
+    int vb[2];     // e4m3: V^T operand source addresses, of even and odd chunks (bytes)
     int g, qpos;  // g: the lane's quarter
     float scale_log2;
 };
@@ -734,16 +900,27 @@ __device__ __forceinline__ float quarters_sum(float x) {
 __device__ __forceinline__ float4v mfma16(const half8v& a, const half8v& b, const float4v& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ void init_wave(Few& w, const PagedAttnArgs& a, const Item& it, int rin, int h, int lane) {
+template <class P>
+__device__ __forceinline__ void init_wave(Few<P>& w, const PagedAttnArgs& a, const Item& it, int rin, int h, int lane) {
     const int r = min(rin, it.rows - 1), n = lane & 15;
     w.g = lane >> 4;
     const f16* q = a.q + ((int64_t)(it.row0 + r) * a.nkvh + it.kvh) * (kRep * kHeadDim) + h * kHeadDim + 8 * w.g;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
         w.qb[ks] = *(const half8v*)(q + 32 * ks);
-        w.kaddr[ks] = n * kHeadDim + (((4 * ks + w.g) ^ swz16(n)) * 8);
+        if constexpr (kScaled<P>)
+            w.kaddr[ks] = n * P::kRow + (((2 * ks + (w.g >> 1)) ^ (n >> 1)) * 16) + 8 * (w.g & 1);
+        else
+            w.kaddr[ks] = n * P::kRow + (((4 * ks + w.g) ^ swz16(n)) * 16);
     }
-    w.vbase = (4 * w.g + (n >> 2)) * 32 + 4 * (n & 3);
+    if constexpr (kScaled<P>) {  // source lane 2 k + m of a quarter: row 4 g + k % 4 of group k / 4
+        const int k = n >> 1, group = k >> 2;
+#pragma unroll
+        for (int odd = 0; odd < 2; ++odd)
+            w.vb[odd] = group * 16 * P::kRow + ((4 * w.g + (k & 3)) ^ 4 * odd ^ 8 * group) * 16 + 8 * (n & 1);
+    } else {
+        w.vbase = (4 * w.g + (n >> 2)) * 32 + 4 * (n & 3);
+    }
     w.qpos = it.pos0 + r;
     w.scale_log2 = a.scale_log2;
 #pragma unroll
@@ -751,7 +928,8 @@ __device__ __forceinline__ void init_wave(Few& w, const PagedAttnArgs& a, const 
     w.m = kNegInf;
     w.l = 0.0f;
 }
-__device__ __forceinline__ void wait_q(Few& w) {
+template <class P>
+__device__ __forceinline__ void wait_q(Few<P>& w) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) asm volatile("" : "+v"(w.qb[ks]));
@@ -759,9 +937,11 @@ __device__ __forceinline__ void wait_q(Few& w) {
 // P^T of a slice: S^T of keys 16 kb + 4 g + i, masked, the running maximum,
 // the weights (B operand: its k 8 g + j is key 16 (j / 4) + 4 g + j % 4), hi and
 // lo, and their sum.
-__device__ __forceinline__ void slice_scores(const Few& w, const f16* kt, float4v (&s)[2]) {
-    half8v ka[8];
-    auto read = [&](int x) { ka[x] = *(const half8v*)&kt[(x & 1) * 16 * kHeadDim + w.kaddr[x >> 1]]; };
+template <class P>
+__device__ __forceinline__ void slice_scores(const Few<P>& w, const char* kt, const Units<2>& u, float4v (&s)[2]) {
+    using Raw = std::conditional_t<kScaled<P>, uint2, half8v>;
+    Raw ka[8];
+    auto read = [&](int x) { ka[x] = *(const Raw*)(kt + (x & 1) * 16 * P::kRow + w.kaddr[x >> 1]); };
     s[0] = s[1] = (float4v){};
 #pragma unroll
     for (int x = 0; x < 4; ++x) read(x);
@@ -770,11 +950,17 @@ __device__ __forceinline__ void slice_scores(const Few& w, const f16* kt, float4
     for (int x = 0; x < 8; ++x) {
         if (x + 4 < 8) read(x + 4);
         keep_order();
-        s[x & 1] = mfma16(ka[x], w.qb[x >> 1], s[x & 1]);
+        half8v k;
+        if constexpr (kScaled<P>)
+            k = widen(ka[x], u.k[x & 1], u.k[x & 1]);
+        else
+            k = ka[x];
+        s[x & 1] = mfma16(k, w.qb[x >> 1], s[x & 1]);
         keep_order();
     }
 }
-__device__ __forceinline__ void slice_weights(Few& w, float4v (&s)[2], int k0, bool mask, uint32_t hidden, half8v (&pb)[2]) {
+template <class P>
+__device__ __forceinline__ void slice_weights(Few<P>& w, float4v (&s)[2], int k0, bool mask, uint32_t hidden, half8v (&pb)[2]) {
 #pragma clang fp contract(off)
     if (mask) {
         const int last = w.qpos - k0 - 4 * w.g;
@@ -816,16 +1002,23 @@ __device__ __forceinline__ void slice_weights(Few& w, float4v (&s)[2], int k0, b
     }
     w.l += quarters_sum(ps[0] + ps[1]);
 }
-__device__ __forceinline__ void slice_product(Few& w, const f16* vt, const half8v (&pb)[2]) {
+template <class P>
+__device__ __forceinline__ void slice_product(Few<P>& w, const char* vt, const Units<2>& u, const half8v (&pb)[2]) {
     half4v lo[8], hi[8];  // keys 0..15 and 16..31
+    uint2 both[8];
+    half8v va[8];
     auto add = [&](int x, int part) {
-        w.o[x] = mfma16(__builtin_shufflevector(lo[x], hi[x], 0, 1, 2, 3, 4, 5, 6, 7), pb[part], w.o[x]);
+        w.o[x] = mfma16(va[x], pb[part], w.o[x]);
         keep_order();
     };
     auto read = [&](int x) {
-        const f16* vp = vt + w.vbase + (x >> 1) * (kSlice * 32) + (x & 1) * 16;
-        lo[x] = read_tr(vp);
-        hi[x] = read_tr(vp + 16 * 32);
+        if constexpr (kScaled<P>) {
+            both[x] = read_tr8(vt + w.vb[x & 1] + x * 256);
+        } else {
+            const f16* vp = (const f16*)vt + w.vbase + (x >> 1) * (kSlice * 32) + (x & 1) * 16;
+            lo[x] = read_tr(vp);
+            hi[x] = read_tr(vp + 16 * 32);
+        }
     };
 #pragma unroll
     for (int x = 0; x < 4; ++x) read(x);
@@ -834,14 +1027,18 @@ __device__ __forceinline__ void slice_product(Few& w, const f16* vt, const half8
     for (int x = 0; x < 8; ++x) {
         if (x + 4 < 8) read(x + 4);
         keep_order();
+        if constexpr (kScaled<P>)
+            va[x] = widen(both[x], u.v[0], u.v[1]);
+        else
+            va[x] = __builtin_shufflevector(lo[x], hi[x], 0, 1, 2, 3, 4, 5, 6, 7);
         add(x, 0);
         if (x >= 2) add(x - 2, 1);  // not right behind the product it adds to
     }
     add(6, 1);
     add(7, 1);
 }
-template <int NW>
-__device__ __forceinline__ void leave_all(Shared<NW>& sh, const Few& w, int wave, int lane) {
+template <int NW, class P>
+__device__ __forceinline__ void leave_all(Shared<NW>& sh, const Few<P>& w, int wave, int lane) {
     float4* dst = reinterpret_cast<float4*>(sh.buf) + wave * 1024 + lane;
 #pragma unroll
     for (int db = 0; db < 8; ++db) dst[db * 64] = make_float4(w.o[db][0], w.o[db][1], w.o[db][2], w.o[db][3]);
@@ -853,19 +1050,28 @@ __device__ __forceinline__ void put_dims(const PagedAttnArgs& a, const Item& it,
 }
 
 // And of up to 16 rows.
-struct Many : Wave {
+template <class P>
+struct Many : PageWave<P> {
+    using Pages = P;
     static constexpr int kRows = kNarrowRows;
 };
-__device__ __forceinline__ void slice_scores(const Many& w, const f16* kt, float16v (&s)[1]) { scores<1>(w, kt, s); }
-__device__ __forceinline__ void slice_weights(Many& w, float16v (&s)[1], int k0, bool mask, uint32_t hidden, half8v (&pb)[2]) {
+template <class P>
+__device__ __forceinline__ void slice_scores(const Many<P>& w, const char* kt, const Units<2>& u, float16v (&s)[1]) {
+    scores<P, 1>(w, kt, u, s);
+}
+template <class P>
+__device__ __forceinline__ void slice_weights(Many<P>& w, float16v (&s)[1], int k0, bool mask, uint32_t hidden, half8v (&pb)[2]) {
     if (mask) mask_scores<1>(w, s, k0);
     if (rarely(hidden)) hide_scores<1>(s, hidden);
     const Exponent e = move_max<1>(w, s);
     weights<1>(w, s, e, pb);
 }
-__device__ __forceinline__ void slice_product(Many& w, const f16* vt, const half8v (&pb)[2]) { product<kSlice, 1>(w, vt, pb); }
-template <int NW>
-__device__ __forceinline__ void leave_all(Shared<NW>& sh, const Many& w, int wave, int lane) { leave<4>(sh, w, wave, 0, lane); }
+template <class P>
+__device__ __forceinline__ void slice_product(Many<P>& w, const char* vt, const Units<2>& u, const half8v (&pb)[2]) {
+    product<P, kSlice, 1>(w, vt, u, pb);
+}
+template <int NW, class P>
+__device__ __forceinline__ void leave_all(Shared<NW>& sh, const Many<P>& w, int wave, int lane) { leave<4>(sh, w, wave, 0, lane); }
 __device__ __forceinline__ void put_dims(const PagedAttnArgs& a, const Item& it, const float (&o)[16], float l, int wave,
                                          int g, int r, int h) {
     put_block<4>(a, it, o, l, wave, 0, g, r, h);
@@ -873,21 +1079,27 @@ __device__ __forceinline__ void put_dims(const PagedAttnArgs& a, const Item& it,
 
 template <class W, class S, int NS, int NP>
 __device__ __forceinline__ void run_narrow(const PagedAttnArgs& a, const Item& it, Pages pg, Shared<kNarrowWaves>& sh, Draw& next) {
+    using P = typename W::Pages;
     const int tid = thread_id(), lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     constexpr int kCols = kRep * W::kRows, kElems = kCols / 2;
     const int n = lane & (kCols - 1), h = n / W::kRows, rin = n % W::kRows;
-    f16* kbuf = sh.buf + wave * (2 * kSlice * kHeadDim);
-    f16* vbuf = kbuf + kSlice * kHeadDim;
-    const Offsets whole = group_offsets(lane, 0, 15, (uint32_t)a.kv_stride * 2);
+    // (16 KB a wave in both formats: the state that it leaves for the others at
+    // the end takes them, while they may still read their slices.)
+    const char* kbuf = (const char*)sh.buf + wave * (2 * kSlice * kHeadDim * (int)sizeof(f16));
+    const char* vbuf = kbuf + kSlice * P::kRow;
+    const Offsets<P> whole = group_offsets<P>(a, lane, 0, 15);
+    constexpr int kGroup = 16 * P::kRow;
 
     // Copies of the slice of tile t: its K or its V.
     auto copy_slice = [&](int t, bool v) {
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
             const int key = t * kNarrowTile + wave * kSlice + 16 * p;
-            const uint32_t lds = v ? lds_addr(vbuf) + p * 1024 : lds_addr(kbuf) + p * 4096;
-            copy_group(a, it, group_base(a, it, pg, key), whole, key, v, lds, v ? kSlice * 64 : 1024);
+            const bool slabs = v && !kScaled<P>;  // f16: 32 dims of the whole slice together
+            const uint32_t lds = lds_addr(v ? vbuf : kbuf) + p * (slabs ? 1024 : kGroup);
+            copy_group<P>(a, it, group_base<P>(a, it, pg, key), whole, key, v, kScaled<P> ? p : 0, lds,
+                          slabs ? kSlice * 64 : 1024);
         }
     };
     W w;
@@ -896,9 +1108,18 @@ __device__ __forceinline__ void run_narrow(const PagedAttnArgs& a, const Item& i
         copy_slice(it.tile0, false);
         copy_slice(it.tile0, true);
     }
+    uint32_t scales = 0;
+    if constexpr (kScaled<P>) scales = load_scales(a, it, pg, it.tile0 * kNarrowTile + wave * kSlice);
     wait_q(w);
+    asm volatile("" : "+v"(scales));
     for (int t = it.tile0; t < it.tile1; ++t) {
         const int k0 = t * kNarrowTile + wave * kSlice;
+        Units<2> u{};
+        if constexpr (kScaled<P>) {
+            const int turn = (t - it.tile0) % kScaleTiles;
+            if (rarely(turn == 0 && t > it.tile0)) scales = load_scales(a, it, pg, k0);
+            u = units<2>(scales, turn * (kNarrowTile / 16));
+        }
         const bool more = t + 1 < it.tile1;
         const uint32_t hidden = hidden_groups<2>(a, it, pg, k0);
         if (more) advance_pages(a, it, pg, k0 + kNarrowTile);
@@ -906,20 +1127,20 @@ __device__ __forceinline__ void run_narrow(const PagedAttnArgs& a, const Item& i
             WAIT_VM(0);
             break;
         }
-        WAIT_VM(8);  // K landed, V in flight
+        wait_copies<2 * P::kCopies>();  // K landed, V in flight
         S s[NS];
         half8v pb[NP];
-        slice_scores(w, kbuf, s);
+        slice_scores(w, kbuf, u, s);
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             copy_slice(t + 1, false);
         }
         slice_weights(w, s, k0, k0 + kSlice - 1 > it.pos0, hidden, pb);
         if (more)
-            WAIT_VM(8);
+            wait_copies<2 * P::kCopies>();
         else
             WAIT_VM(0);
-        slice_product(w, vbuf, pb);
+        slice_product(w, vbuf, u, pb);
         if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
             copy_slice(t + 1, true);
@@ -942,63 +1163,82 @@ __device__ __forceinline__ void run_narrow(const PagedAttnArgs& a, const Item& i
         t = not_finite<kElems>(o, L);
     }
     if (rarely(__ballot(t != t)))
-        put_exact(a, it, it.tile0 * kNarrowTile, min(it.tile1 * kNarrowTile, it.kend), L, wave, rin, h, valid,
+        put_exact<P>(a, it, it.tile0 * kNarrowTile, min(it.tile1 * kNarrowTile, it.kend), L, wave, rin, h, valid,
                   kCols == 32 ? ~0u : 0xffffu);
     else if (valid)
         put_dims(a, it, o, L, wave, w.g, rin, h);
     if (it.splits > 1 && valid && wave == 0 && w.g == 0) store_dev2(range_ml(a, it, it.split) + column(it, rin, h) * 2, M, L);
 }
 
+template <class P>
 __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it, Pages pg, Shared<kNarrowWaves>& sh, Draw& next) {
     if (it.planned <= kFewRows)
-        run_narrow<Few, float4v, 2, 2>(a, it, pg, sh, next);
+        run_narrow<Few<P>, float4v, 2, 2>(a, it, pg, sh, next);
     else
-        run_narrow<Many, float16v, 1, 2>(a, it, pg, sh, next);
+        run_narrow<Many<P>, float16v, 1, 2>(a, it, pg, sh, next);
     if (it.splits > 1) arrive(a, it, sh);
 }
 
+template <class P>
 __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it, Pages pg, Shared<kWideWaves>& sh, Draw& next) {
     const int tid = thread_id(), lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rw = wave & 3, kg = wave >> 2;  // 16 rows; 64 keys of every tile
     const int n = lane & 31, h = n >> 4, rin = rw * 16 + (n & 15);
-    constexpr int kTile = kWideTile * kHeadDim, kGroup = kWideTile / 2;
-    const Offsets whole = group_offsets(lane, 0, 15, (uint32_t)a.kv_stride * 2);
+    constexpr int kTile = kWideTile * P::kRow, kGroup = kWideTile / 2;  // bytes, keys
+    const Offsets<P> whole = group_offsets<P>(a, lane, 0, 15);
 
     // This wave's 16 keys of tile t into buffer t & 1: K, then V in slabs.
     auto copy_tile = [&](int t) {
         const int key = t * kWideTile + wave * 16;
-        const f16* base = group_base(a, it, pg, key);
-        const uint32_t lds = lds_addr(sh.buf) + (t & 1) * (4 * kTile);
-        copy_group(a, it, base, whole, key, false, lds + wave * 4096, 1024);
-        copy_group(a, it, base, whole, key, true, lds + 2 * kTile + wave * 1024, kWideTile * 64);
+        const char* base = group_base<P>(a, it, pg, key);
+        const uint32_t lds = lds_addr(sh.buf) + (t & 1) * (2 * kTile);
+        copy_group<P>(a, it, base, whole, key, false, 0, lds + wave * 16 * P::kRow, 1024);
+        if constexpr (kScaled<P>) {  // (a select of the two orders' registers, not an index)
+            if (wave & 1)
+                copy_group<P>(a, it, base, whole, key, true, 1, lds + kTile + wave * 16 * P::kRow, 1024);
+            else
+                copy_group<P>(a, it, base, whole, key, true, 0, lds + kTile + wave * 16 * P::kRow, 1024);
+        } else {
+            copy_group<P>(a, it, base, whole, key, true, 0, lds + kTile + wave * 1024, kWideTile * 64);
+        }
     };
-    Wave w;
+    PageWave<P> w;
     init_wave(w, a, it, rin, h, lane);
     if (it.tile0 < it.tile1) copy_tile(it.tile0);
     const int first_pos = it.pos0 + rw * 16;
     const int last_pos = it.pos0 + min(rw * 16 + 15, it.rows - 1);
     const bool live = rw * 16 < it.rows;
+    uint32_t scales = 0;
+    if constexpr (kScaled<P>) scales = load_scales(a, it, pg, it.tile0 * kWideTile);
     wait_q(w);
+    asm volatile("" : "+v"(scales));
     for (int t = it.tile0; t < it.tile1; ++t) {
         WAIT_VM(0);
         __syncthreads();  // tile t is here, and the other buffer is read
         const int k0 = t * kWideTile + kg * kGroup;
+        Units<4> u{};
+        if constexpr (kScaled<P>) {
+            const int turn = (t - it.tile0) % kScaleTiles;
+            if (rarely(turn == 0 && t > it.tile0)) scales = load_scales(a, it, pg, t * kWideTile);
+            u = units<4>(scales, turn * (kWideTile / 16) + kg * 4);
+        }
         const uint32_t hidden = hidden_groups<4>(a, it, pg, k0);
         if (t + 1 < it.tile1) {
             advance_pages(a, it, pg, (t + 1) * kWideTile);
             copy_tile(t + 1);
         }
         if (!live || k0 > last_pos) continue;
-        const f16* kt = sh.buf + (t & 1) * 2 * kTile + kg * kGroup * kHeadDim;
+        const char* kt = (const char*)sh.buf + (t & 1) * 2 * kTile + kg * kGroup * P::kRow;
         float16v s[2];
         half8v pb[4];
-        scores<2>(w, kt, s);
+        scores<P, 2>(w, kt, u, s);
         if (k0 + kGroup - 1 > first_pos) mask_scores<2>(w, s, k0);
         if (rarely(hidden)) hide_scores<2>(s, hidden);
         const Exponent e = move_max<2>(w, s);
         weights<2>(w, s, e, pb);
-        product<kWideTile, 2>(w, sh.buf + (t & 1) * 2 * kTile + kTile + kg * kGroup * 32, pb);
+        const char* vt = (const char*)sh.buf + (t & 1) * 2 * kTile + kTile + kg * kGroup * (kScaled<P> ? P::kRow : 64);
+        product<P, kWideTile, 2>(w, vt, u, pb);
     }
     draw(next);
     __syncthreads();  // the buffers are read
@@ -1015,7 +1255,7 @@ __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it,
         combine<2, 16>(sh, rw, 4, db * 16, lane, o, M, L);
         const float t = not_finite<16>(o, L);
         if (rarely(__ballot(valid && t != t)))
-            put_exact(a, it, it.tile0 * kWideTile, min(it.tile1 * kWideTile, it.kend), L, db, rin, h, valid, ~0u);
+            put_exact<P>(a, it, it.tile0 * kWideTile, min(it.tile1 * kWideTile, it.kend), L, db, rin, h, valid, ~0u);
         else if (valid)
             put_block<4>(a, it, o, L, db, 0, w.g, rin, h);
     }
@@ -1027,7 +1267,7 @@ __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it,
 // launch) start with one each and, where there are more items, draw the next
 // from the head's counter, so that a workgroup of short items takes more of
 // them.  The last workgroup to leave puts the counters back to zero.
-template <int NW>
+template <class P, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_kernel(
     PagedAttnArgs a) {
     __shared__ __attribute__((aligned(1024))) Shared<NW> sh;
@@ -1065,7 +1305,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         it.page0 = word(8);
         it.last_page = (it.kend - 1) >> a.page_shift;
         it.table = a.table + (int64_t)word(0) * a.stride;
-        it.base = a.base + it.kvh * a.head_stride;
+        it.base = (const char*)a.base + it.kvh * a.head_stride * P::kElem;
         if (it.rows > 0) {
             Pages pg;
             pg.cur = check_pages(a, words);
@@ -1073,7 +1313,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
             pg.lo = -kPagedItemHead;
             pg.nxt = {0, 0};
             if (it.last_page - it.page0 >= kPagedItemPages) pg.nxt = check_pages(a, load_pages(it, kPagedItemPages));
-            run_item(a, it, pg, sh, draw_next);
+            run_item<P>(a, it, pg, sh, draw_next);
         } else {
             draw(draw_next);
         }
@@ -1093,17 +1333,26 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
 }  // namespace
 
-hipError_t launch_paged_attn(const PagedAttnArgs& a, int cus, hipStream_t stream) {
-    if (a.rows <= 0) return hipSuccess;
+namespace {
+
+template <class P>
+hipError_t launch(const PagedAttnArgs& a, int cus, hipStream_t stream) {
     if (a.max_wide > 0) {
         const int64_t wgs = std::min<int64_t>((int64_t)a.max_wide * a.nkvh, cus);
-        hipLaunchKernelGGL(paged_attn_kernel<kWideWaves>, dim3((unsigned)wgs), dim3(kWideWaves * 64), 0, stream, a);
+        hipLaunchKernelGGL((paged_attn_kernel<P, kWideWaves>), dim3((unsigned)wgs), dim3(kWideWaves * 64), 0, stream, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
     const int64_t wgs = std::min<int64_t>((int64_t)a.max_narrow * a.nkvh, 2 * (int64_t)cus);
-    hipLaunchKernelGGL(paged_attn_kernel<kNarrowWaves>, dim3((unsigned)wgs), dim3(kNarrowWaves * 64), 0, stream, a);
+    hipLaunchKernelGGL((paged_attn_kernel<P, kNarrowWaves>), dim3((unsigned)wgs), dim3(kNarrowWaves * 64), 0, stream, a);
     return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_paged_attn(const PagedAttnArgs& a, int cus, hipStream_t stream) {
+    if (a.rows <= 0) return hipSuccess;
+    return a.scales ? launch<E4m3Pages>(a, cus, stream) : launch<F16Pages>(a, cus, stream);
 }
 
 }  // namespace qasr

@@ -42,6 +42,7 @@ ABI_SYMBOLS = (
     "qasr_pages_create", "qasr_pages_destroy", "qasr_pages_get_info", "qasr_paged_plan_create",
     "qasr_paged_plan_destroy", "qasr_paged_plan_get_info", "qasr_paged_plan_build",
     "qasr_paged_append", "qasr_paged_attn", "qasr_plan_paged",
+    "qasr_pages_create_e4m3", "qasr_pages_get_scales",
 )
 MAX_PREFILL_SEGMENTS = 64  # segments per qasr_decoder_prefill_batch call
 
@@ -110,6 +111,18 @@ class PagesInfo(ctypes.Structure):
         ("page_stride", ctypes.c_int64),
         ("kv_stride", ctypes.c_int64),
         ("head_stride", ctypes.c_int64),
+        ("bytes", ctypes.c_size_t),
+    ]
+
+
+class PagesScales(ctypes.Structure):
+    _fields_ = [
+        ("base_dev", ctypes.c_void_p),
+        ("block_rows", ctypes.c_int32),
+        ("head_stride", ctypes.c_int32),
+        ("kv_stride", ctypes.c_int32),
+        ("page_stride", ctypes.c_int32),
+        ("layer_stride", ctypes.c_int64),
         ("bytes", ctypes.c_size_t),
     ]
 
@@ -184,6 +197,8 @@ def load(path: str = LIB_PATH):
     L.qasr_plan_decode.argtypes = [ctypes.c_int, i32p, ctypes.c_int, ctypes.c_int, i32p, i32p, i32p]
     L.qasr_plan_prefill.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int, i32p, i32p, i32p, i32p]
     L.qasr_pages_create.argtypes = [_vp, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)]
+    L.qasr_pages_create_e4m3.argtypes = L.qasr_pages_create.argtypes
+    L.qasr_pages_get_scales.argtypes = [_vp, ctypes.POINTER(PagesScales)]
     L.qasr_pages_destroy.argtypes = [_vp]
     L.qasr_pages_destroy.restype = None
     L.qasr_pages_get_info.argtypes = [_vp, ctypes.POINTER(PagesInfo)]
@@ -360,7 +375,7 @@ class KVPool:
 
 class _DeviceView:
     """__cuda_array_interface__ over library-owned device memory (f16, or
-    int32 with typestr "<i4").  A torch tensor made of it, and every view of
+    int32 with typestr "<i4", bytes with "|u1").  A torch tensor made of it, and every view of
     that tensor, holds on to it and so to `owner`, the object that frees the
     memory."""
 
@@ -484,15 +499,19 @@ PAGED_MAX_ROWS = 65536
 
 class PagePool:
     """One pool of KV pages for all sequences (qasr_pages):
-    [layer][page][K|V][kvh][page_rows][hd] f16, zeroed."""
+    [layer][page][K|V][kvh][page_rows][hd], zeroed; `fmt` "f16", or "e4m3" with
+    one power of two for each 16 rows of a head."""
 
-    def __init__(self, ctx: Context, pages: int, page_rows: int = 16):
+    def __init__(self, ctx: Context, pages: int, page_rows: int = 16, fmt: str = "f16"):
         self.ctx = ctx
         self.handle = None
+        if fmt not in ("f16", "e4m3"):
+            raise QasrError(QASR_EINVAL, f'fmt must be "f16" or "e4m3", got {fmt!r}')
         h = _vp()
-        _check(load().qasr_pages_create(ctx.handle, pages, page_rows, ctypes.byref(h)))
+        create = load().qasr_pages_create if fmt == "f16" else load().qasr_pages_create_e4m3
+        _check(create(ctx.handle, pages, page_rows, ctypes.byref(h)))
         self.handle = h
-        self.pages, self.page_rows = pages, page_rows
+        self.pages, self.page_rows, self.fmt = pages, page_rows, fmt
 
     def info(self) -> PagesInfo:
         if not self.ctx.handle:
@@ -503,13 +522,27 @@ class PagePool:
 
     def tensor(self):
         """A torch view of the whole pool, shaped
-        [layer][page][2][kvh][page_rows][hd]."""
+        [layer][page][2][kvh][page_rows][hd], f16 or float8_e4m3fn."""
         import torch
 
         inf = self.info()
-        storage = _DeviceView(inf.base_dev, inf.bytes, self.ctx.device, owner=self)
+        f16 = self.fmt == "f16"
+        storage = _DeviceView(inf.base_dev, inf.bytes, self.ctx.device, "<f2" if f16 else "|u1", self)
         t = torch.as_tensor(storage, device=f"cuda:{self.ctx.device}")
+        t = t if f16 else t.view(torch.float8_e4m3fn)
         return t.view(inf.layers, inf.pages, 2, inf.nkvh, inf.page_rows, inf.head_dim)
+
+    def scales(self):
+        """A torch view of an e4m3 pool's scales, float8_e8m0fnu, shaped
+        [layer][page][2][kvh][page_rows / 16]: what an element stands for is
+        itself times its block's scale."""
+        import torch
+
+        inf, s = self.info(), PagesScales()
+        _check(load().qasr_pages_get_scales(self.handle, ctypes.byref(s)))
+        storage = _DeviceView(s.base_dev, s.bytes, self.ctx.device, "|u1", self)
+        t = torch.as_tensor(storage, device=f"cuda:{self.ctx.device}").view(torch.float8_e8m0fnu)
+        return t.view(inf.layers, inf.pages, 2, inf.nkvh, inf.page_rows // s.block_rows)
 
     def free_ring(self):
         """The ring and cursor of a pool with every page free: int32 CUDA
