@@ -110,12 +110,14 @@ struct Item {
 // places as from f16 pages: the outputs have the same bits as over f16 pages
 // that hold these numbers.
 struct F16Pages {
+    using T = f16;
     static constexpr int kElem = 2;
     static constexpr int kRow = kHeadDim * kElem;  // bytes
     static constexpr int kCopies = 4;              // 1 KB each, of a 16-row group's K or V
     static constexpr int kOrders = 1;              // of a group's V in the LDS
 };
 struct E4m3Pages {
+    using T = uint8_t;
     static constexpr int kElem = 1;
     static constexpr int kRow = kHeadDim * kElem;
     static constexpr int kCopies = 2;
@@ -234,7 +236,7 @@ __device__ __forceinline__ const char* group_base(const PagedAttnArgs& a, const 
     const int k = min(key, it.kend - 1), r = (k >> a.page_shift) - it.page0 - p.lo;
     const int id = __builtin_amdgcn_readlane(r < 64 ? p.cur.id : p.nxt.id, r & 63);
     const uint64_t page = (uint64_t)(uint32_t)id * (uint32_t)a.page_stride;  // a page is < 2^21 elements
-    return it.base + page * P::kElem + ((k & ((1 << a.page_shift) - 1)) & ~15) * P::kRow;
+    return (const char*)((const typename P::T*)it.base + page + ((k & ((1 << a.page_shift) - 1)) & ~15) * kHeadDim);
 }
 // Scales of the 64 16-key groups from that of `key` on, a lane each, K's byte
 // (an f32's exponent) and V's above it; past the end: of the last key's group.
@@ -476,6 +478,7 @@ template <class P>
 __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& it, int key0, int key1, int r, int h,
                                             int db, int lane, float& sum) {
     const int pos = it.pos0 + r, end = min(key1, pos + 1);
+    const auto* base = (const typename P::T*)it.base;
     const f16* q = a.q + ((int64_t)(it.row0 + r) * a.nkvh + it.kvh) * (kRep * kHeadDim) + h * kHeadDim;
     // This lane's key of the 64 from k0 on: its row (and the unit of its V),
     // whether it is seen, and its score.
@@ -496,9 +499,9 @@ __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& 
         for (int d = 0; d < kHeadDim; d += 8) {
             H8 x, y;
             if constexpr (kScaled<P>)
-                x.h = widen(*(const uint2*)(it.base + row + d), k_unit, k_unit);
+                x.h = widen(*(const uint2*)(base + row + d), k_unit, k_unit);
             else
-                x.u = *(const uint4*)(it.base + (row + d) * P::kElem);
+                x.u = *(const uint4*)(base + row + d);
             y.u = *(const uint4*)(q + d);
 #pragma unroll
             for (int e = 0; e < 8; ++e) s = fmaf(h2f(x.e[e]), h2f(y.e[e]), s);
@@ -524,12 +527,12 @@ __device__ __forceinline__ float exact_dims(const PagedAttnArgs& a, const Item& 
             todo &= todo - 1;
             const uint64_t at = (uint64_t)__shfl((int)(uint32_t)(row >> 32), j) << 32 |
                                 (uint32_t)__shfl((int)(uint32_t)row, j);
-            const char* v = it.base + (at + a.kv_stride + 32 * db + (lane & 31)) * P::kElem;
+            const auto v = base[at + a.kv_stride + 32 * db + (lane & 31)];
             if constexpr (kScaled<P>) {
                 const float u = __shfl(unit, j);
-                o = fmaf(__shfl(p, j), h2f(widen(make_uint2(*(const uint8_t*)v, 0), u, u)[0]), o);
+                o = fmaf(__shfl(p, j), h2f(widen(make_uint2(v, 0), u, u)[0]), o);
             } else {
-                o = fmaf(__shfl(p, j), h2f(*(const f16*)v), o);
+                o = fmaf(__shfl(p, j), h2f(v), o);
             }
         }
     }
@@ -759,7 +762,11 @@ __device__ __forceinline__ void scores(const PageWave<P>& w, const char* kt, con
     if constexpr (kScaled<P>) {
         const bool second = thread_id() & 16;
 #pragma unroll
-        for (int kb = 0; kb < NB; ++kb) unit[kb] = second ? u.k[2 * kb + 1] : u.k[2 * kb];
+        for (int kb = 0; kb < NB; ++kb) {
+            float even = u.k[2 * kb], odd = u.k[2 * kb + 1];
+            asm("" : "+s"(even), "+s"(odd));  // (else a select of addresses, and `u` in memory)
+            unit[kb] = second ? odd : even;
+        }
     }
 #pragma unroll
     for (int x = 0; x < kAhead; ++x) read(x);
