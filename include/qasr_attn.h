@@ -362,6 +362,93 @@ int qasr_paged_attn(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows,
                     const int32_t* table_dev, int table_stride, const void* q_dev, void* out_dev,
                     void* stream);
 
+/* Forks: requests go on as others do (beams after a selection, several
+ * continuations of one prompt), and end.  shared_dev, `pages` numbers, counts
+ * the requests beyond the first that hold a page: 0 for one that one request
+ * holds, and for a free one.  A pool without shared pages starts with zeros;
+ * qasr_paged_plan_build leaves them as they are.  */
+typedef struct qasr_paged_fork_ws qasr_paged_fork_ws;
+typedef struct qasr_paged_fork_info {
+    int32_t max_requests;
+    int32_t max_pages;   /* of a request */
+    int32_t* status_dev; /* [max_requests] QASR_OK, or why the last fork was not carried out */
+    size_t bytes;        /* device memory of the workspace */
+} qasr_paged_fork_info;
+
+/* A workspace for forks of up to max_requests (<= QASR_PAGED_MAX_REQUESTS)
+ * requests whose tables are up to max_pages wide; 4 bytes for each entry of such
+ * a table. */
+int qasr_paged_fork_create(qasr_ctx* ctx, qasr_pages* pool, int max_requests, int max_pages,
+                           qasr_paged_fork_ws** out);
+void qasr_paged_fork_destroy(qasr_paged_fork_ws* fork);
+int qasr_paged_fork_get_info(const qasr_paged_fork_ws* fork, qasr_paged_fork_info* out);
+
+/* Request i goes on as request parent_dev[i] is (itself: it stays as it is), or
+ * is released (-1); len_dev, table_dev, shared_dev, ring_dev and cursor_dev are
+ * changed in place.  len_dev[i] becomes its parent's, or 0; its table entries its
+ * parent's.  Full pages are shared.  The unfinished last page of a parent, which
+ * the next step writes, stays with the parent itself if it goes on from itself,
+ * else with the first request that does; each other one gets a page of the ring, in
+ * request order, with the rows that are there of all layers (and, of an e4m3 pool,
+ * their scales).  An unfinished page that another request outside the call holds is
+ * copied for all.  Pages that nobody holds any more go to the ring's end, by
+ * their place in the table, then by request, and are free from the next call on.
+ * Entries outside the pool are handed on as they are, and nothing is copied from
+ * or to such a page.
+ *
+ * All or nothing: status_dev[i] is QASR_EINVAL for a parent outside [-1, nreq) or
+ * a length that is negative or past the table, QASR_ENOMEM for the requests that
+ * want a copy when the free pages do not reach for all of them; if any is not
+ * QASR_OK, nothing is changed.
+ *
+ * A page lies at the same place of every table that lists it (a shared prefix
+ * does), and shared_dev holds the truth about all requests of the pool, those of
+ * other calls too.  len_dev and cursor_dev may be a plan's lens_dev and
+ * cursor_dev.  No two arrays overlap.  The call does not allocate or synchronise
+ * and may be captured; calls that share the workspace, or pages, are ordered on
+ * one stream. */
+int qasr_paged_fork(qasr_ctx* ctx, qasr_paged_fork_ws* fork, int nreq, int32_t* len_dev,
+                    const int32_t* parent_dev, int32_t* table_dev, int table_stride,
+                    int32_t* shared_dev, int32_t* ring_dev, int32_t* cursor_dev, void* stream);
+
+/* ---- Beam selection -------------------------------------------------------
+ * The reference decodes greedily: no counterpart in it.  Takes the logits that
+ * qasr_decoder_step writes (a row for each beam); what it selects is what
+ * qasr_paged_fork takes. */
+typedef struct qasr_beam qasr_beam;
+
+/* A workspace for up to max_groups (1 .. 1024) groups of `width` (1 .. 32) beams
+ * over `vocab` (1 .. 1 << 20) tokens, k (1 .. 32) candidates a group. */
+int qasr_beam_create(qasr_ctx* ctx, int max_groups, int width, int vocab, int k, qasr_beam** out);
+void qasr_beam_destroy(qasr_beam* beam);
+
+/* The k best candidates of each group, best first.  Beam b of group g is row r =
+ * g*width + b; candidate (r, t) has the score scores_dev[r] + logits[r][t] -
+ * log(sum over u of exp(logits[r][u])), logits row r at logits_dev +
+ * r*logits_stride (floats; rows need not be aligned).  A beam that has ended
+ * (done_dev[r] not 0; done_dev may be NULL) has one candidate, (r, eos) with
+ * scores_dev[r].  Equal scores go to the lower beam, then to the lower token.
+ * Place i of group g in the outputs, all [groups][k]: parent_dev the row r,
+ * token_dev t, out_scores_dev the score, out_done_dev (or NULL) 1 if the beam has
+ * ended or t is eos (-1: no token ends a beam), else 0.
+ *
+ * A beam whose score is not finite, or with a NaN or +inf among its logits, has
+ * no candidate, and tokens of -inf are none: a group at its first step is one
+ * beam with scores of -inf beside it.  Places behind the last candidate hold
+ * parent and token -1, score -inf, done 0.  Rows that have no logits to offer
+ * are not read.
+ *
+ * Sums are formed in f32 over pieces of 4096 tokens and more, everything behind
+ * them in f64; scores are compared in f64 and rounded once.  A group's results
+ * are a function of its own rows.  Outputs may be the inputs' arrays (out_scores
+ * scores, out_done done) if k is width; they overlap nothing else.  Does not
+ * allocate or synchronise, may be captured; calls that share the workspace are
+ * ordered on one stream. */
+int qasr_beam_select(qasr_ctx* ctx, qasr_beam* beam, int groups, const float* logits_dev,
+                     int64_t logits_stride, const float* scores_dev, const int32_t* done_dev, int eos,
+                     int32_t* parent_dev, int32_t* token_dev, float* out_scores_dev,
+                     int32_t* out_done_dev, void* stream);
+
 /* ---- Whole text decoder around the attention path ------------------------
  * The layer sequence of src/cpu_decoder.rs:367-532 (CpuTextDecoder::forward,
  * final_norm_logits, argmax, prefill, step), i.e. what WgpuTextDecoder::step

@@ -10,6 +10,7 @@
 
 #include "abi_internal.hpp"
 #include "paged.hpp"
+#include "paged_fork.hpp"
 
 using qasr::f16;
 using qasr_abi::DeviceScope;
@@ -44,6 +45,21 @@ struct qasr_paged_plan {
     // The last build, for the checks of the calls that follow it.
     int32_t nreq = 0;
     int32_t stride = 0;
+};
+
+struct qasr_paged_fork_ws {
+    qasr_ctx* ctx;
+    int device;
+    qasr_pages* pool;
+    int32_t max_requests;
+    int32_t max_pages;
+    char* mem = nullptr;
+    size_t bytes = 0;
+    int32_t* status;
+    qasr::ForkHead* head;
+    qasr::ForkRow* rows;
+    qasr::ForkCopy* copies;
+    int32_t *gone, *n_gone;
 };
 
 namespace {
@@ -458,6 +474,131 @@ int qasr_paged_attn(qasr_ctx* ctx, qasr_paged_plan* plan, int layer, int rows, c
     a.drawn = plan->drawn;
     const hipError_t e = qasr::launch_paged_attn(a, ctx->cus, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(e, "paged attention launch");
+    return QASR_OK;
+}
+
+int qasr_paged_fork_create(qasr_ctx* ctx, qasr_pages* pool, int max_requests, int max_pages, qasr_paged_fork_ws** out) {
+    if (!ctx || !pool || !out) return fail(QASR_EINVAL, "null argument");
+    *out = nullptr;
+    if (pool->ctx != ctx) return fail(QASR_EINVAL, "page pool belongs to another context");
+    if (max_requests < 1 || max_requests > qasr::kPagedMaxRequests)
+        return fail(QASR_EINVAL, "max_requests %d outside [1, %d]", max_requests, qasr::kPagedMaxRequests);
+    if (max_pages < 1 || max_pages > 1 << 24) return fail(QASR_EINVAL, "max_pages %d outside [1, %d]", max_pages, 1 << 24);
+    qasr_paged_fork_ws* f = new (std::nothrow) qasr_paged_fork_ws();
+    if (!f) return fail(QASR_ENOMEM, "out of host memory");
+    f->ctx = ctx;
+    f->device = ctx->device;
+    f->pool = pool;
+    f->max_requests = max_requests;
+    f->max_pages = max_pages;
+    const size_t blocks = (max_pages + qasr::kForkColumns - 1) / qasr::kForkColumns;
+    size_t at = 0;
+    auto part = [&](size_t n) {
+        const size_t a = at;
+        at += (n + 255) / 256 * 256;
+        return a;
+    };
+    const size_t o_head = part(sizeof(qasr::ForkHead)), o_st = part(4 * (size_t)max_requests), clear = at;
+    const size_t o_rows = part(sizeof(qasr::ForkRow) * max_requests), o_cp = part(sizeof(qasr::ForkCopy) * max_requests);
+    const size_t o_n = part(4 * blocks), o_gone = part(4 * blocks * qasr::kForkColumns * max_requests);
+    f->bytes = at;
+    DeviceScope ds(ctx->device);
+    hipError_t e = ds.err;
+    if (e == hipSuccess) e = hipMalloc(&f->mem, f->bytes);
+    if (e == hipSuccess) e = hipMemset(f->mem, 0, clear);
+    if (e == hipSuccess) e = hipDeviceSynchronize();
+    if (e != hipSuccess) {
+        if (f->mem) (void)hipFree(f->mem);
+        delete f;
+        (void)hipGetLastError();  // the next launch must not report it
+        return hip_fail(e, "paged fork allocation");
+    }
+    f->head = (qasr::ForkHead*)(f->mem + o_head);
+    f->status = (int32_t*)(f->mem + o_st);
+    f->rows = (qasr::ForkRow*)(f->mem + o_rows);
+    f->copies = (qasr::ForkCopy*)(f->mem + o_cp);
+    f->n_gone = (int32_t*)(f->mem + o_n);
+    f->gone = (int32_t*)(f->mem + o_gone);
+    *out = f;
+    return QASR_OK;
+}
+
+void qasr_paged_fork_destroy(qasr_paged_fork_ws* f) {
+    if (!f) return;
+    DeviceScope ds(f->device);
+    (void)hipDeviceSynchronize();
+    if (f->mem) (void)hipFree(f->mem);
+    delete f;
+}
+
+int qasr_paged_fork_get_info(const qasr_paged_fork_ws* f, qasr_paged_fork_info* out) {
+    if (!f || !out) return fail(QASR_EINVAL, "null argument");
+    out->max_requests = f->max_requests;
+    out->max_pages = f->max_pages;
+    out->status_dev = f->status;
+    out->bytes = f->bytes;
+    return QASR_OK;
+}
+
+int qasr_paged_fork(qasr_ctx* ctx, qasr_paged_fork_ws* fork, int nreq, int32_t* len_dev, const int32_t* parent_dev,
+                    int32_t* table_dev, int table_stride, int32_t* shared_dev, int32_t* ring_dev, int32_t* cursor_dev,
+                    void* stream) {
+    if (!ctx || !fork) return fail(QASR_EINVAL, "null context or fork");
+    if (fork->ctx != ctx) return fail(QASR_EINVAL, "fork belongs to another context");
+    if (nreq < 1) return fail(QASR_EINVAL, "nreq must be > 0");
+    if (nreq > fork->max_requests)
+        return fail(QASR_ERANGE, "%d requests, the fork holds %d", nreq, fork->max_requests);
+    if (table_stride < 1) return fail(QASR_EINVAL, "table_stride must be > 0");
+    if (table_stride > fork->max_pages)
+        return fail(QASR_ERANGE, "tables of %d pages, the fork holds %d", table_stride, fork->max_pages);
+    if (!len_dev || !parent_dev || !table_dev || !shared_dev || !ring_dev || !cursor_dev)
+        return fail(QASR_EINVAL, "null device pointer");
+    if (((uintptr_t)len_dev | (uintptr_t)parent_dev | (uintptr_t)table_dev | (uintptr_t)shared_dev | (uintptr_t)ring_dev |
+         (uintptr_t)cursor_dev) & 3)
+        return fail(QASR_EINVAL, "an array of 32-bit numbers is not 4-byte aligned");
+    const qasr_pages* pool = fork->pool;
+    const Range arrays[] = {{(uintptr_t)len_dev, (int64_t)nreq * 4},
+                            {(uintptr_t)parent_dev, (int64_t)nreq * 4},
+                            {(uintptr_t)table_dev, (int64_t)nreq * table_stride * 4},
+                            {(uintptr_t)shared_dev, (int64_t)pool->pages * 4},
+                            {(uintptr_t)ring_dev, (int64_t)pool->pages * 4},
+                            {(uintptr_t)cursor_dev, 8},
+                            {(uintptr_t)fork->mem, (int64_t)fork->bytes}};
+    for (const Range& x : arrays)
+        for (const Range& y : arrays)
+            if (&x != &y && x.meets(y)) return fail(QASR_EINVAL, "two arrays overlap, or one lies in the fork's own");
+    DeviceScope ds(ctx->device);
+    if (ds.err != hipSuccess) return hip_fail(ds.err, "hipSetDevice");
+    const qasr::CacheGeom g = page_geom(pool);
+    const ScaleGeom s = scale_geom(pool);
+    qasr::ForkArgs a;
+    a.len = len_dev;
+    a.parent = parent_dev;
+    a.table = table_dev;
+    a.shared = shared_dev;
+    a.ring = ring_dev;
+    a.cursor = cursor_dev;
+    a.nreq = nreq;
+    a.stride = table_stride;
+    a.pages = pool->pages;
+    a.page_shift = pool->shift;
+    a.status = fork->status;
+    a.w = fork->head;
+    a.rows = fork->rows;
+    a.copies = fork->copies;
+    a.gone = fork->gone;
+    a.n_gone = fork->n_gone;
+    a.base = pool->base;
+    a.layer_bytes = g.layer_stride * pool->elem;
+    a.page_bytes = g.slot_stride * pool->elem;
+    a.row_bytes = qasr::kHeadDim * pool->elem;
+    a.layers = ctx->cfg.num_hidden_layers;
+    a.heads = 2 * g.nkvh;
+    a.scales = pool->scales;
+    a.layer_scales = (int64_t)s.page * pool->pages;
+    a.page_scales = s.page;
+    const hipError_t e = qasr::launch_paged_fork(a, ctx->cus, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "paged fork launch");
     return QASR_OK;
 }
 

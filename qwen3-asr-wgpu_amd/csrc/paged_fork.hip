@@ -1,0 +1,287 @@
+// paged_fork.hip -- the requests of a step go on as their parents do: what
+// beams need after a selection, and whoever samples one prompt several times.
+//
+// Request i takes its parent's length and pages.  A full page is held by as many
+// requests as go on from its holder, one more or fewer in `shared` for each; a
+// page that none holds any more goes back to the ring.  An unfinished last page
+// will be written: one of those that go on from its holder (itself, else the
+// first) keeps it, if no request outside holds it too, the others get copies of
+// its rows on fresh pages.
+//
+// Two launches.  The first, a workgroup with a request a thread, finds who goes
+// on from whom, ranks the copies (their fresh pages are the ring's next ones, in
+// request order) and decides whether the call is carried out at all.  In the
+// second, one part of the workgroups copies rows of K and V of all layers, 16
+// bytes a thread, the other part rewrites the table, 16 columns each: a page
+// lies at the same place in all tables that list it, so a workgroup meets every
+// holder that the call has of its pages, and rows of the table can be replaced
+// by others of the same columns in place.  Counts change by atomics, whose
+// order leaves no trace: exactly the last holder finds the count below zero, and
+// the pages given back are put in the order of their columns, then of the first
+// request that listed them, before the last workgroup to arrive moves them to
+// the ring.
+//
+// Bound by the copies' bytes where there are many, by the two launches and some
+// dependent loads (parent, table, count, ring) where there are few.
+#include "paged_fork.hpp"
+
+namespace qasr {
+
+namespace {
+
+constexpr int kThreads = 256;
+enum : int32_t { kOk = 0, kInvalid = 1, kNoPage = 3 };  // QASR_OK, _EINVAL, _ENOMEM
+
+__device__ __forceinline__ int wrap(int x, int pages) { return x >= pages ? x - pages : x; }
+
+// One workgroup, a request a thread.
+__global__ __launch_bounds__(kPagedMaxRequests) void fork_rows_kernel(ForkArgs a) {
+    __shared__ int s_len[kPagedMaxRequests], s_last[kPagedMaxRequests];  // unfinished page: its id, -1: none
+    __shared__ int s_sons[kPagedMaxRequests], s_heir[kPagedMaxRequests];
+    __shared__ int s_wave[kPagedMaxRequests / 64];
+    __shared__ uint8_t s_alone[kPagedMaxRequests];
+
+    const int i = threadIdx.x, lane = i & 63, ps = 1 << a.page_shift;
+    const bool mine = i < a.nreq;
+    int parent = -1, len = 0, head = 0, free = 0;
+    if (mine) {
+        parent = a.parent[i];
+        len = a.len[i];
+    }
+    head = a.cursor[0];
+    free = a.cursor[1];
+    if (head < 0 || head >= a.pages || free < 0 || free > a.pages) head = free = 0;
+    const bool bad = mine && (parent < -1 || parent >= a.nreq || len < 0 ||
+                              ((int64_t)len + ps - 1) >> a.page_shift > a.stride);
+    const bool refused = __syncthreads_or(bad);
+    if (refused) {  // nothing is done
+        if (mine) a.status[i] = bad ? kInvalid : kOk;
+        if (i == 0) a.w->ok = 0;
+        return;
+    }
+    const int whole = len >> a.page_shift, rest = len & (ps - 1);
+    s_sons[i] = 0;
+    s_heir[i] = kPagedMaxRequests;
+    int last = mine && rest ? a.table[(int64_t)i * a.stride + whole] : -1;
+    last = (uint32_t)last < (uint32_t)a.pages ? last : -1;
+    s_len[i] = len;
+    s_last[i] = last;
+    const bool alone = last >= 0 && a.shared[last] <= 0;
+    s_alone[i] = alone;
+    __syncthreads();
+    if (parent >= 0) {
+        atomicAdd(&s_sons[parent], 1);
+        atomicMin(&s_heir[parent], parent == i ? -1 : i);
+    }
+    __syncthreads();
+    bool copy = false;
+    if (parent >= 0 && s_last[parent] >= 0) {
+        const int heir = s_heir[parent] < 0 ? parent : s_heir[parent];
+        copy = !(heir == i && s_alone[parent]);
+    }
+    // Copies of the requests before this one.
+    const uint64_t votes = __ballot(copy);
+    if (lane == 0) s_wave[i >> 6] = __popcll(votes);
+    __syncthreads();
+    int rank = __popcll(votes & ((1ull << lane) - 1)), copies = 0;
+    for (int w = 0; w < kPagedMaxRequests / 64; ++w) {
+        rank += w < i >> 6 ? s_wave[w] : 0;
+        copies += s_wave[w];
+    }
+    const bool ok = copies <= free;
+    if (mine) {
+        a.status[i] = !ok && copy ? kNoPage : kOk;
+        ForkRow r;
+        r.parent = parent;
+        r.used = (len + ps - 1) >> a.page_shift;
+        r.whole = whole;
+        r.more = s_sons[i] - 1;
+        r.more_last = (s_sons[i] > 0 && alone ? 1 : 0) - 1;
+        r.copy = copy;
+        r.fresh = copy && ok ? a.ring[wrap(head + rank, a.pages)] : -1;
+        r.unused = 0;
+        a.rows[i] = r;
+        if (copy && ok) {
+            const bool there = (uint32_t)r.fresh < (uint32_t)a.pages;
+            a.copies[rank] = {s_last[parent], there ? r.fresh : 0, there ? s_len[parent] & (ps - 1) : 0, 0};
+        }
+        if (ok) a.len[i] = parent >= 0 ? s_len[parent] : 0;  // (every length was read)
+    }
+    if (i == 0) {
+        a.w->ok = ok;
+        a.w->copies = copies;
+        a.w->head = head;
+        a.w->free = free;
+    }
+}
+
+// Rows of K and V, 16 bytes a thread: unit (copy, part of 1024 of them).
+constexpr int kCopyVectors = 1024;
+__device__ __forceinline__ void copy_pages(const ForkArgs& a, int first, int step, int parts) {
+    const int units = a.w->copies * parts;
+    for (int u = first; u < units; u += step) {
+        const int c = u / parts, part = u - c * parts;
+        const ForkCopy p = a.copies[c];
+        const int n = p.rows * (a.row_bytes / 16);  // vectors of a head
+        const int64_t head_bytes = (int64_t)a.row_bytes << a.page_shift;
+        const int all = n * a.heads * a.layers;
+        uint4 x[kCopyVectors / kThreads];
+        int64_t to[kCopyVectors / kThreads];
+#pragma unroll
+        for (int k = 0; k < kCopyVectors / kThreads; ++k) {
+            const int v = part * kCopyVectors + k * kThreads + (int)threadIdx.x;
+            to[k] = -1;
+            if (v < all) {
+                const int h = v / n, at = v - h * n, layer = h / a.heads, head = h - layer * a.heads;
+                const int64_t in = layer * a.layer_bytes + head * head_bytes + at * 16ll;
+                x[k] = *(const uint4*)(a.base + in + p.from * a.page_bytes);
+                to[k] = in + p.to * a.page_bytes;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kCopyVectors / kThreads; ++k)
+            if (to[k] >= 0) *(uint4*)(a.base + to[k]) = x[k];
+        if (part == 0 && a.scales && p.rows) {  // units of the copied rows' blocks
+            const int blocks = (1 << a.page_shift) / kPagedScaleRows, held = (p.rows + kPagedScaleRows - 1) / kPagedScaleRows;
+            for (int s = threadIdx.x; s < a.layers * a.page_scales; s += kThreads) {
+                const int layer = s / a.page_scales, at = s - layer * a.page_scales;
+                if (at % blocks < held) {
+                    uint8_t* q = a.scales + layer * a.layer_scales + at;
+                    q[p.to * (int64_t)a.page_scales] = q[p.from * (int64_t)a.page_scales];
+                }
+            }
+        }
+    }
+}
+
+// kForkColumns columns of the table.
+__device__ __forceinline__ void rewrite_columns(const ForkArgs& a, int block, int blocks, int* s_page) {
+    // s_page: [nreq][kForkColumns] pages listed now, -1: none that counts.
+    constexpr int C = kForkColumns, kWords = kPagedMaxRequests / 32;
+    __shared__ uint32_t s_gone[C][kWords];  // requests whose page of the column nobody holds any more
+    __shared__ uint32_t s_many[C][kWords];  // whose page's count changes
+    __shared__ int s_first[C + 1];
+    __shared__ int s_arrived;
+    const int tid = threadIdx.x, n = a.nreq * C, k0 = block * C;
+    for (int x = tid; x < C * kWords; x += kThreads) s_gone[x / kWords][x % kWords] = s_many[x / kWords][x % kWords] = 0;
+    for (int x = tid; x < n; x += kThreads) {
+        const int j = x / C, k = k0 + x % C;
+        int page = -1;
+        if (k < a.rows[j].used) page = a.table[(int64_t)j * a.stride + k];
+        s_page[x] = page;
+    }
+    __syncthreads();
+    // Holders.  Whose page has no other loses its last one; counts of pages with
+    // several, and of those that get more, change behind the barrier.
+    auto more_of = [&](int x) {
+        if ((uint32_t)s_page[x] >= (uint32_t)a.pages) return 0;
+        const ForkRow& r = a.rows[x / C];
+        return k0 + x % C < r.whole ? r.more : r.more_last;
+    };
+    auto set = [&](uint32_t (*bits)[kWords], int j, int c) { atomicOr(&bits[c][j >> 5], 1u << (j & 31)); };
+    for (int x = tid; x < n; x += kThreads) {
+        const int more = more_of(x);
+        if (more < 0 && a.shared[s_page[x]] <= 0)
+            set(s_gone, x / C, x % C);
+        else if (more)
+            set(s_many, x / C, x % C);
+    }
+    __syncthreads();
+    for (int x = tid; x < n; x += kThreads) {
+        if (!(s_many[x % C][x / C >> 5] >> (x / C & 31) & 1)) continue;
+        const int more = more_of(x);
+        int* count = a.shared + s_page[x];
+        const int was = __hip_atomic_fetch_add(count, more, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (more < 0 && was == 0) {  // the last holder
+            __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            int j = x % C;  // the first request that lists it
+            while (j < x && s_page[j] != s_page[x]) j += C;
+            set(s_gone, j / C, x % C);
+        }
+    }
+    __syncthreads();
+    // Their pages by column, then by request.
+    if (tid < C) {
+        int sum = 0;
+        for (int w = 0; w < kWords; ++w) sum += __popc(s_gone[tid][w]);
+        s_first[tid + 1] = sum;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        s_first[0] = 0;
+        for (int c = 0; c < C; ++c) s_first[c + 1] += s_first[c];
+    }
+    __syncthreads();
+    int* gone = a.gone + (int64_t)block * a.nreq * C;
+    for (int x = tid; x < n; x += kThreads) {
+        const int j = x / C, c = x % C;
+        if (!(s_gone[c][j >> 5] >> (j & 31) & 1)) continue;
+        int at = s_first[c] + __popc(s_gone[c][j >> 5] & ((1u << (j & 31)) - 1));
+        for (int w = 0; w < j >> 5; ++w) at += __popc(s_gone[c][w]);
+        __hip_atomic_store(gone + at, s_page[x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (tid == 0)
+        __hip_atomic_store(a.n_gone + block, s_first[C], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // New rows of the table.
+    for (int x = tid; x < n; x += kThreads) {
+        const ForkRow r = a.rows[x / C];
+        if (r.parent < 0 || (r.parent == x / C && !r.copy)) continue;
+        const ForkRow& p = a.rows[r.parent];
+        const int k = k0 + x % C;
+        if (k >= p.used) continue;
+        a.table[(int64_t)(x / C) * a.stride + k] = r.copy && k == p.whole ? r.fresh : s_page[r.parent * C + x % C];
+    }
+    // The last workgroup moves all that is gone to the ring's end.
+    stores_done_barrier();
+    if (tid == 0) s_arrived = ticket_add(&a.w->arrived) == (uint32_t)(blocks - 1);
+    __syncthreads();
+    if (!s_arrived) return;
+    const int head = a.w->head, free = a.w->free, copies = a.w->copies;
+    int pushed = 0;
+    for (int b0 = 0; b0 < blocks; b0 += kThreads) {  // (one turn for tables of up to 4096 pages)
+        const int m = b0 + tid < blocks ? __hip_atomic_load(a.n_gone + b0 + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+        __syncthreads();
+        s_page[tid] = m;
+        __syncthreads();
+        for (int b = 0; b < min(kThreads, blocks - b0); ++b) {
+            const int* from = a.gone + (int64_t)(b0 + b) * a.nreq * C;
+            for (int x = tid; x < s_page[b] && free + pushed + x < a.pages; x += kThreads)  // (a page given back twice)
+                a.ring[wrap(head + free + pushed + x, a.pages)] =
+                    __hip_atomic_load(from + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            pushed += s_page[b];
+        }
+    }
+    if (tid == 0) {
+        a.cursor[0] = wrap(head + copies, a.pages);
+        a.cursor[1] = min(free + pushed, a.pages) - copies;
+        ticket_reset(&a.w->arrived);
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void fork_pages_kernel(ForkArgs a, int blocks, int parts) {
+    extern __shared__ int s_page[];
+    if (!a.w->ok) return;
+    if ((int)blockIdx.x < blocks)
+        rewrite_columns(a, blockIdx.x, blocks, s_page);
+    else
+        copy_pages(a, blockIdx.x - blocks, gridDim.x - blocks, parts);
+}
+
+}  // namespace
+
+hipError_t launch_paged_fork(const ForkArgs& a, int cus, hipStream_t stream) {
+    if (a.nreq < 1 || a.nreq > kPagedMaxRequests || a.stride < 1) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(fork_rows_kernel, dim3(1), dim3(kPagedMaxRequests), 0, stream, a);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const int blocks = (a.stride + kForkColumns - 1) / kForkColumns;
+    const int64_t most = (int64_t)((1 << a.page_shift) - 1) * (a.row_bytes / 16) * a.heads * a.layers;  // vectors of a copy
+    const int parts = (int)((most + kCopyVectors - 1) / kCopyVectors);
+    const int64_t units = (int64_t)parts * a.nreq;
+    const int64_t copiers = units < 8 * cus ? units : 8 * cus;
+    hipLaunchKernelGGL(fork_pages_kernel, dim3((unsigned)(blocks + copiers)), dim3(kThreads),
+                       (size_t)(a.nreq > kThreads / kForkColumns ? a.nreq : kThreads / kForkColumns) * kForkColumns * 4, stream, a, blocks, parts);
+    return hipGetLastError();
+}
+
+}  // namespace qasr

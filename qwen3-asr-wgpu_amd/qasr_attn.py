@@ -43,6 +43,8 @@ ABI_SYMBOLS = (
     "qasr_paged_plan_destroy", "qasr_paged_plan_get_info", "qasr_paged_plan_build",
     "qasr_paged_append", "qasr_paged_attn", "qasr_plan_paged",
     "qasr_pages_create_e4m3", "qasr_pages_get_scales",
+    "qasr_paged_fork_create", "qasr_paged_fork_destroy", "qasr_paged_fork_get_info", "qasr_paged_fork",
+    "qasr_beam_create", "qasr_beam_destroy", "qasr_beam_select",
 )
 MAX_PREFILL_SEGMENTS = 64  # segments per qasr_decoder_prefill_batch call
 
@@ -134,6 +136,11 @@ class PagedPlanInfo(ctypes.Structure):
     ] + [("bytes", ctypes.c_size_t)]
 
 
+class PagedForkInfo(ctypes.Structure):
+    _fields_ = [("max_requests", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+                ("status_dev", ctypes.c_void_p), ("bytes", ctypes.c_size_t)]
+
+
 _lib = None
 _vp = ctypes.c_void_p
 _i32p = ctypes.POINTER(ctypes.c_int32)
@@ -212,6 +219,18 @@ def load(path: str = LIB_PATH):
     L.qasr_paged_attn.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, _vp, ctypes.c_int, _vp,
                                   _vp, _vp]
     L.qasr_plan_paged.argtypes = [ctypes.c_int, ctypes.c_int, i32p, i32p, i32p]
+    L.qasr_paged_fork_create.argtypes = [_vp, _vp, ctypes.c_int, ctypes.c_int, ctypes.POINTER(_vp)]
+    L.qasr_paged_fork_destroy.argtypes = [_vp]
+    L.qasr_paged_fork_destroy.restype = None
+    L.qasr_paged_fork_get_info.argtypes = [_vp, ctypes.POINTER(PagedForkInfo)]
+    L.qasr_paged_fork.argtypes = [_vp, _vp, ctypes.c_int, _vp, _vp, _vp, ctypes.c_int, _vp, _vp, _vp,
+                                  _vp]
+    L.qasr_beam_create.argtypes = [_vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
+                                   ctypes.POINTER(_vp)]
+    L.qasr_beam_destroy.argtypes = [_vp]
+    L.qasr_beam_destroy.restype = None
+    L.qasr_beam_select.argtypes = [_vp, _vp, ctypes.c_int, _vp, ctypes.c_int64, _vp, _vp, ctypes.c_int,
+                                   _vp, _vp, _vp, _vp, _vp]
     _lib = L
     return L
 
@@ -553,6 +572,13 @@ class PagePool:
         return (torch.arange(self.pages, dtype=torch.int32, device=dev),
                 torch.tensor([0, self.pages], dtype=torch.int32, device=dev))
 
+    def share_counts(self):
+        """How many requests beyond the first hold each page, for `paged_fork`:
+        none yet; an int32 CUDA tensor [pages]."""
+        import torch
+
+        return torch.zeros(self.pages, dtype=torch.int32, device=f"cuda:{self.ctx.device}")
+
     def close(self):
         """Free the pages now; their views must not be used any more, calls of
         the pool's plans are refused."""
@@ -721,6 +747,141 @@ def paged_attn(ctx: Context, plan: PagedPlan, layer: int, table, q, out, stream=
     _check(load().qasr_paged_attn(
         ctx.handle, plan.handle, layer, rows, _on(ctx, table, "table", torch.int32), stride,
         _on(ctx, q, "q", f16), _on(ctx, out, "out", f16), _ctx_stream(ctx, stream)))
+
+
+class _ForkMemory:
+    """A qasr_paged_fork_ws and what it needs alive, as _PlanMemory."""
+
+    def __init__(self, ctx: Context, pool: PagePool, max_requests: int, max_pages: int):
+        self.keep = (ctx, pool)
+        self.handle = None
+        h = _vp()
+        _check(load().qasr_paged_fork_create(ctx.handle, pool.handle, max_requests, max_pages,
+                                             ctypes.byref(h)))
+        self.handle = h
+
+    def close(self):
+        if self.handle:
+            load().qasr_paged_fork_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class PagedFork:
+    """Workspace of forks (qasr_paged_fork_ws) of up to max_requests requests
+    with tables of up to max_pages pages, and `status` [max_requests], int32."""
+
+    def __init__(self, ctx: Context, pool: PagePool, max_requests: int, max_pages: int):
+        import torch
+
+        self.ctx, self.pool = ctx, pool
+        self.max_requests, self.max_pages = max_requests, max_pages
+        self._mem = _ForkMemory(ctx, pool, max_requests, max_pages)
+        inf = PagedForkInfo()
+        _check(load().qasr_paged_fork_get_info(self.handle, ctypes.byref(inf)))
+        self.bytes = inf.bytes
+        v = _DeviceView(inf.status_dev, 4 * max_requests, ctx.device, "<i4", self._mem)
+        self.status = torch.as_tensor(v, device=f"cuda:{ctx.device}")
+
+    @property
+    def handle(self):
+        """None once the fork or its pool is closed: calls on it are refused."""
+        return self._mem.handle if self.pool.handle else None
+
+    def close(self):
+        """Free the workspace now; `status` must not be used any more."""
+        self._mem.close()
+
+
+def paged_fork(ctx: Context, fork: PagedFork, lens, parent, table, shared, ring, cursor, stream=None):
+    """Requests go on as others (qasr_paged_fork): request i of len(parent) as
+    request parent[i] is, or is released (-1).  lens, table [requests][pages of a
+    request], shared [pages] (PagePool.share_counts), ring and cursor change in
+    place; all int32 CUDA tensors.  `lens` may be plan.lens and `cursor`
+    plan.cursor.  `fork.status` says whether it was carried out."""
+    import torch
+
+    i32 = torch.int32
+    n = int(parent.numel())
+    _need(lens, n, "lens")
+    stride = _table(table, n)
+    _need(shared, fork.pool.pages, "shared", exact=True)
+    _need(ring, fork.pool.pages, "ring", exact=True)
+    _need(cursor, 2, "cursor", exact=True)
+    _check(load().qasr_paged_fork(
+        ctx.handle, fork.handle, n, _on(ctx, lens, "lens", i32), _on(ctx, parent, "parent", i32),
+        _on(ctx, table, "table", i32), stride, _on(ctx, shared, "shared", i32),
+        _on(ctx, ring, "ring", i32), _on(ctx, cursor, "cursor", i32), _ctx_stream(ctx, stream)))
+
+
+# ---- beam selection -------------------------------------------------------
+
+class BeamSelect:
+    """Workspace of beam selections (qasr_beam): up to max_groups groups of
+    `width` beams over `vocab` tokens, k candidates a group."""
+
+    def __init__(self, ctx: Context, max_groups: int, width: int, vocab: int, k: Optional[int] = None):
+        self.ctx = ctx
+        self.handle = None
+        self.max_groups, self.width, self.vocab = max_groups, width, vocab
+        self.k = width if k is None else k
+        h = _vp()
+        _check(load().qasr_beam_create(ctx.handle, max_groups, width, vocab, self.k, ctypes.byref(h)))
+        self.handle = h
+
+    def close(self):
+        if self.handle:
+            load().qasr_beam_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def beam_select(ctx: Context, sel: BeamSelect, logits, scores, parent, token, out_scores, done=None,
+                eos: int = -1, out_done=None, stream=None):
+    """The k best continuations of each group of beams (qasr_beam_select).
+    logits [groups * width][vocab] f32 (rows may lie further apart), scores
+    [groups * width] f32, done the same in int32 or None; parent, token (int32),
+    out_scores (f32) and out_done (int32 or None) [groups * k].  out_scores may be
+    `scores` and out_done `done` if k is width."""
+    import torch
+
+    i32, f32 = torch.int32, torch.float32
+    if logits.dim() != 2 or logits.shape[1] != sel.vocab:
+        raise QasrError(QASR_EINVAL, f"logits must be [rows][{sel.vocab}], got {list(logits.shape)}")
+    rows = int(logits.shape[0])
+    groups = rows // sel.width
+    if rows == 0 or groups * sel.width != rows:
+        raise QasrError(QASR_EINVAL, f"{rows} rows of logits for groups of {sel.width} beams")
+    if logits.shape[1] > 1 and logits.stride(1) != 1:
+        raise ValueError("the logits of a row must be contiguous")
+    stride = int(logits.stride(0)) if rows > 1 else sel.vocab
+    if stride < sel.vocab:
+        raise QasrError(QASR_EINVAL, f"rows of {sel.vocab} logits are {stride} apart")
+    _need(scores, rows, "scores")
+    _need(parent, groups * sel.k, "parent")
+    _need(token, groups * sel.k, "token")
+    _need(out_scores, groups * sel.k, "out_scores")
+    if done is not None:
+        _need(done, rows, "done")
+    if out_done is not None:
+        _need(out_done, groups * sel.k, "out_done")
+    if logits.dtype is not f32 or logits.get_device() != ctx.device:
+        _on(ctx, logits[0], "logits", f32)
+    _check(load().qasr_beam_select(
+        ctx.handle, sel.handle, groups, logits.data_ptr(), stride, _on(ctx, scores, "scores", f32),
+        _on(ctx, done, "done", i32) if done is not None else None, eos, _on(ctx, parent, "parent", i32),
+        _on(ctx, token, "token", i32), _on(ctx, out_scores, "out_scores", f32),
+        _on(ctx, out_done, "out_done", i32) if out_done is not None else None, _ctx_stream(ctx, stream)))
 
 
 class AttnBackend:
