@@ -438,8 +438,7 @@ void qasr_beam_destroy(qasr_beam* beam);
  * parent and token -1, score -inf, done 0.  Rows that have no logits to offer
  * are not read.
  *
- * Sums are formed in f32 over pieces of 4096 tokens and more, everything behind
- * them in f64; scores are compared in f64 and rounded once.  A group's results
+ * Sums are formed in f32 over pieces of 2048 tokens, everything behind them in f64; scores are compared in f64 and rounded once.  A group's results
  * are a function of its own rows.  Outputs may be the inputs' arrays (out_scores
  * scores, out_done done) if k is width; they overlap nothing else.  Does not
  * allocate or synchronise, may be captured; calls that share the workspace are

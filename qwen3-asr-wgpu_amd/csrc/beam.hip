@@ -5,43 +5,48 @@
 // ended beam has one, (b, eos) with s_b.  The k best of a group, ties to the
 // lower beam, then to the lower token.
 //
-// One pass over the logits.  A workgroup holds a piece of a row in registers
-// (512 threads of 8 values, two 16-byte loads each): its maximum, the sum of
-// exponentials against it, and its k best.  For these every wave finds the k-th
-// largest of its 64 lanes' maxima, by bisection of the keys' bits with ballots;
-// at least k values of the row are as large as the largest of the waves' finds,
-// so only those that are, mostly little more than k, go to LDS and are ranked
-// there by comparing each with all.  A key is the logit's order-preserving bits
-// over the complement of its token, unique, so that ties cost nothing and the
-// list is never longer than waves * k * values.
+// One pass over the logits.  A wave holds a tile of 2048 of a row's in registers:
+// their maximum, the sum of exponentials against it (published, a pair a tile),
+// and what of them is among the wave's k best so far.  A tile whose largest is
+// below the k-th best has nothing; else the k-th largest of the lanes' maxima,
+// found by bisection with ballots, is a border that at least k values reach, and
+// the few that reach both go to the wave's list in LDS, which is ranked by
+// comparing each with all and cut to k.  A key is the logit's order-preserving
+// bits over the complement of its token, unique, so ties cost nothing and no
+// list can be longer than k + k * 32.  A workgroup's four lists merge at its end.
+// Tiles and sums are the same whatever the number of workgroups a row has, which
+// follows the number of rows.
 //
-// The last workgroup of a group to arrive (ticket) merges: a wave a beam takes
-// the pieces' sums, in 64 bits and in order, and out of its sorted pieces' lists
-// the k best in the same way, by the k-th largest of the lists' heads; then each
-// of the beams' sorted candidates finds its rank by a bisection in the other
-// beams' lists, in 64-bit scores.  Everything is a function of the row alone up
-// to there: results do not depend on the batch, or on who comes last.
-//
-// Bound by the logits' bytes for many rows, by launch, one load, the ballots and
-// the merge's two round trips for few.
+// The last workgroup of a group to arrive (ticket) merges: a wave a beam adds up
+// the tiles' sums, in order and in 64 bits, and takes the k best of the
+// workgroups' lists in the same way as of a tile; then each of the beams'
+// candidates finds its rank by bisection in the other beams' lists, in 64-bit
+// scores.  Results are a function of the group's rows alone.
 #include "beam.hpp"
 
 namespace qasr {
 
 namespace {
 
-constexpr int kWaves = kBeamThreads / 64;
+constexpr int kThreads = kBeamWaves * 64;
+// A lane's logits of a tile; a vector, as a choice between elements of an array
+// is one between addresses and puts it into memory.
+typedef float Tile __attribute__((ext_vector_type(kBeamValues)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNone = -__builtin_inff();
 
-__device__ __forceinline__ uint64_t key_of(float x, int token) {
+__device__ __forceinline__ uint32_t order_of(float x) {
     const uint32_t u = __float_as_uint(x);
-    const uint32_t o = u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u);
-    return (uint64_t)o << 32 | ~(uint32_t)token;
+    return u ^ ((int32_t)u < 0 ? 0xffffffffu : 0x80000000u);
 }
+__device__ __forceinline__ uint64_t key_of(float x, int token) { return (uint64_t)order_of(x) << 32 | ~(uint32_t)token; }
 __device__ __forceinline__ float logit_of(uint64_t key) {
     const uint32_t o = (uint32_t)(key >> 32);
     return __uint_as_float(o ^ ((int32_t)o < 0 ? 0x80000000u : 0xffffffffu));
+}
+// The least finite value whose ordered bits reach `border`.
+__device__ __forceinline__ float value_of(uint32_t border) {
+    return logit_of((uint64_t)max(border, order_of(-3.4028234663852886e38f)) << 32);
 }
 __device__ __forceinline__ int token_of(uint64_t key) { return (int)~(uint32_t)key; }
 
@@ -51,265 +56,326 @@ __device__ __forceinline__ void store_dev64(uint64_t* p, uint64_t v) {
 __device__ __forceinline__ uint64_t load_dev64(const uint64_t* p) {
     return __hip_atomic_load(const_cast<uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// A scalar load of what no workgroup writes before all have read it.
+template <class T>
+__device__ __forceinline__ T scalar(const T* p) {
+    return *(const __attribute__((address_space(4))) T*)p;
+}
 
-// The k-th largest of the lanes' keys, or 0 if fewer than k are not 0.
-__device__ __forceinline__ uint64_t kth_of_lanes(uint64_t key, int k) {
-    uint64_t t = 0;
-    for (int b = 63; b >= 0; --b) {
-        const uint64_t cand = t | 1ull << b;
-        const int n = __popcll(__ballot(key >= cand));
-        if (n >= k) {
-            t = cand;
-            if (n == k) break;  // as good a border as the k-th itself
+__device__ __forceinline__ float wave_max(float x) {
+    x = fmaxf(x, dpp<kDppXor1>(x));
+    x = fmaxf(x, dpp<kDppXor2>(x));
+    x = fmaxf(x, dpp<kDppHalfMirror>(x));
+    x = fmaxf(x, dpp<kDppMirror>(x));
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float wave_sum(float x) {
+    x = row_sum16(x);
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The largest of some borders that at least k of the lanes' values reach, by
+// their ordered bits, of which `top` are the largest; 0 if fewer than k are not 0.
+// Exactly k reach it but where several are equal to the k-th.
+__device__ __forceinline__ uint32_t border_of(uint32_t mine, uint32_t top, int k) {
+    uint32_t lo = 0, hi = top + 1;  // at least k reach lo, fewer hi (none has all bits set)
+    int n = __popcll(__ballot(mine != 0));
+    if (n < k) return 0;
+    // (The k-th is mostly near: from further below the top each time.)
+    for (uint32_t d = 1u << 20; d != 0 && d < top; d <<= 2) {  // 2^20 .. 2^30, then 0
+        const int m = __popcll(__ballot(mine >= top - d));
+        if (m >= k) {
+            lo = top - d;
+            n = m;
+            break;
         }
     }
-    return t;
+    while (n != k && hi - lo > 1) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        const int m = __popcll(__ballot(mine >= mid));
+        if (m >= k) {
+            lo = mid;
+            n = m;
+        } else {
+            hi = mid;
+        }
+    }
+    return max(lo, 1u);
 }
 
 // A beam that offers nothing: its score is -inf, +inf or NaN.
 __device__ __forceinline__ bool dead(float score) { return !(fabsf(score) < __builtin_inff()); }
 
-struct Shared {
-    uint64_t border[kWaves];
-    float top[kWaves];
-    float sum[kWaves];
-    int count[kWaves];
-    int last;
-    int offers[kBeamMaxWidth];
-};
-// And by the call's sizes: a list, of what reaches the border in a piece or, a
-// part for each wave, in the pieces' lists; the beams' candidates, best first.
-__host__ __device__ constexpr int list_entries(int values, int k) { return kWaves * k * (values > k ? values : k); }
-struct Lists {
-    uint64_t* list;
-    double* score;
-    int* token;
-};
-
-// LDS writes of this wave before its reads behind.
+// LDS accesses of this wave in order.
 __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
+__device__ __forceinline__ uint64_t lane_key(uint64_t key, int lane) {
+    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)key, lane);
+}
 
-__device__ __forceinline__ void merge(const BeamArgs& a, int group, int splits, Shared& sh, const Lists& ls) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.k;
-    uint64_t* list = ls.list + wave * k * k;
-    for (int b = wave; b < a.width; b += kWaves) {
+// A wave's k best keys so far, best first, a lane each.
+struct Best {
+    uint64_t key = 0;  // lane i < held: the i-th
+    uint64_t kth = 0;  // 0 while there are fewer
+    int held = 0;
+};
+// Takes a key of each lane (0: none) among them.  Those that are better than the
+// k-th come to all lanes one by one, and each lane counts what comes before its
+// own: few, as callers leave out what cannot be among the k best.
+__device__ __forceinline__ void take(Best& b, uint64_t key, int k, int lane, uint64_t* slot) {
+    key = key > b.kth ? key : 0;
+    const uint64_t todo = __ballot(key != 0);
+    if (todo == 0) return;
+    int rank = 0, held_rank = lane;
+    for (uint64_t t = todo; t; t &= t - 1) {
+        const int l = __builtin_ctzll(t);
+        const uint64_t x = lane_key(key, l);
+        const int before = __popcll(__ballot(b.key > x));
+        rank += (x > key) + (lane == l ? before : 0);
+        held_rank += x > b.key;
+    }
+    if (key != 0 && rank < k) slot[rank] = key;
+    if (lane < b.held && held_rank < k) slot[held_rank] = b.key;
+    b.held = min(b.held + __popcll(todo), k);
+    wave_sync();
+    b.key = lane < b.held ? slot[lane] : 0;
+    wave_sync();
+    b.kth = b.held == k ? lane_key(b.key, k - 1) : 0;
+}
+
+// A tile's values, of which this lane's largest is `top`, the wave's M.  Token of
+// v[i]: first + 256 (i / 4) + i % 4.
+__device__ __forceinline__ void take_tile(Best& b, const Tile& v, float top, float M, int first, int k, int lane, uint64_t* slot) {
+    // At least k of the row reach the border, a value.
+    uint32_t border = max((uint32_t)(b.kth >> 32), 1u);
+    const uint32_t mine = top == kNone ? 0 : order_of(top + 0.0f);
+    if (__popcll(__ballot(mine >= border)) > k) border = max(border, border_of(mine, order_of(M + 0.0f), k));
+    const float least = value_of(border);
+    uint32_t mask = 0;
+#pragma unroll
+    for (int i = kBeamValues - 1; i >= 0; --i) mask = 2 * mask + (v[i] >= least);
+    while (__ballot(mask != 0)) {  // a value of each lane at a time, the lower token first
+        const int i = mask ? __builtin_ctz(mask) : 0;
+        Tile x = v;  // v[i]: a bit of i a step
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = i & 1 ? x[2 * j + 1] : x[2 * j];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = i & 2 ? x[2 * j + 1] : x[2 * j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = i & 4 ? x[2 * j + 1] : x[2 * j];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) x[j] = i & 8 ? x[2 * j + 1] : x[2 * j];
+        const float y = (i & 16 ? x[1] : x[0]) + 0.0f;  // -0 is 0
+        take(b, mask ? key_of(y, first + 256 * (i >> 2) + (i & 3)) : 0, k, lane, slot);
+        mask &= mask - 1;
+    }
+}
+
+struct Shared {
+    uint64_t slot[kBeamWaves][kBeamMaxK];
+    int last;
+    int offers[kBeamMaxWidth];
+};
+
+// Row sums and lists of the group's beams, a wave a beam; then the beams'
+// candidates against each other.  score, ended: of beam `lane`.
+constexpr int kBatch = 8;  // keys of a lane at a time
+typedef unsigned long long Keys __attribute__((ext_vector_type(kBatch)));
+__device__ __forceinline__ void merge(const BeamArgs& a, int group, int lists, float score, bool ended, Shared& sh,
+                                      double* s_score) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), k = a.k;
+    const int tiles = (a.vocab + kBeamTile - 1) / kBeamTile, n = a.width * k;
+    int* s_token = (int*)(s_score + n);
+    const uint64_t endeds = __ballot(ended);
+    for (int b = wave; b < a.width; b += kBeamWaves) {
         const int row = group * a.width + b;
-        const float score = a.scores[row];
-        const bool ended = a.done && a.done[row];
-        int offers = 0;
-        if (!dead(score) && ended) {
+        const float s_b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(score), b));
+        double mine = kNone;  // candidate `lane`
+        int token = a.eos, offers = 0;
+        if (!dead(s_b) && (endeds >> b & 1)) {
             offers = 1;
-            if (lane == 0) {
-                ls.score[b * k] = score;
-                ls.token[b * k] = a.eos;
+            mine = lane == 0 ? (double)s_b : mine;
+        } else if (!dead(s_b)) {
+            const uint64_t* keys = a.keys + (int64_t)row * (kBeamMaxParts * kBeamWaves) * k;
+            const uint64_t* sums = a.sums + (int64_t)row * tiles;
+            Best best;
+            Keys x;
+            auto load = [&](int i0) {
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    const int i = i0 + 64 * j + lane;
+                    x[j] = i < lists * k ? load_dev64(keys + i) : 0;
+                }
+            };
+            load(0);
+            float top = kNone;
+            bool broken = false;
+            double sum = 0.0;
+            for (int t0 = 0; t0 < tiles; t0 += 128) {  // (one turn for up to 262144 tokens)
+                float m[2], s[2];
+                const float before = top;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int t = t0 + 64 * i + lane;
+                    const uint64_t y = t < tiles ? load_dev64(sums + t) : (uint64_t)__float_as_uint(kNone);
+                    m[i] = __uint_as_float((uint32_t)y);
+                    s[i] = __uint_as_float((uint32_t)(y >> 32));
+                    broken |= s[i] != s[i];
+                    top = fmaxf(top, m[i]);
+                }
+                top = wave_max(top);
+                const float base = top == kNone ? 0.0f : top;
+                sum *= before == kNone ? 0.0f : fast_exp2((before - base) * kLog2e);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) sum += (double)(s[i] * fast_exp2((m[i] - base) * kLog2e));
             }
-        } else if (!dead(score)) {
-            const uint64_t* keys = a.keys + (int64_t)row * splits * k;
-            const float* sums = a.sums + (int64_t)row * splits * 2;
-            const bool on = lane < splits;
-            const uint64_t head = on ? load_dev64(keys + lane * k) : 0;
-            const uint64_t ms = on ? load_dev64((const uint64_t*)sums + lane) : 0;
-            const float m = on ? __uint_as_float((uint32_t)ms) : kNone, s = __uint_as_float((uint32_t)(ms >> 32));
-            const bool broken = __ballot(on && s != s);
-            float top = m;
-#pragma unroll
-            for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-            double sum = on && m != kNone ? (double)s * exp((double)m - (double)top) : 0.0;
-#pragma unroll
-            for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+            broken = __ballot(broken);
             if (!broken && top != kNone) {
+#pragma unroll
+                for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
                 const double lse = (double)top + log(sum);
-                const uint64_t border = kth_of_lanes(head, k);
-                // At most k lists have such heads.
-                if (lane == 0) sh.count[wave] = 0;
-                wave_sync();
-                for (int i = lane; i < splits * k; i += 64) {
-                    const uint64_t key = load_dev64(keys + i);
-                    if (key != 0 && key >= border) list[atomicAdd(&sh.count[wave], 1)] = key;
-                }
-                wave_sync();
-                const int n = sh.count[wave];
-                for (int i = lane; i < n; i += 64) {
-                    const uint64_t key = list[i];
-                    int rank = 0;
-                    for (int j = 0; j < n; ++j) rank += list[j] > key;
-                    if (rank < k) {
-                        ls.score[b * k + rank] = (double)score + ((double)logit_of(key) - lse);
-                        ls.token[b * k + rank] = token_of(key);
+                for (int i0 = 0;;) {  // (one turn for up to 512 keys)
+                    uint64_t most = 0;
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) most = max(most, (uint64_t)x[j]);
+                    const uint32_t border = border_of((uint32_t)(most >> 32), order_of(top + 0.0f), k);
+                    uint32_t mask = 0;
+#pragma unroll
+                    for (int j = kBatch - 1; j >= 0; --j) mask = 2 * mask + (x[j] != 0 && (uint32_t)(x[j] >> 32) >= border);
+                    while (__ballot(mask != 0)) {
+                        const int j = mask ? __builtin_ctz(mask) : 0;
+                        const uint64_t y0 = j & 1 ? x[1] : x[0], y1 = j & 1 ? x[3] : x[2], y2 = j & 1 ? x[5] : x[4], y3 = j & 1 ? x[7] : x[6];
+                        const uint64_t z0 = j & 2 ? y1 : y0, z1 = j & 2 ? y3 : y2;
+                        take(best, mask ? (j & 4 ? z1 : z0) : 0, k, lane, sh.slot[wave]);
+                        mask &= mask - 1;
                     }
+                    i0 += 64 * kBatch;
+                    if (i0 >= lists * k) break;
+                    load(i0);
                 }
-                offers = min(n, k);
+                offers = best.held;
+                if (lane < offers) {
+                    mine = (double)s_b + ((double)logit_of(best.key) - lse);
+                    token = token_of(best.key);
+                }
             }
+        }
+        if (lane < k) {
+            s_score[b * k + lane] = mine;
+            s_token[b * k + lane] = token;
         }
         if (lane == 0) sh.offers[b] = offers;
     }
     __syncthreads();
-    int all = 0;
-    for (int b = 0; b < a.width; ++b) all += sh.offers[b];
-    for (int i = tid; i < a.width * k; i += kBeamThreads) {
-        const int b = i / k, j = i - b * k;
-        if (j >= sh.offers[b]) continue;
-        const double score = ls.score[i];
-        int rank = j;  // and how many of the other beams' come before it
-        for (int c = 0; c < a.width && rank < k; ++c) {
-            if (c == b) continue;
-            int lo = 0, hi = sh.offers[c];
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                const double x = ls.score[c * k + mid];
-                if (x > score || (x == score && c < b))
-                    lo = mid + 1;
-                else
-                    hi = mid;
-            }
-            rank += lo;
+    // Each candidate's rank: how many come before it.
+    int total = 0;
+    for (int b = 0; b < a.width; ++b) total += sh.offers[b];
+    for (int i = tid; i < n; i += kThreads) {
+        const double x = s_score[i];
+        int rank = 0;
+#pragma unroll 8
+        for (int j = 0; j < n; ++j) {
+            const double y = s_score[j];
+            rank += y > x || (y == x && j < i);
         }
-        if (rank >= k) continue;
-        const int row = group * a.width + b, token = ls.token[i];
-        const bool ended = (a.done && a.done[row]) || (a.eos >= 0 && token == a.eos);
-        ls.list[2 * rank] = (uint64_t)(uint32_t)token << 32 | (uint32_t)(row << 1 | (int)ended);
-        ls.list[2 * rank + 1] = __float_as_uint((float)score);
+        if (x == (double)kNone || rank >= k) continue;
+        const int at = group * k + rank, b = i / k, token = s_token[i];
+        a.parent[at] = group * a.width + b;
+        a.token[at] = token;
+        a.out_scores[at] = (float)x;
+        if (a.out_done) a.out_done[at] = (int)(endeds >> b & 1) || (a.eos >= 0 && token == a.eos);
     }
-    __syncthreads();  // what may be replaced in place has been read
-    if (tid < k) {
+    if (tid >= total && tid < k) {
         const int at = group * k + tid;
-        const bool some = tid < all;
-        const uint64_t x = ls.list[2 * tid];
-        a.parent[at] = some ? (int)((uint32_t)x >> 1) : -1;
-        a.token[at] = some ? (int)(x >> 32) : -1;
-        a.out_scores[at] = some ? __uint_as_float((uint32_t)ls.list[2 * tid + 1]) : kNone;
-        if (a.out_done) a.out_done[at] = some ? (int)(x & 1) : 0;
+        a.parent[at] = -1;
+        a.token[at] = -1;
+        a.out_scores[at] = kNone;
+        if (a.out_done) a.out_done[at] = 0;
     }
 }
 
-template <int VALUES>
-__global__ __launch_bounds__(kBeamThreads) __attribute__((amdgpu_waves_per_eu(6, 6))) void beam_select_kernel(BeamArgs a, int splits) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(6, 8))) void beam_select_kernel(BeamArgs a, int parts) {
     __shared__ Shared sh;
-    extern __shared__ uint64_t s_lists[];
-    Lists ls;
-    ls.list = s_lists;
-    ls.score = (double*)(s_lists + list_entries(VALUES, a.k));
-    ls.token = (int*)(ls.score + a.width * a.k);
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, k = a.k;
-    const int row = blockIdx.x / splits, split = blockIdx.x - row * splits, group = row / a.width;
-    const float score = a.scores[row];
-    if (!dead(score) && !(a.done && a.done[row])) {
+    extern __shared__ double s_score[];  // [width][k], and as many tokens
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), k = a.k;
+    const int row = __builtin_amdgcn_readfirstlane(blockIdx.x / parts), part = blockIdx.x - row * parts;
+    const int group = __builtin_amdgcn_readfirstlane(row / a.width);
+    // Of the group, a beam a lane, for the merge: read before any output is written.
+    const int beam = group * a.width + min(lane, a.width - 1);
+    const float score = a.scores[beam];
+    const bool ended = a.done && a.done[beam];
+    if (!dead(scalar(a.scores + row)) && !(a.done && scalar(a.done + row))) {
         // (A row need not start at a 16-byte border: its loads only ask for one of 4.)
         typedef float float4u __attribute__((ext_vector_type(4), aligned(4)));
         const float* x = a.logits + row * a.stride;
-        const int first = split * (kBeamThreads * VALUES) + tid * 4;
-        float v[VALUES];
+        const int tiles = (a.vocab + kBeamTile - 1) / kBeamTile;
+        Best best;
+        for (int t = part * kBeamWaves + wave; t < tiles; t += parts * kBeamWaves) {
+            const int first = t * kBeamTile + lane * 4;
+            Tile v;
+            if ((t + 1) * kBeamTile <= a.vocab) {
 #pragma unroll
-        for (int i = 0; i < VALUES / 4; ++i) {
-            const int t = first + i * kBeamThreads * 4;
-            if (t + 4 <= a.vocab) {
-                const float4u y = *(const float4u*)(x + t);
+                for (int i = 0; i < kBeamValues / 4; ++i) {
+                    const float4u y = *(const float4u*)(x + first + 256 * i);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * i + e] = y[e];
+                    for (int e = 0; e < 4; ++e) v[4 * i + e] = y[e];
+                }
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[4 * i + e] = t + e < a.vocab ? x[t + e] : kNone;
+                for (int i = 0; i < kBeamValues; ++i) {
+                    const int at = first + 256 * (i >> 2) + (i & 3);
+                    v[i] = at < a.vocab ? x[at] : kNone;
+                }
             }
-        }
-        float top = kNone;
-        bool broken = false;
+            float top = kNone;
 #pragma unroll
-        for (int i = 0; i < VALUES; ++i) {
-            v[i] += 0.0f;  // -0 is 0
-            broken |= !(v[i] < __builtin_inff());
-            top = fmaxf(top, v[i]);
-        }
-        int best = -1;  // the first of the largest
+            for (int i = 0; i < kBeamValues; ++i) top = fmaxf(top, v[i]);
+            const float M = wave_max(top), base = M == kNone ? 0.0f : M;
+            float4v s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = VALUES - 1; i >= 0; --i) best = v[i] == top ? i : best;
-        auto token = [&](int i) { return first + (i >> 2) * kBeamThreads * 4 + (i & 3); };
-        const uint64_t mine = top == kNone || broken ? 0 : key_of(top, token(best));
-        uint64_t border = kth_of_lanes(mine, k);
-        float wave_top = top;
-#pragma unroll
-        for (int d = 32; d; d >>= 1) wave_top = fmaxf(wave_top, __shfl_xor(wave_top, d));
-        broken = __ballot(broken);
-        if (lane == 0) {
-            sh.border[wave] = border;
-            sh.top[wave] = broken ? __builtin_nanf("") : wave_top;
+            for (int i = 0; i < kBeamValues; ++i) s[i & 3] += fast_exp2((v[i] - base) * kLog2e);
+            // (NaN if a value is NaN, or +inf, which is the maximum then.)
+            const float sum = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
+            if (lane == 0)
+                store_dev64(a.sums + (int64_t)row * tiles + t, (uint64_t)__float_as_uint(sum) << 32 | __float_as_uint(M));
+            if (!(sum == sum) || M == kNone || (best.kth != 0 && M <= logit_of(best.kth))) continue;  // (of equal ones the earlier tile's)
+            take_tile(best, v, top, M, first, k, lane, sh.slot[wave]);
         }
-        if (tid == 0) sh.count[0] = 0;
-        __syncthreads();
-        float M = kNone;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            border = max(border, sh.border[w]);
-            M = fmaxf(M, sh.top[w]);
-            broken |= sh.top[w] != sh.top[w];
-        }
-        // Sums of exponentials against the workgroup's maximum.
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const float base = M == kNone ? 0.0f : M;
-        const float least = logit_of(border);
-#pragma unroll
-        for (int i = 0; i < VALUES; ++i) {
-            s[i & 3] += fast_exp2((v[i] - base) * kLog2e);
-            if (v[i] >= least || border == 0) {
-                const uint64_t key = key_of(v[i], token(i));
-                if (v[i] != kNone && !broken && key >= border) ls.list[atomicAdd(&sh.count[0], 1)] = key;
-            }
-        }
-        float sum = (s[0] + s[1]) + (s[2] + s[3]);
-#pragma unroll
-        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-        if (lane == 0) sh.sum[wave] = sum;
-        __syncthreads();
-        uint64_t* keys = a.keys + ((int64_t)row * splits + split) * k;
-        const int n = sh.count[0];
-        for (int i = tid; i < n; i += kBeamThreads) {
-            const uint64_t key = ls.list[i];
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += ls.list[j] > key;
-            if (rank < k) store_dev64(keys + rank, key);
-        }
-        if (tid >= n && tid < k) store_dev64(keys + tid, 0);
-        if (tid == 0) {
-            float total = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) total += sh.sum[w];
-            if (broken) total = __builtin_nanf("");
-            store_dev64((uint64_t*)a.sums + (int64_t)row * splits + split,
-                        (uint64_t)__float_as_uint(total) << 32 | __float_as_uint(M));
-        }
+        uint64_t* keys = a.keys + ((int64_t)row * (kBeamMaxParts * kBeamWaves) + part * kBeamWaves + wave) * k;
+        if (lane < k) store_dev64(keys + lane, best.key);
     }
     stores_done_barrier();
     uint32_t* arrived = a.arrived + group * kBeamCounterStep;
-    if (tid == 0) sh.last = ticket_add(arrived) == (uint32_t)(a.width * splits - 1);
+    if (tid == 0) sh.last = ticket_add(arrived) == (uint32_t)(a.width * parts - 1);
     __syncthreads();
     if (!sh.last) return;
-    merge(a, group, splits, sh, ls);
+    merge(a, group, parts * kBeamWaves, score, ended, sh, s_score);
     if (tid == 0) ticket_reset(arrived);
-}
-
-template <int VALUES>
-hipError_t launch(const BeamArgs& a, hipStream_t stream) {
-    const int splits = beam_splits(a.vocab);
-    const size_t lds = (size_t)list_entries(VALUES, a.k) * 8 + (size_t)a.width * a.k * 12;
-    const int64_t wgs = (int64_t)a.groups * a.width * splits;
-    hipLaunchKernelGGL(beam_select_kernel<VALUES>, dim3((unsigned)wgs), dim3(kBeamThreads), lds, stream, a, splits);
-    return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_beam_select(const BeamArgs& a, hipStream_t stream) {
+hipError_t launch_beam_select(const BeamArgs& a, int cus, hipStream_t stream) {
     if (a.groups < 1 || a.groups > kBeamMaxGroups || a.width < 1 || a.width > kBeamMaxWidth || a.k < 1 ||
         a.k > kBeamMaxK || a.vocab < 1 || a.vocab > kBeamMaxVocab)
         return hipErrorInvalidValue;
-    switch (beam_values(a.vocab)) {
-        case 8: return launch<8>(a, stream);
-        case 16: return launch<16>(a, stream);
-        default: return launch<32>(a, stream);
-    }
+    const int rows = a.groups * a.width, tiles = beam_tiles(a.vocab);
+    const int64_t turns = ((int64_t)rows * tiles + 16 * cus - 1) / (16 * cus);  // tiles of a wave
+    int64_t parts = (tiles + turns * kBeamWaves - 1) / (turns * kBeamWaves);
+    parts = parts < kBeamMaxParts ? parts : kBeamMaxParts;
+    hipLaunchKernelGGL(beam_select_kernel, dim3((unsigned)(rows * parts)), dim3(kThreads), (size_t)a.width * a.k * 12,
+                       stream, a, (int)parts);
+    return hipGetLastError();
 }
 
 }  // namespace qasr

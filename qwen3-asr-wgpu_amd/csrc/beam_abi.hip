@@ -18,8 +18,8 @@ struct qasr_beam {
     int device;
     int32_t max_groups, width, vocab, k;
     char* mem = nullptr;
-    uint64_t* keys;
-    float* sums;
+    size_t bytes = 0;
+    uint64_t *keys, *sums;
     uint32_t* arrived;
 };
 
@@ -53,11 +53,13 @@ int qasr_beam_create(qasr_ctx* ctx, int max_groups, int width, int vocab, int k,
     b->width = width;
     b->vocab = vocab;
     b->k = k;
-    const size_t pieces = (size_t)max_groups * width * qasr::beam_splits(vocab);
-    const size_t o_sums = (size_t)max_groups * qasr::kBeamCounterStep * 4, o_keys = o_sums + pieces * 8;
+    const size_t rows = (size_t)max_groups * width;
+    const size_t o_sums = (size_t)max_groups * qasr::kBeamCounterStep * 4;
+    const size_t o_keys = o_sums + rows * qasr::beam_tiles(vocab) * 8;
+    b->bytes = o_keys + rows * qasr::kBeamMaxParts * qasr::kBeamWaves * k * 8;
     DeviceScope ds(ctx->device);
     hipError_t e = ds.err;
-    if (e == hipSuccess) e = hipMalloc(&b->mem, o_keys + pieces * k * 8);
+    if (e == hipSuccess) e = hipMalloc(&b->mem, b->bytes);
     if (e == hipSuccess) e = hipMemset(b->mem, 0, o_sums);
     if (e == hipSuccess) e = hipDeviceSynchronize();
     if (e != hipSuccess) {
@@ -67,7 +69,7 @@ int qasr_beam_create(qasr_ctx* ctx, int max_groups, int width, int vocab, int k,
         return hip_fail(e, "beam selection allocation");
     }
     b->arrived = (uint32_t*)b->mem;
-    b->sums = (float*)(b->mem + o_sums);
+    b->sums = (uint64_t*)(b->mem + o_sums);
     b->keys = (uint64_t*)(b->mem + o_keys);
     *out = b;
     return QASR_OK;
@@ -105,9 +107,7 @@ int qasr_beam_select(qasr_ctx* ctx, qasr_beam* beam, int groups, const float* lo
     const Range ins[] = {{(uintptr_t)scores_dev, in}, {(uintptr_t)done_dev, in}};
     const Range outs[] = {{(uintptr_t)parent_dev, res}, {(uintptr_t)token_dev, res}, {(uintptr_t)out_scores_dev, res},
                           {(uintptr_t)out_done_dev, res}};
-    const Range own{(uintptr_t)beam->mem, (int64_t)((char*)(beam->keys + (int64_t)beam->max_groups * beam->width *
-                                                                             qasr::beam_splits(beam->vocab) * beam->k) -
-                                                    beam->mem)};
+    const Range own{(uintptr_t)beam->mem, (int64_t)beam->bytes};
     for (const Range& o : outs) {
         if (o.meets(logits) || o.meets(own)) return fail(QASR_EINVAL, "an output lies in the logits or the workspace");
         for (const Range& i : ins)
@@ -135,7 +135,7 @@ int qasr_beam_select(qasr_ctx* ctx, qasr_beam* beam, int groups, const float* lo
     a.keys = beam->keys;
     a.sums = beam->sums;
     a.arrived = beam->arrived;
-    const hipError_t e = qasr::launch_beam_select(a, (hipStream_t)stream);
+    const hipError_t e = qasr::launch_beam_select(a, ctx->cus, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(e, "beam selection launch");
     return QASR_OK;
 }
