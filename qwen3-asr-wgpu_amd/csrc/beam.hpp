@@ -7,7 +7,7 @@
 namespace qasr {
 
 constexpr int kBeamMaxGroups = 1024, kBeamMaxWidth = 32, kBeamMaxK = 32;
-constexpr int kBeamWaves = 4;      // of a workgroup
+constexpr int kBeamWaves = 8;      // of a workgroup
 constexpr int kBeamValues = 32;    // logits of a lane
 constexpr int kBeamTile = 64 * kBeamValues;  // of a wave
 constexpr int kBeamMaxVocab = 1 << 20;
