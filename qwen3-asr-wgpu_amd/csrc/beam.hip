@@ -80,9 +80,10 @@ __device__ __forceinline__ float wave_sum(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// The largest of some borders that at least k of the lanes' values reach, by
-// their ordered bits, of which `top` are the largest; 0 if fewer than k are not 0.
-// Exactly k reach it but where several are equal to the k-th.
+// A border that at least k of the lanes' values reach, by their ordered bits, of
+// which `top` are the largest, and few more than k, unless several are equal to
+// the k-th; 0 if fewer than k are not 0.
+constexpr int kSpare = 3;  // (a value more is cheaper to rank than another step of the bisection)
 __device__ __forceinline__ uint32_t border_of(uint32_t mine, uint32_t top, int k) {
     uint32_t lo = 0, hi = top + 1;  // at least k reach lo, fewer hi (none has all bits set)
     int n = __popcll(__ballot(mine != 0));
@@ -95,8 +96,9 @@ __device__ __forceinline__ uint32_t border_of(uint32_t mine, uint32_t top, int k
             n = m;
             break;
         }
+        hi = top - d;
     }
-    while (n != k && hi - lo > 1) {
+    while (n > k + kSpare && hi - lo > 1) {
         const uint32_t mid = lo + (hi - lo) / 2;
         const int m = __popcll(__ballot(mine >= mid));
         if (m >= k) {
@@ -118,48 +120,56 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
-__device__ __forceinline__ uint64_t lane_key(uint64_t key, int lane) {
-    return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), lane) << 32 |
-           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)key, lane);
-}
 
-// A wave's k best keys so far, best first, a lane each.
+// A wave's k best keys so far, best first, in its list in LDS, and behind them
+// what may be among them.
+constexpr int kPending = 64;
+constexpr int kList = kBeamMaxK + kPending;
 struct Best {
-    uint64_t key = 0;  // lane i < held: the i-th
     uint64_t kth = 0;  // 0 while there are fewer
-    int held = 0;
+    int held = 0, pending = 0;
 };
-// Takes a key of each lane (0: none) among them.  Those that are better than the
-// k-th come to all lanes one by one, and each lane counts what comes before its
-// own: few, as callers leave out what cannot be among the k best.
-__device__ __forceinline__ void take(Best& b, uint64_t key, int k, int lane, uint64_t* slot) {
-    key = key > b.kth ? key : 0;
-    const uint64_t todo = __ballot(key != 0);
-    if (todo == 0) return;
-    int rank = 0, held_rank = lane;
-    for (uint64_t t = todo; t; t &= t - 1) {
-        const int l = __builtin_ctzll(t);
-        const uint64_t x = lane_key(key, l);
-        const int before = __popcll(__ballot(b.key > x));
-        rank += (x > key) + (lane == l ? before : 0);
-        held_rank += x > b.key;
+// Each key's rank is the number of better ones: every lane compares its own (or
+// two) with all, which it reads two at a time.  Keys are unique.
+__device__ __forceinline__ void rank_list(Best& b, int k, int lane, uint64_t* list) {
+    typedef unsigned long long Two __attribute__((ext_vector_type(2)));
+    const int total = b.held + b.pending;
+    if (lane == 0) list[total] = 0;
+    wave_sync();
+    const uint64_t x = list[lane], y = total > 64 ? list[min(lane + 64, kList)] : 0;
+    int rank = 0, rank_y = 0;
+#pragma unroll 4
+    for (int j = 0; j < total; j += 2) {
+        const Two z = *(const Two*)(list + j);
+        rank += (z[0] > x) + (z[1] > x);
+        if (total > 64) rank_y += (z[0] > y) + (z[1] > y);
     }
-    if (key != 0 && rank < k) slot[rank] = key;
-    if (lane < b.held && held_rank < k) slot[held_rank] = b.key;
-    b.held = min(b.held + __popcll(todo), k);
     wave_sync();
-    b.key = lane < b.held ? slot[lane] : 0;
+    if (lane < total && rank < k) list[rank] = x;
+    if (lane + 64 < total && rank_y < k) list[rank_y] = y;
+    b.held = min(total, k);
+    b.pending = 0;
     wave_sync();
-    b.kth = b.held == k ? lane_key(b.key, k - 1) : 0;
+    b.kth = b.held == k ? list[k - 1] : 0;
+}
+// Takes a key of each lane (0: none) into the list.
+__device__ __forceinline__ void take(Best& b, uint64_t key, int k, int lane, uint64_t* list) {
+    uint64_t some = __ballot(key > b.kth);
+    if (b.pending + __popcll(some) > kPending) {
+        rank_list(b, k, lane, list);
+        some = __ballot(key > b.kth);
+    }
+    if (key > b.kth) list[b.held + b.pending + __popcll(some & ((1ull << lane) - 1))] = key;
+    b.pending += __popcll(some);
 }
 
 // A tile's values, of which this lane's largest is `top`, the wave's M.  Token of
 // v[i]: first + 256 (i / 4) + i % 4.
-__device__ __forceinline__ void take_tile(Best& b, const Tile& v, float top, float M, int first, int k, int lane, uint64_t* slot) {
+__device__ __forceinline__ void take_tile(Best& b, const Tile& v, float top, float M, int first, int k, int lane, uint64_t* list) {
     // At least k of the row reach the border, a value.
     uint32_t border = max((uint32_t)(b.kth >> 32), 1u);
     const uint32_t mine = top == kNone ? 0 : order_of(top + 0.0f);
-    if (__popcll(__ballot(mine >= border)) > k) border = max(border, border_of(mine, order_of(M + 0.0f), k));
+    if (__popcll(__ballot(mine >= border)) > k + kSpare) border = max(border, border_of(mine, order_of(M + 0.0f), k));
     const float least = value_of(border);
     uint32_t mask = 0;
 #pragma unroll
@@ -176,15 +186,15 @@ __device__ __forceinline__ void take_tile(Best& b, const Tile& v, float top, flo
 #pragma unroll
         for (int j = 0; j < 2; ++j) x[j] = i & 8 ? x[2 * j + 1] : x[2 * j];
         const float y = (i & 16 ? x[1] : x[0]) + 0.0f;  // -0 is 0
-        take(b, mask ? key_of(y, first + 256 * (i >> 2) + (i & 3)) : 0, k, lane, slot);
+        take(b, mask ? key_of(y, first + 256 * (i >> 2) + (i & 3)) : 0, k, lane, list);
         mask &= mask - 1;
     }
+    if (b.pending) rank_list(b, k, lane, list);
 }
 
 struct Shared {
-    uint64_t slot[kBeamWaves][kBeamMaxK];
+    alignas(16) uint64_t list[kBeamWaves][kList + 2];
     int last;
-    int offers[kBeamMaxWidth];
 };
 
 // Row sums and lists of the group's beams, a wave a beam; then the beams'
@@ -201,9 +211,8 @@ __device__ __forceinline__ void merge(const BeamArgs& a, int group, int lists, f
         const int row = group * a.width + b;
         const float s_b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(score), b));
         double mine = kNone;  // candidate `lane`
-        int token = a.eos, offers = 0;
+        int token = a.eos;
         if (!dead(s_b) && (endeds >> b & 1)) {
-            offers = 1;
             mine = lane == 0 ? (double)s_b : mine;
         } else if (!dead(s_b)) {
             const uint64_t* keys = a.keys + (int64_t)row * (kBeamMaxParts * kBeamWaves) * k;
@@ -256,17 +265,18 @@ __device__ __forceinline__ void merge(const BeamArgs& a, int group, int lists, f
                         const int j = mask ? __builtin_ctz(mask) : 0;
                         const uint64_t y0 = j & 1 ? x[1] : x[0], y1 = j & 1 ? x[3] : x[2], y2 = j & 1 ? x[5] : x[4], y3 = j & 1 ? x[7] : x[6];
                         const uint64_t z0 = j & 2 ? y1 : y0, z1 = j & 2 ? y3 : y2;
-                        take(best, mask ? (j & 4 ? z1 : z0) : 0, k, lane, sh.slot[wave]);
+                        take(best, mask ? (j & 4 ? z1 : z0) : 0, k, lane, sh.list[wave]);
                         mask &= mask - 1;
                     }
                     i0 += 64 * kBatch;
                     if (i0 >= lists * k) break;
                     load(i0);
                 }
-                offers = best.held;
-                if (lane < offers) {
-                    mine = (double)s_b + ((double)logit_of(best.key) - lse);
-                    token = token_of(best.key);
+                if (best.pending) rank_list(best, k, lane, sh.list[wave]);
+                if (lane < best.held) {
+                    const uint64_t key = sh.list[wave][lane];
+                    mine = (double)s_b + ((double)logit_of(key) - lse);
+                    token = token_of(key);
                 }
             }
         }
@@ -274,12 +284,10 @@ __device__ __forceinline__ void merge(const BeamArgs& a, int group, int lists, f
             s_score[b * k + lane] = mine;
             s_token[b * k + lane] = token;
         }
-        if (lane == 0) sh.offers[b] = offers;
     }
     __syncthreads();
-    // Each candidate's rank: how many come before it.
-    int total = 0;
-    for (int b = 0; b < a.width; ++b) total += sh.offers[b];
+    // Each candidate's rank: how many come before it; those that are none are the
+    // last.
     for (int i = tid; i < n; i += kThreads) {
         const double x = s_score[i];
         int rank = 0;
@@ -288,19 +296,13 @@ __device__ __forceinline__ void merge(const BeamArgs& a, int group, int lists, f
             const double y = s_score[j];
             rank += y > x || (y == x && j < i);
         }
-        if (x == (double)kNone || rank >= k) continue;
+        if (rank >= k) continue;
+        const bool none = x == (double)kNone;
         const int at = group * k + rank, b = i / k, token = s_token[i];
-        a.parent[at] = group * a.width + b;
-        a.token[at] = token;
+        a.parent[at] = none ? -1 : group * a.width + b;
+        a.token[at] = none ? -1 : token;
         a.out_scores[at] = (float)x;
-        if (a.out_done) a.out_done[at] = (int)(endeds >> b & 1) || (a.eos >= 0 && token == a.eos);
-    }
-    if (tid >= total && tid < k) {
-        const int at = group * k + tid;
-        a.parent[at] = -1;
-        a.token[at] = -1;
-        a.out_scores[at] = kNone;
-        if (a.out_done) a.out_done[at] = 0;
+        if (a.out_done) a.out_done[at] = !none && ((endeds >> b & 1) || (a.eos >= 0 && token == a.eos));
     }
 }
 
@@ -320,9 +322,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(6, 8))
         const float* x = a.logits + row * a.stride;
         const int tiles = (a.vocab + kBeamTile - 1) / kBeamTile;
         Best best;
-        for (int t = part * kBeamWaves + wave; t < tiles; t += parts * kBeamWaves) {
+        auto load = [&](Tile& v, int t) {
             const int first = t * kBeamTile + lane * 4;
-            Tile v;
             if ((t + 1) * kBeamTile <= a.vocab) {
 #pragma unroll
                 for (int i = 0; i < kBeamValues / 4; ++i) {
@@ -337,6 +338,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(6, 8))
                     v[i] = at < a.vocab ? x[at] : kNone;
                 }
             }
+        };
+        const int step = parts * kBeamWaves;
+        for (int t = part * kBeamWaves + wave; t < tiles; t += step) {
+            Tile v;
+            load(v, t);
             float top = kNone;
 #pragma unroll
             for (int i = 0; i < kBeamValues; ++i) top = fmaxf(top, v[i]);
@@ -349,10 +355,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(6, 8))
             if (lane == 0)
                 store_dev64(a.sums + (int64_t)row * tiles + t, (uint64_t)__float_as_uint(sum) << 32 | __float_as_uint(M));
             if (!(sum == sum) || M == kNone || (best.kth != 0 && M <= logit_of(best.kth))) continue;  // (of equal ones the earlier tile's)
-            take_tile(best, v, top, M, first, k, lane, sh.slot[wave]);
+            take_tile(best, v, top, M, t * kBeamTile + lane * 4, k, lane, sh.list[wave]);
         }
         uint64_t* keys = a.keys + ((int64_t)row * (kBeamMaxParts * kBeamWaves) + part * kBeamWaves + wave) * k;
-        if (lane < k) store_dev64(keys + lane, best.key);
+        if (lane < k) store_dev64(keys + lane, lane < best.held ? sh.list[wave][lane] : 0);
     }
     stores_done_barrier();
     uint32_t* arrived = a.arrived + group * kBeamCounterStep;
