@@ -56,6 +56,39 @@ __device__ __forceinline__ float head_inv_rms(const f16* raw, float eps) {
     return 1.0f / sqrtf(sum2 / (float)kHeadDim + eps);
 }
 
+// The same in 32 registers less than half as many: a quarter of the head is read
+// while the one before is added.
+__device__ __forceinline__ float head_inv_rms_lean(const f16* raw, float eps) {
+#pragma clang fp contract(off)
+    constexpr int kPart = 4;
+    H8 v[kPart], w[kPart];
+    auto read = [&](H8 (&x)[kPart], int part) {
+#pragma unroll
+        for (int i = 0; i < kPart; ++i) x[i].u = *(const uint4*)(raw + 8 * (kPart * part + i));
+    };
+    float sum2 = 0.0f;
+    auto add = [&](const H8 (&x)[kPart]) {
+#pragma unroll
+        for (int i = 0; i < kPart; ++i) {
+            const uint32_t d[4] = {x[i].u.x, x[i].u.y, x[i].u.z, x[i].u.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                asm("v_fma_mix_f32 %0, %1, %1, %0 op_sel_hi:[1,1,0]" : "+v"(sum2) : "v"(d[e]));
+                asm("v_fma_mix_f32 %0, %1, %1, %0 op_sel:[1,1,0] op_sel_hi:[1,1,0]" : "+v"(sum2) : "v"(d[e]));
+            }
+        }
+    };
+    read(v, 0);
+#pragma unroll 1
+    for (int part = 0; part < kHeadDim / 8 / kPart; part += 2) {
+        read(w, part + 1);
+        add(v);
+        read(v, (part + 2) & 3);  // (the last is the first again: not used)
+        add(w);
+    }
+    return 1.0f / sqrtf(sum2 / (float)kHeadDim + eps);
+}
+
 // One roped element j of a head whose raw values, gains and cos/sin rows are
 // given (all f16).  `inv` is the head's inverse RMS.
 __device__ __forceinline__ f16 rope_elem(const f16* raw, const f16* gain, const f16* cos_row,

@@ -79,10 +79,15 @@ __device__ __forceinline__ H8 widen8(uint2 x, float unit) {
     y.h2[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x.y, unit, true);
     return y;
 }
+template <int Ctrl>
+__device__ __forceinline__ uint32_t other(uint32_t x) {
+    return __float_as_uint(dpp<Ctrl>(__uint_as_float(x)));
+}
 __device__ __forceinline__ float unit_value(uint32_t byte) { return __uint_as_float(byte << 23); }
 
-__global__ __launch_bounds__(kThreads) void paged_append8_kernel(PagedAppend8Args a) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) void paged_append8_kernel(PagedAppend8Args a) {
     __shared__ __attribute__((aligned(16))) f16 s_raw[3 * kRun * kPad];
+    __shared__ __attribute__((aligned(16))) f16 s_gain[2 * kHeadDim];  // of Q, of K
     __shared__ float s_inv[3 * kRun];
     __shared__ int s_slot[kWindow], s_pos[kWindow];
     __shared__ uint32_t s_starts;  // rows of the window at which a run starts
@@ -91,6 +96,27 @@ __global__ __launch_bounds__(kThreads) void paged_append8_kernel(PagedAppend8Arg
 
     const int tid = threadIdx.x, chunk = blockIdx.x / a.nkvh, kvh = blockIdx.x - chunk * a.nkvh;
     const int first = chunk * kRun, rows = min(kWindow, a.rows - first);
+    // A thread: 8 dims and their partners of row `ar` of a pass, of Q's head `half`
+    // of the two and of K (0) or V (1).
+    const int w = tid & 7, d = 8 * w, half = (tid >> 3) & 1, ar = tid >> 4;
+    const int nh = a.nqh + 2 * a.nkvh;
+    const f16* q_src = a.qkv + ((int64_t)first * nh + 2 * kvh + half) * kHeadDim + d;
+    const f16* k_src = a.qkv + ((int64_t)first * nh + a.nqh + half * a.nkvh + kvh) * kHeadDim + d;
+    H8 q[2], k[2];
+    auto load_row = [&](int row) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            q[i].u = *(const uint4*)(q_src + (int64_t)row * nh * kHeadDim + i * (kHeadDim / 2));
+            k[i].u = *(const uint4*)(k_src + (int64_t)row * nh * kHeadDim + i * (kHeadDim / 2));
+        }
+    };
+    // (The step's first row starts a run: rows of small steps need not wait for
+    // their places.)
+    if (chunk == 0) load_row(min(ar, rows - 1));
+    if (tid >= kThreads - 32) {  // (not the wave of the serial sums)
+        const int i = tid & 15;
+        *(uint4*)&s_gain[8 * (tid & 31)] = *(const uint4*)((tid & 16 ? a.k_gain : a.q_gain) + 8 * i);
+    }
     // The window's rows: a slot of -1 where there is nothing to store.  A row
     // goes on with the run of the row before it if it lies behind it in its block.
     if (tid < 64) {
@@ -114,50 +140,34 @@ __global__ __launch_bounds__(kThreads) void paged_append8_kernel(PagedAppend8Arg
         const uint32_t x = r < 32 ? starts >> r : 0;
         return x ? r + __builtin_ctz(x) : rows;
     };
-    const int w = tid & 7;
-    const int qr = tid >> 4, qh = (tid >> 3) & 1;             // Q: row of the pass, head
-    const int kr = (tid & 127) >> 3, kv = tid >> 7;           // K or V: row of the pass
-    const int nh = a.nqh + 2 * a.nkvh;
-    const int d = 8 * w;
-
     const int end = start_from(kRun);  // runs that start behind are the next workgroup's
     for (int p0 = start_from(0), p1; p0 < min(kRun, rows); p0 = p1) {
         p1 = p0 + kRun < end ? run_of(p0 + kRun) : end;  // whole runs, 16 rows at most
-        const bool q_on = p0 + qr < p1, k_on = p0 + kr < p1;
-        const int q_row = min(p0 + qr, p1 - 1), k_row = min(p0 + kr, p1 - 1);
-        const f16* src = a.qkv + (int64_t)first * nh * kHeadDim + d;
-        const f16* qs = src + ((int64_t)q_row * nh + 2 * kvh + qh) * kHeadDim;
-        const f16* ks = src + ((int64_t)k_row * nh + a.nqh + kv * a.nkvh + kvh) * kHeadDim;
-        const int q_pos = max(s_pos[q_row], 0), k_pos = max(s_pos[k_row], 0);
-        const int slot = s_slot[k_row], start = run_of(k_row), start_slot = s_slot[start];
-        H8 q[2], k[2], qc[2], qn[2], kc[2], kn[2], qg[2], kg[2];
+        const bool on = p0 + ar < p1;
+        const int row = min(p0 + ar, p1 - 1);
+        if (chunk != 0 || p0 != 0) load_row(row);
+        const int pos = max(s_pos[row], 0), slot = s_slot[row], start = run_of(row), start_slot = s_slot[start];
+        H8 c[2], sn[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int j = i * (kHeadDim / 2);
-            q[i].u = *(const uint4*)(qs + j);
-            k[i].u = *(const uint4*)(ks + j);
-            qc[i].u = *(const uint4*)(a.cos_tab + (int64_t)q_pos * kHeadDim + d + j);
-            qn[i].u = *(const uint4*)(a.sin_tab + (int64_t)q_pos * kHeadDim + d + j);
-            kc[i].u = *(const uint4*)(a.cos_tab + (int64_t)k_pos * kHeadDim + d + j);
-            kn[i].u = *(const uint4*)(a.sin_tab + (int64_t)k_pos * kHeadDim + d + j);
-            qg[i].u = *(const uint4*)(a.q_gain + d + j);
-            kg[i].u = *(const uint4*)(a.k_gain + d + j);
+            c[i].u = *(const uint4*)(a.cos_tab + (int64_t)pos * kHeadDim + d + i * (kHeadDim / 2));
+            sn[i].u = *(const uint4*)(a.sin_tab + (int64_t)pos * kHeadDim + d + i * (kHeadDim / 2));
         }
         // Block of the run: its byte, and its first row's place.
         const int page = max(start_slot, 0) >> a.page_shift, in_page = max(start_slot, 0) & ((1 << a.page_shift) - 1);
-        uint8_t* unit_at = a.scales + (int64_t)page * a.page_scales + kv * a.kv_scales + kvh * a.head_scales + (in_page >> 4);
-        uint8_t* block = a.base + (int64_t)page * a.page_stride + kv * a.kv_stride + kvh * a.head_stride +
+        uint8_t* unit_at = a.scales + (int64_t)page * a.page_scales + half * a.kv_scales + kvh * a.head_scales + (in_page >> 4);
+        uint8_t* block = a.base + (int64_t)page * a.page_stride + half * a.kv_stride + kvh * a.head_stride +
                          (int64_t)(in_page & ~(kRun - 1)) * kHeadDim;
         uint32_t old = *unit_at;
         const int held = start_slot >= 0 ? start_slot & (kRun - 1) : 0;  // rows that the block has
         old = held ? old : 0;
-        if (q_on) {
-            f16* at = &s_raw[(2 * qr + qh) * kPad + d];
+        if (on) {
+            f16* at = &s_raw[(2 * ar + half) * kPad + d];
             *(uint4*)at = q[0].u;
             *(uint4*)(at + kHeadDim / 2) = q[1].u;
         }
-        if (k_on && !kv) {
-            f16* at = &s_raw[(2 * kRun + kr) * kPad + d];
+        if (on && !half) {
+            f16* at = &s_raw[(2 * kRun + ar) * kPad + d];
             *(uint4*)at = k[0].u;
             *(uint4*)(at + kHeadDim / 2) = k[1].u;
         }
@@ -166,41 +176,51 @@ __global__ __launch_bounds__(kThreads) void paged_append8_kernel(PagedAppend8Arg
         {
             const int n = p1 - p0;
             if (tid < 3 * kRun && (tid < 2 * kRun ? tid >> 1 : tid - 2 * kRun) < n)
-                s_inv[tid] = head_inv_rms(&s_raw[tid * kPad], a.eps);
+                s_inv[tid] = head_inv_rms_lean(&s_raw[tid * kPad], a.eps);
         }
         __syncthreads();
         {
-            H8 o[2];
-            rope16(q, qg, qc, qn, s_inv[2 * qr + qh], o);
-            if (q_on && s_pos[q_row] >= 0) {
-                f16* dst = a.q_out + ((int64_t)(first + q_row) * a.nqh + 2 * kvh + qh) * kHeadDim + d;
+            H8 o[2], gain[2];
+            auto from = [&](H8 (&x)[2], const f16* p) {
+                x[0].u = *(const uint4*)p;
+                x[1].u = *(const uint4*)(p + kHeadDim / 2);
+            };
+            from(q, &s_raw[(2 * ar + half) * kPad + d]);
+            from(gain, s_gain + d);
+            rope16(q, gain, c, sn, s_inv[2 * ar + half], o);
+            if (on && s_pos[row] >= 0) {
+                f16* dst = a.q_out + ((int64_t)(first + row) * a.nqh + 2 * kvh + half) * kHeadDim + d;
                 *(uint4*)dst = o[0].u;
                 *(uint4*)(dst + kHeadDim / 2) = o[1].u;
             }
+            from(gain, s_gain + kHeadDim + d);
+            rope16(k, gain, c, sn, s_inv[2 * kRun + ar], o);
+            if (!half) {
+                k[0] = o[0];
+                k[1] = o[1];
+            }
         }
-        if (!kv) {
-            H8 o[2];
-            rope16(k, kg, kc, kn, s_inv[2 * kRun + kr], o);
-            k[0] = o[0];
-            k[1] = o[1];
-        }
-        if (k_on && slot >= 0) atomicMax(&s_top[kv][start - p0], max(top_of(k[0]), top_of(k[1])));
-        if (k_on && start == k_row && w == 0) s_old[kv][kr] = slot >= 0 ? old | held << 8 : 0;
+        uint32_t top = max(top_of(k[0]), top_of(k[1]));  // of the row's: of 8 lanes
+        top = max(top, other<kDppXor1>(top));
+        top = max(top, other<kDppXor2>(top));
+        top = max(top, other<kDppHalfMirror>(top));
+        if (on && slot >= 0 && w == 0) atomicMax(&s_top[half][start - p0], top);
+        if (on && start == row && w == 0) s_old[half][ar] = slot >= 0 ? old | held << 8 : 0;
         __syncthreads();
-        const uint32_t need = unit_of(s_top[kv][start - p0]), unit = max(old, need);
-        if (k_on && slot >= 0) {
+        const uint32_t need = unit_of(s_top[half][start - p0]), unit = max(old, need);
+        if (on && slot >= 0) {
             uint8_t* dst = block + (slot & (kRun - 1)) * kHeadDim + d;
             *(uint2*)dst = narrow8(k[0], unit_value(unit));
             *(uint2*)(dst + kHeadDim / 2) = narrow8(k[1], unit_value(unit));
-            if (start == k_row && w == 0) *unit_at = (uint8_t)unit;
+            if (start == row && w == 0) *unit_at = (uint8_t)unit;
         }
         // Earlier rows of blocks whose unit grew, a row for 8 lanes.
         for (int j = p0; j < p1; j = start_from(j + 1)) {
-            const uint32_t was = s_old[kv][j - p0], had = was >> 8, now = unit_of(s_top[kv][j - p0]);
-            if (kr >= (int)had || (was & 0xff) >= now) continue;
+            const uint32_t was = s_old[half][j - p0], had = was >> 8, now = unit_of(s_top[half][j - p0]);
+            if (ar >= (int)had || (was & 0xff) >= now) continue;
             const int s = s_slot[j], pg = s >> a.page_shift, ip = s & ((1 << a.page_shift) - 1);
-            uint8_t* at = a.base + (int64_t)pg * a.page_stride + kv * a.kv_stride + kvh * a.head_stride +
-                          (int64_t)((ip & ~(kRun - 1)) + kr) * kHeadDim + d;
+            uint8_t* at = a.base + (int64_t)pg * a.page_stride + half * a.kv_stride + kvh * a.head_stride +
+                          (int64_t)((ip & ~(kRun - 1)) + ar) * kHeadDim + d;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 uint2* x = (uint2*)(at + i * (kHeadDim / 2));
