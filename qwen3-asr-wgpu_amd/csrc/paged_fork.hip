@@ -84,7 +84,7 @@ __global__ __launch_bounds__(kPagedMaxRequests) void fork_rows_kernel(ForkArgs a
     if (lane == 0) s_wave[i >> 6] = __popcll(votes);
     __syncthreads();
     int rank = __popcll(votes & ((1ull << lane) - 1)), copies = 0;
-    for (int w = 0; w < kPagedMaxRequests / 64; ++w) {
+    for (int w = 0; w < (int)blockDim.x / 64; ++w) {
         rank += w < i >> 6 ? s_wave[w] : 0;
         copies += s_wave[w];
     }
@@ -156,31 +156,33 @@ __device__ __forceinline__ void copy_pages(const ForkArgs& a, int first, int ste
 
 // kForkColumns columns of the table.
 __device__ __forceinline__ void rewrite_columns(const ForkArgs& a, int block, int blocks, int* s_page) {
-    // s_page: [nreq][kForkColumns] pages listed now, -1: none that counts.
+    // s_page, s_more: [nreq][kForkColumns] pages listed now, -1: none that counts,
+    // and how many holders more (or, below zero, one less) they get.
     constexpr int C = kForkColumns, kWords = kPagedMaxRequests / 32;
     __shared__ uint32_t s_gone[C][kWords];  // requests whose page of the column nobody holds any more
     __shared__ uint32_t s_many[C][kWords];  // whose page's count changes
     __shared__ int s_first[C + 1];
+    __shared__ int s_upto[kThreads], s_wave[kThreads / 64];
     __shared__ int s_arrived;
-    const int tid = threadIdx.x, n = a.nreq * C, k0 = block * C;
+    const int tid = threadIdx.x, n = a.nreq * C, k0 = block * C, words = (a.nreq + 31) / 32;
+    int* s_more = s_page + n;
     for (int x = tid; x < C * kWords; x += kThreads) s_gone[x / kWords][x % kWords] = s_many[x / kWords][x % kWords] = 0;
+    const int ok = a.w->ok;
     for (int x = tid; x < n; x += kThreads) {
         const int j = x / C, k = k0 + x % C;
-        int page = -1;
-        if (k < a.rows[j].used) page = a.table[(int64_t)j * a.stride + k];
+        const ForkRow r = a.rows[j];  // (of an earlier call if this one is not carried out)
+        int page = a.table[(int64_t)j * a.stride + min(k, a.stride - 1)];
+        page = k < r.used ? page : -1;
         s_page[x] = page;
+        s_more[x] = (uint32_t)page >= (uint32_t)a.pages ? 0 : k < r.whole ? r.more : r.more_last;
     }
+    if (!ok) return;
     __syncthreads();
     // Holders.  Whose page has no other loses its last one; counts of pages with
     // several, and of those that get more, change behind the barrier.
-    auto more_of = [&](int x) {
-        if ((uint32_t)s_page[x] >= (uint32_t)a.pages) return 0;
-        const ForkRow& r = a.rows[x / C];
-        return k0 + x % C < r.whole ? r.more : r.more_last;
-    };
     auto set = [&](uint32_t (*bits)[kWords], int j, int c) { atomicOr(&bits[c][j >> 5], 1u << (j & 31)); };
     for (int x = tid; x < n; x += kThreads) {
-        const int more = more_of(x);
+        const int more = s_more[x];
         if (more < 0 && a.shared[s_page[x]] <= 0)
             set(s_gone, x / C, x % C);
         else if (more)
@@ -189,7 +191,7 @@ __device__ __forceinline__ void rewrite_columns(const ForkArgs& a, int block, in
     __syncthreads();
     for (int x = tid; x < n; x += kThreads) {
         if (!(s_many[x % C][x / C >> 5] >> (x / C & 31) & 1)) continue;
-        const int more = more_of(x);
+        const int more = s_more[x];
         int* count = a.shared + s_page[x];
         const int was = __hip_atomic_fetch_add(count, more, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         if (more < 0 && was == 0) {  // the last holder
@@ -203,7 +205,7 @@ __device__ __forceinline__ void rewrite_columns(const ForkArgs& a, int block, in
     // Their pages by column, then by request.
     if (tid < C) {
         int sum = 0;
-        for (int w = 0; w < kWords; ++w) sum += __popc(s_gone[tid][w]);
+        for (int w = 0; w < words; ++w) sum += __popc(s_gone[tid][w]);
         s_first[tid + 1] = sum;
     }
     __syncthreads();
@@ -238,18 +240,32 @@ __device__ __forceinline__ void rewrite_columns(const ForkArgs& a, int block, in
     if (!s_arrived) return;
     const int head = a.w->head, free = a.w->free, copies = a.w->copies;
     int pushed = 0;
-    for (int b0 = 0; b0 < blocks; b0 += kThreads) {  // (one turn for tables of up to 4096 pages)
+    for (int b0 = 0; b0 < blocks; b0 += kThreads) {  // (one turn for tables of up to 1024 pages)
         const int m = b0 + tid < blocks ? __hip_atomic_load(a.n_gone + b0 + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
-        __syncthreads();
-        s_page[tid] = m;
-        __syncthreads();
-        for (int b = 0; b < min(kThreads, blocks - b0); ++b) {
-            const int* from = a.gone + (int64_t)(b0 + b) * a.nreq * C;
-            for (int x = tid; x < s_page[b] && free + pushed + x < a.pages; x += kThreads)  // (a page given back twice)
-                a.ring[wrap(head + free + pushed + x, a.pages)] =
-                    __hip_atomic_load(from + x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            pushed += s_page[b];
+        // How many the blocks up to each have, then a page a thread: its block is
+        // the first that has more up to it than come before the page.
+        int upto = m;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int y = __shfl_up(upto, d);
+            upto += (tid & 63) >= d ? y : 0;
         }
+        __syncthreads();
+        if ((tid & 63) == 63) s_wave[tid >> 6] = upto;
+        __syncthreads();
+        for (int w = 0; w < tid >> 6; ++w) upto += s_wave[w];
+        s_upto[tid] = upto;
+        __syncthreads();
+        const int all = s_upto[kThreads - 1];
+        for (int x = tid; x < all && free + pushed + x < a.pages; x += kThreads) {  // (a page given back twice)
+            int b = 0;
+#pragma unroll
+            for (int d = kThreads / 2; d; d /= 2) b += s_upto[b + d - 1] <= x ? d : 0;
+            const int at = x - (b ? s_upto[b - 1] : 0);
+            a.ring[wrap(head + free + pushed + x, a.pages)] = __hip_atomic_load(
+                a.gone + (int64_t)(b0 + b) * a.nreq * C + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        pushed += all;
     }
     if (tid == 0) {
         a.cursor[0] = wrap(head + copies, a.pages);
@@ -260,10 +276,9 @@ __device__ __forceinline__ void rewrite_columns(const ForkArgs& a, int block, in
 
 __global__ __launch_bounds__(kThreads) void fork_pages_kernel(ForkArgs a, int blocks, int parts) {
     extern __shared__ int s_page[];
-    if (!a.w->ok) return;
     if ((int)blockIdx.x < blocks)
         rewrite_columns(a, blockIdx.x, blocks, s_page);
-    else
+    else if (a.w->ok)
         copy_pages(a, blockIdx.x - blocks, gridDim.x - blocks, parts);
 }
 
@@ -271,7 +286,7 @@ __global__ __launch_bounds__(kThreads) void fork_pages_kernel(ForkArgs a, int bl
 
 hipError_t launch_paged_fork(const ForkArgs& a, int cus, hipStream_t stream) {
     if (a.nreq < 1 || a.nreq > kPagedMaxRequests || a.stride < 1) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(fork_rows_kernel, dim3(1), dim3(kPagedMaxRequests), 0, stream, a);
+    hipLaunchKernelGGL(fork_rows_kernel, dim3(1), dim3((a.nreq + 63) / 64 * 64), 0, stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int blocks = (a.stride + kForkColumns - 1) / kForkColumns;
@@ -280,7 +295,7 @@ hipError_t launch_paged_fork(const ForkArgs& a, int cus, hipStream_t stream) {
     const int64_t units = (int64_t)parts * a.nreq;
     const int64_t copiers = units < 8 * cus ? units : 8 * cus;
     hipLaunchKernelGGL(fork_pages_kernel, dim3((unsigned)(blocks + copiers)), dim3(kThreads),
-                       (size_t)(a.nreq > kThreads / kForkColumns ? a.nreq : kThreads / kForkColumns) * kForkColumns * 4, stream, a, blocks, parts);
+                       (size_t)a.nreq * kForkColumns * 8, stream, a, blocks, parts);
     return hipGetLastError();
 }
 

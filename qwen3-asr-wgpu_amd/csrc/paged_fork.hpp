@@ -7,7 +7,7 @@
 
 namespace qasr {
 
-constexpr int kForkColumns = 16;  // table columns of a workgroup: 64 bytes of a row
+constexpr int kForkColumns = 2;  // table columns of a workgroup
 
 // What the first kernel finds out about each request, for the second.
 struct ForkRow {
