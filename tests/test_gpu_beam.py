@@ -238,6 +238,59 @@ def test_replayed_on_another_stream(gpu):
     s.close()
 
 
+def test_the_largest_selection(gpu):
+    """1024 groups of 32 beams, 32 candidates each, most of them equal."""
+    groups, width, vocab, k = 1024, 32, 33, 32
+    s = Sel(groups, width, vocab, k)
+    logits = torch.randint(-2, 3, (groups * width, vocab), device="cuda", generator=gen(1)).float()
+    scores = -torch.randint(0, 4, (groups * width,), device="cuda", generator=gen(2)).float()
+    got = [t.view(groups, k) for t in s.run(logits, scores)]
+    x = logits.double()
+    p = (x - x.logsumexp(-1, keepdim=True) + scores.double()[:, None]).view(groups, width * vocab).cpu()
+    at = (got[0] % width).long() * vocab + got[1]
+    bound = score_bound(vocab, 12.0)
+    # The k best, whatever stands between equal ones of different rows, whose
+    # sums may differ in their last bits; each once, best first.
+    assert float((p.gather(1, at) - p.topk(k)[0]).abs().max()) <= 2 * bound
+    assert float((p.gather(1, at) - got[2]).abs().max()) <= bound
+    assert bool((at.sort(-1)[0].diff() > 0).all()) and bool((got[2].diff() <= 0).all())
+    s.close()
+
+
+def test_two_at_once_and_two_graphs_of_one_workspace(gpu):
+    """Selections on two streams, each with its own workspace; then two graphs of
+    one workspace, replayed in turn with an eager call between them."""
+    vocab, width = 151936, 4
+    a, b = Sel(3, width, vocab, 4), Sel(20, width, 5000, 9)
+    x = peaked(1, 3 * width, vocab), peaked(2, 20 * width, 5000)
+    sc = [-torch.rand(t.shape[0], device="cuda", generator=gen(3)) for t in x]
+    want = a.run(x[0], sc[0]), b.run(x[1], sc[1])
+    outs = [[torch.zeros(n, dtype=t, device="cuda") for t in (torch.int32, torch.int32, torch.float32)] for n in (12, 180)]
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, s in enumerate((a, b)):
+            Q.beam_select(s.ctx, s.sel, x[i], sc[i], *outs[i], stream=streams[i].cuda_stream)
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert all(torch.equal(t.cpu(), u) for t, u in zip(o, w))
+    graphs = []
+    for rows in (slice(0, 4), slice(0, 12)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            Q.beam_select(a.ctx, a.sel, x[0][rows], sc[0][rows], *outs[0])
+        graphs.append(g)
+    for _ in range(3):
+        graphs[0].replay()
+        assert all(torch.equal(t[:4].cpu(), u[:4]) for t, u in zip(outs[0], want[0]))
+        a.run(x[0][:8], sc[0][:8])
+        graphs[1].replay()
+        assert all(torch.equal(t.cpu(), u) for t, u in zip(outs[0], want[0]))
+    del g, graphs
+    a.close()
+    b.close()
+
+
 def test_logits_past_32_bits(gpu):
     """Rows whose offsets pass 2^32 bytes and 2^31 values."""
     vocab, rows = 1 << 20, 2600

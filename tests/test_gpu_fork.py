@@ -203,6 +203,60 @@ def test_on_another_stream_and_replayed(gpu):
     s.close()
 
 
+def test_the_largest_fork(gpu):
+    """1024 requests with tables of 700 pages: a prefix that all share, pages of
+    their own, most of them given up at once; then all."""
+    rnd = random.Random(5)
+    n, ps, width, pages = 1024, 16, 700, 40000
+    s = State(n, pages, ps, width, True, 1, 1)
+    s.grow(0, 16 * 600 + 5)
+    s.step([0] * n)
+    s.shuffle(rnd)
+    for i in range(n):
+        s.grow(i, rnd.randint(0, 300))
+    s.step([rnd.randrange(40) for _ in range(n)])
+    assert s.cursor[1] > 20000
+    s.step([-1] * n)
+    assert s.cursor[1] == pages and not any(s.shared)
+    s.close()
+
+
+def test_replayed_with_copies(gpu):
+    """A graph whose every replay shares, copies and gives back, of 8-bit pages,
+    with eager work between the replays."""
+    rnd = random.Random(9)
+    s = State(6, 200, 32, 12, True, 2, 2)
+    for i in range(6):
+        s.grow(i, 40 + 11 * i)
+    d = [i32(x) for x in (s.lens, s.table, s.shared, s.ring, s.cursor)]
+    parent = i32(list(range(6)))
+    pool = s.p.pool
+    Q.paged_fork(s.p.ctx, s.fork, d[0], parent, *d[1:])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        Q.paged_fork(s.p.ctx, s.fork, d[0], parent, *d[1:])
+    for _ in range(5):
+        parents = [rnd.randrange(6) for _ in range(6)]
+        parent.copy_(i32(parents))
+        want, units = bits(pool.tensor()).clone(), bits(pool.scales()).clone()
+        graph.replay()
+        torch.cuda.synchronize()
+        _, copies = B.fork(s.lens, parents, s.table, s.shared, s.ring, s.cursor, s.pages, s.ps)
+        for a, b, r in copies:
+            want[:, b, :, :, :r] = want[:, a, :, :, :r]
+            units[:, b, :, :, :-(-r // 16)] = units[:, a, :, :, :-(-r // 16)]
+        for got, w in zip(d, (s.lens, s.table, s.shared, s.ring, s.cursor)):
+            assert got.tolist() == w
+        assert torch.equal(bits(pool.tensor()), want) and torch.equal(bits(pool.scales()), units)
+        for i in range(6):  # the requests go on, each by its own rows
+            s.grow(i, rnd.randint(0, 9))
+        for t, v in zip(d, (s.lens, s.table, s.shared, s.ring, s.cursor)):
+            t.copy_(i32(v))
+    del graph
+    s.close()
+
+
 def test_fork_refuses(gpu):
     p = Paged(20, 16, 4, 8, rope=False)
     for bad in ((0, 4), (1025, 4), (4, 0), (4, (1 << 24) + 1)):
