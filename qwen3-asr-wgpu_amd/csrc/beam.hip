@@ -205,7 +205,7 @@ __device__ __forceinline__ void merge(const BeamArgs& a, int group, int lists, f
                                       double* s_score) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), k = a.k;
     const int tiles = (a.vocab + kBeamTile - 1) / kBeamTile, n = a.width * k;
-    int* s_token = (int*)(s_score + n);
+    int *s_token = (int*)(s_score + n), *s_rank = s_token + n;
     const uint64_t endeds = __ballot(ended);
     for (int b = wave; b < a.width; b += kBeamWaves) {
         const int row = group * a.width + b;
@@ -283,20 +283,29 @@ __device__ __forceinline__ void merge(const BeamArgs& a, int group, int lists, f
         if (lane < k) {
             s_score[b * k + lane] = mine;
             s_token[b * k + lane] = token;
+            s_rank[b * k + lane] = 0;
         }
     }
     __syncthreads();
     // Each candidate's rank: how many come before it; those that are none are the
-    // last.
-    for (int i = tid; i < n; i += kThreads) {
-        const double x = s_score[i];
+    // last.  64 candidates a wave, against a part of them all.
+    const int chunks = (n + 63) / 64, shares = max(1, kBeamWaves / chunks);
+    for (int u = wave; u < chunks * shares; u += kBeamWaves) {
+        const int chunk = u / shares, share = u - chunk * shares, i = chunk * 64 + lane;
+        const double x = s_score[min(i, n - 1)];
         int rank = 0;
 #pragma unroll 8
-        for (int j = 0; j < n; ++j) {
+        for (int j = share * n / shares; j < (share + 1) * n / shares; ++j) {
             const double y = s_score[j];
             rank += y > x || (y == x && j < i);
         }
+        if (i < n) atomicAdd(s_rank + i, rank);
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += kThreads) {
+        const int rank = s_rank[i];
         if (rank >= k) continue;
+        const double x = s_score[i];
         const bool none = x == (double)kNone;
         const int at = group * k + rank, b = i / k, token = s_token[i];
         a.parent[at] = none ? -1 : group * a.width + b;
@@ -308,7 +317,7 @@ __device__ __forceinline__ void merge(const BeamArgs& a, int group, int lists, f
 
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(6, 8))) void beam_select_kernel(BeamArgs a, int parts) {
     __shared__ Shared sh;
-    extern __shared__ double s_score[];  // [width][k], and as many tokens
+    extern __shared__ double s_score[];  // [width][k], and as many tokens and ranks
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), k = a.k;
     const int row = __builtin_amdgcn_readfirstlane(blockIdx.x / parts), part = blockIdx.x - row * parts;
     const int group = __builtin_amdgcn_readfirstlane(row / a.width);
@@ -379,7 +388,7 @@ hipError_t launch_beam_select(const BeamArgs& a, int cus, hipStream_t stream) {
     const int64_t turns = ((int64_t)rows * tiles + 16 * cus - 1) / (16 * cus);  // tiles of a wave
     int64_t parts = (tiles + turns * kBeamWaves - 1) / (turns * kBeamWaves);
     parts = parts < kBeamMaxParts ? parts : kBeamMaxParts;
-    hipLaunchKernelGGL(beam_select_kernel, dim3((unsigned)(rows * parts)), dim3(kThreads), (size_t)a.width * a.k * 12,
+    hipLaunchKernelGGL(beam_select_kernel, dim3((unsigned)(rows * parts)), dim3(kThreads), (size_t)a.width * a.k * 16,
                        stream, a, (int)parts);
     return hipGetLastError();
 }
