@@ -115,8 +115,11 @@ __global__ __launch_bounds__(kPagedMaxRequests) void fork_rows_kernel(ForkArgs a
     }
 }
 
-// Rows of K and V, 16 bytes a thread: unit (copy, part of 1024 of them).
+// Rows of K and V, 16 bytes a thread: unit (copy, part of 1024 of them).  Past the
+// caches, as nothing here reads them again: 1.0 GB of 16 x 5 beams on pages of 256
+// rows 283 -> 175 us (5.8 TB/s), 104 MB on pages of 64 36 -> 26.
 constexpr int kCopyVectors = 1024;
+typedef unsigned int Vector __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void copy_pages(const ForkArgs& a, int first, int step, int parts) {
     const int units = a.w->copies * parts;
     for (int u = first; u < units; u += step) {
@@ -125,7 +128,7 @@ __device__ __forceinline__ void copy_pages(const ForkArgs& a, int first, int ste
         const int n = p.rows * (a.row_bytes / 16);  // vectors of a head
         const int64_t head_bytes = (int64_t)a.row_bytes << a.page_shift;
         const int all = n * a.heads * a.layers;
-        uint4 x[kCopyVectors / kThreads];
+        Vector x[kCopyVectors / kThreads];
         int64_t to[kCopyVectors / kThreads];
 #pragma unroll
         for (int k = 0; k < kCopyVectors / kThreads; ++k) {
@@ -134,13 +137,13 @@ __device__ __forceinline__ void copy_pages(const ForkArgs& a, int first, int ste
             if (v < all) {
                 const int h = v / n, at = v - h * n, layer = h / a.heads, head = h - layer * a.heads;
                 const int64_t in = layer * a.layer_bytes + head * head_bytes + at * 16ll;
-                x[k] = *(const uint4*)(a.base + in + p.from * a.page_bytes);
+                x[k] = __builtin_nontemporal_load((const Vector*)(a.base + in + p.from * a.page_bytes));
                 to[k] = in + p.to * a.page_bytes;
             }
         }
 #pragma unroll
         for (int k = 0; k < kCopyVectors / kThreads; ++k)
-            if (to[k] >= 0) *(uint4*)(a.base + to[k]) = x[k];
+            if (to[k] >= 0) __builtin_nontemporal_store(x[k], (Vector*)(a.base + to[k]));
         if (part == 0 && a.scales && p.rows) {  // units of the copied rows' blocks
             const int blocks = (1 << a.page_shift) / kPagedScaleRows, held = (p.rows + kPagedScaleRows - 1) / kPagedScaleRows;
             for (int s = threadIdx.x; s < a.layers * a.page_scales; s += kThreads) {
