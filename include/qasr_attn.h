@@ -327,7 +327,8 @@ int qasr_paged_plan_get_info(const qasr_paged_plan* plan, qasr_paged_plan_info* 
  * none of them stores rows in it: a request's first new row goes into its last
  * page while that has room, so a shared prefix is whole pages.  A page that two
  * ended requests give back is twice in the ring: end all but the last of its
- * requests with their shared entries set to -1. */
+ * requests with their shared entries set to -1, or end requests that share pages
+ * with qasr_paged_fork, which counts. */
 int qasr_paged_plan_build(qasr_ctx* ctx, qasr_paged_plan* plan, int nreq, const int32_t* len_dev,
                           const int32_t* rows_dev, int32_t* table_dev, int table_stride,
                           int32_t* ring_dev, const int32_t* cursor_dev, void* stream);
@@ -427,7 +428,7 @@ void qasr_beam_destroy(qasr_beam* beam);
  * log(sum over u of exp(logits[r][u])), logits row r at logits_dev +
  * r*logits_stride (floats; rows need not be aligned).  A beam that has ended
  * (done_dev[r] not 0; done_dev may be NULL) has one candidate, (r, eos) with
- * scores_dev[r].  Equal scores go to the lower beam, then to the lower token.
+ * scores_dev[r], also where eos is -1.  Equal scores go to the lower beam, then to the lower token.
  * Place i of group g in the outputs, all [groups][k]: parent_dev the row r,
  * token_dev t, out_scores_dev the score, out_done_dev (or NULL) 1 if the beam has
  * ended or t is eos (-1: no token ends a beam), else 0.
@@ -438,8 +439,9 @@ void qasr_beam_destroy(qasr_beam* beam);
  * parent and token -1, score -inf, done 0.  Rows that have no logits to offer
  * are not read.
  *
- * Sums are formed in f32 over pieces of 2048 tokens, everything behind them in f64; scores are compared in f64 and rounded once.  A group's results
- * are a function of its own rows.  Outputs may be the inputs' arrays (out_scores
+ * Sums are formed in f32 over pieces of 2048 tokens, everything behind them in
+ * f64; scores are compared in f64 and rounded once (a difference of logits that no
+ * f32 holds becomes -inf).  A group's results are a function of its own rows.  Outputs may be the inputs' arrays (out_scores
  * scores, out_done done) if k is width; they overlap nothing else.  Does not
  * allocate or synchronise, may be captured; calls that share the workspace are
  * ordered on one stream. */

@@ -8,20 +8,30 @@
 // One pass over the logits.  A wave holds a tile of 2048 of a row's in registers:
 // their maximum, the sum of exponentials against it (published, a pair a tile),
 // and what of them is among the wave's k best so far.  A tile whose largest is
-// below the k-th best has nothing; else the k-th largest of the lanes' maxima,
-// found by bisection with ballots, is a border that at least k values reach, and
-// the few that reach both go to the wave's list in LDS, which is ranked by
-// comparing each with all and cut to k.  A key is the logit's order-preserving
-// bits over the complement of its token, unique, so ties cost nothing and no
-// list can be longer than k + k * 32.  A workgroup's four lists merge at its end.
-// Tiles and sums are the same whatever the number of workgroups a row has, which
-// follows the number of rows.
+// no better than the k-th best has nothing.  Else a border is searched, by
+// bisection with ballots, that at least k of the lanes' maxima reach and few
+// more; the values that reach it and the k-th best so far go to the wave's list
+// in LDS, in which each finds its rank by comparing itself with all.  A key is the
+// logit's order-preserving bits over the complement of its token, unique, so ties
+// cost nothing.  Tiles and sums are the same whatever the number of workgroups a
+// row has, which follows the number of rows: waves get one tile more at a time
+// once there are more than 16 a CU.
 //
 // The last workgroup of a group to arrive (ticket) merges: a wave a beam adds up
-// the tiles' sums, in order and in 64 bits, and takes the k best of the
-// workgroups' lists in the same way as of a tile; then each of the beams'
-// candidates finds its rank by bisection in the other beams' lists, in 64-bit
-// scores.  Results are a function of the group's rows alone.
+// the tiles' sums, in order and in 64 bits, and takes the k best of the waves'
+// lists in the same way as of a tile; then each of the beams' candidates counts
+// those that come before it, in 64-bit scores.  Results are a function of the
+// group's rows alone.
+//
+// What bounds it, us a call of 151936 tokens (bytes at the 5.1 TB/s of a large
+// copy in brackets): 1 x 5 beams 9.8 (0.6) and 16 x 5 with 10 candidates 18.9
+// (9.5): a chain of launch 1.5, a tile 2.5-3 (loads 0.5, maximum and sum 0.6, border
+// 0.4, list 1), stores and ticket 2, the merge 4-5 (two trips to memory, list, ranks),
+// and behind it, for 16 x 5, the loads; 64 x 4 with 40 ended 30.0-30.6 (25.7): the loads, 4.4 TB/s.
+// Measured against this: workgroups of 4 waves 12.5 / 23.0 / 31.7; keys ranked one
+// after the other by readlane 10.6 / 21.1 / 30.5; the next tile's loads ahead of a
+// tile (4 waves a SIMD instead of 6) 10.0 / 21.0 / 32.1; loads past the caches 9.8 /
+// 19.5 / 30.0; 8 or 24 tiles a CU and turn instead of 16: 24.4 and 22.3 for 16 x 5.
 #include "beam.hpp"
 
 namespace qasr {
@@ -83,7 +93,7 @@ __device__ __forceinline__ float wave_sum(float x) {
 // A border that at least k of the lanes' values reach, by their ordered bits, of
 // which `top` are the largest, and few more than k, unless several are equal to
 // the k-th; 0 if fewer than k are not 0.
-constexpr int kSpare = 3;  // (a value more is cheaper to rank than another step of the bisection)
+constexpr int kSpare = 3;  // (ranking some values more is cheaper than to go on; 8: the same within 0.2 us)
 __device__ __forceinline__ uint32_t border_of(uint32_t mine, uint32_t top, int k) {
     uint32_t lo = 0, hi = top + 1;  // at least k reach lo, fewer hi (none has all bits set)
     int n = __popcll(__ballot(mine != 0));
@@ -385,6 +395,7 @@ hipError_t launch_beam_select(const BeamArgs& a, int cus, hipStream_t stream) {
         a.k > kBeamMaxK || a.vocab < 1 || a.vocab > kBeamMaxVocab)
         return hipErrorInvalidValue;
     const int rows = a.groups * a.width, tiles = beam_tiles(a.vocab);
+    // (Two workgroups of the three that a CU holds: 8 and 24 waves a CU were slower.)
     const int64_t turns = ((int64_t)rows * tiles + 16 * cus - 1) / (16 * cus);  // tiles of a wave
     int64_t parts = (tiles + turns * kBeamWaves - 1) / (turns * kBeamWaves);
     parts = parts < kBeamMaxParts ? parts : kBeamMaxParts;

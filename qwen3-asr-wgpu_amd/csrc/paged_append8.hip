@@ -18,11 +18,20 @@
 //
 // A run: rows of a step that follow each other in one block.  A workgroup
 // takes the runs that start in 16 rows of the step, for one kv head and its two q
-// heads, at most 16 rows of whole runs at a time: 256 threads hold 8 dims and
-// their rotation partners of a row each, once for Q and once for K or V.  The
-// sums of squares are serial (one lane a head and row, as the reference adds),
-// the largest values meet in LDS.  Units are powers of two so that a growing
-// unit costs the earlier rows nothing, and the conversions are instructions.
+// heads, at most 16 rows of whole runs at a time: a thread of 256 holds 8 dims and
+// their rotation partners of a row, of one of the q heads and of K or V, so that
+// cos and sin are read once for both.  The sums of squares are serial (one lane a
+// head and row, as the reference adds), the largest values meet in LDS.  Units are
+// powers of two so that a growing unit costs the earlier rows nothing, and the
+// conversions are instructions.
+//
+// What bounds it, us a layer of 16 q and 8 kv heads: 1 row 4.4, the chain: launch,
+// places, cos / sin and the blocks' units, the sums, three barriers (stage (a) into
+// f16 pages, without units, 3.1); 5185 rows of 16 prompts 20.0 (74 MB, 14.6 at the
+// rate of a large copy): 115 registers, 4 workgroups a CU.  Q and K or V in
+// separate threads with their own cos and sin and all of a head read ahead of its
+// sum took 179, 2 workgroups: 27.7 and 4.7.  5 a CU spill (32); loads of the rows
+// past the caches 21.6.
 #include "norm_rope.hpp"
 #include "paged.hpp"
 

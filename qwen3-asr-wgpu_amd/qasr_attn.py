@@ -394,9 +394,9 @@ class KVPool:
 
 class _DeviceView:
     """__cuda_array_interface__ over library-owned device memory (f16, or
-    int32 with typestr "<i4", bytes with "|u1").  A torch tensor made of it, and every view of
-    that tensor, holds on to it and so to `owner`, the object that frees the
-    memory."""
+    int32 with typestr "<i4", bytes with "|u1").  A torch tensor made of it, and
+    every view of that tensor, holds on to it and so to `owner`, the object that
+    frees the memory."""
 
     def __init__(self, ptr: int, nbytes: int, device: int, typestr: str = "<f2", owner=None):
         self.owner = owner
