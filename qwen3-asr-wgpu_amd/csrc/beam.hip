@@ -225,7 +225,7 @@ __device__ __forceinline__ void merge(const BeamArgs& a, int group, int lists, f
         if (!dead(s_b) && (endeds >> b & 1)) {
             mine = lane == 0 ? (double)s_b : mine;
         } else if (!dead(s_b)) {
-            const uint64_t* keys = a.keys + (int64_t)row * (kBeamMaxParts * kBeamWaves) * k;
+            const uint64_t* keys = a.keys + (int64_t)row * lists * k;
             const uint64_t* sums = a.sums + (int64_t)row * tiles;
             Best best;
             Keys x;
@@ -376,7 +376,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(6, 8))
             if (!(sum == sum) || M == kNone || (best.kth != 0 && M <= logit_of(best.kth))) continue;  // (of equal ones the earlier tile's)
             take_tile(best, v, top, M, t * kBeamTile + lane * 4, k, lane, sh.list[wave]);
         }
-        uint64_t* keys = a.keys + ((int64_t)row * (kBeamMaxParts * kBeamWaves) + part * kBeamWaves + wave) * k;
+        uint64_t* keys = a.keys + (((int64_t)row * parts + part) * kBeamWaves + wave) * k;
         if (lane < k) store_dev64(keys + lane, lane < best.held ? sh.list[wave][lane] : 0);
     }
     stores_done_barrier();
@@ -394,13 +394,9 @@ hipError_t launch_beam_select(const BeamArgs& a, int cus, hipStream_t stream) {
     if (a.groups < 1 || a.groups > kBeamMaxGroups || a.width < 1 || a.width > kBeamMaxWidth || a.k < 1 ||
         a.k > kBeamMaxK || a.vocab < 1 || a.vocab > kBeamMaxVocab)
         return hipErrorInvalidValue;
-    const int rows = a.groups * a.width, tiles = beam_tiles(a.vocab);
-    // (Two workgroups of the three that a CU holds: 8 and 24 waves a CU were slower.)
-    const int64_t turns = ((int64_t)rows * tiles + 16 * cus - 1) / (16 * cus);  // tiles of a wave
-    int64_t parts = (tiles + turns * kBeamWaves - 1) / (turns * kBeamWaves);
-    parts = parts < kBeamMaxParts ? parts : kBeamMaxParts;
+    const int rows = a.groups * a.width, parts = beam_parts(rows, a.vocab, cus);
     hipLaunchKernelGGL(beam_select_kernel, dim3((unsigned)(rows * parts)), dim3(kThreads), (size_t)a.width * a.k * 16,
-                       stream, a, (int)parts);
+                       stream, a, parts);
     return hipGetLastError();
 }
 

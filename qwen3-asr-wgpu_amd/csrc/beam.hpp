@@ -15,6 +15,17 @@ constexpr int kBeamMaxParts = 32;    // workgroups of a row
 constexpr int kBeamCounterStep = 32;  // words: a line each
 
 inline int beam_tiles(int vocab) { return (vocab + kBeamTile - 1) / kBeamTile; }
+// Workgroups of a row.  A wave gets one tile more at a time once there are more
+// than 16 tiles a CU.  (Two workgroups of the three that a CU holds: 8 and 24 waves
+// a CU were slower.)
+inline int beam_parts(int rows, int vocab, int cus) {
+    const int64_t tiles = beam_tiles(vocab), turns = (rows * tiles + 16 * cus - 1) / (16 * cus);
+    const int64_t parts = (tiles + turns * kBeamWaves - 1) / (turns * kBeamWaves);
+    return (int)(parts < kBeamMaxParts ? parts : kBeamMaxParts);
+}
+// Of up to `rows` rows together: a row's parts are less than its share of
+// 16 cus / kBeamWaves, and one.
+inline int64_t beam_most_parts(int64_t rows, int cus) { return rows + 16 / kBeamWaves * cus; }
 
 struct BeamArgs {
     const float* logits;  // [groups * width] rows, `stride` apart
@@ -26,7 +37,7 @@ struct BeamArgs {
     int32_t* token;
     float* out_scores;
     int32_t* out_done;  // or NULL
-    uint64_t* keys;     // [rows][kBeamMaxParts * kBeamWaves][k], best first, 0: none
+    uint64_t* keys;     // [rows][parts][kBeamWaves][k], best first, 0: none
     uint64_t* sums;     // [rows][tiles]: largest logit; sum of exp(logit - it), NaN: nothing of the row counts
     uint32_t* arrived;  // [groups], a line each, zero at rest
 };

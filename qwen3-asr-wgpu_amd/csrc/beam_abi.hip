@@ -56,7 +56,7 @@ int qasr_beam_create(qasr_ctx* ctx, int max_groups, int width, int vocab, int k,
     const size_t rows = (size_t)max_groups * width;
     const size_t o_sums = (size_t)max_groups * qasr::kBeamCounterStep * 4;
     const size_t o_keys = o_sums + rows * qasr::beam_tiles(vocab) * 8;
-    b->bytes = o_keys + rows * qasr::kBeamMaxParts * qasr::kBeamWaves * k * 8;
+    b->bytes = o_keys + (size_t)qasr::beam_most_parts(rows, ctx->cus) * qasr::kBeamWaves * k * 8;
     DeviceScope ds(ctx->device);
     hipError_t e = ds.err;
     if (e == hipSuccess) e = hipMalloc(&b->mem, b->bytes);

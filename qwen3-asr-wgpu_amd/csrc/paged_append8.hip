@@ -27,7 +27,9 @@
 //
 // What bounds it, us a layer of 16 q and 8 kv heads: 1 row 4.4, the chain: launch,
 // places, cos / sin and the blocks' units, the sums, three barriers (stage (a) into
-// f16 pages, without units, 3.1); 5185 rows of 16 prompts 20.0 (74 MB, 14.6 at the
+// f16 pages, without units, 3.1); 16 and 64 single rows 5.1 and 5.4 (6.5 and 6.8 where
+// every run is looked at for rows to be rounded again, not those found by a
+// ballot); 5185 rows of 16 prompts 20.0 (74 MB, 14.6 at the
 // rate of a large copy): 115 registers, 4 workgroups a CU.  Q and K or V in
 // separate threads with their own cos and sin and all of a head read ahead of its
 // sum took 179, 2 workgroups: 27.7 and 4.7.  5 a CU spill (32); loads of the rows
@@ -223,17 +225,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(4))) v
             *(uint2*)(dst + kHeadDim / 2) = narrow8(k[1], unit_value(unit));
             if (start == row && w == 0) *unit_at = (uint8_t)unit;
         }
-        // Earlier rows of blocks whose unit grew, a row for 8 lanes.
-        for (int j = p0; j < p1; j = start_from(j + 1)) {
-            const uint32_t was = s_old[half][j - p0], had = was >> 8, now = unit_of(s_top[half][j - p0]);
-            if (ar >= (int)had || (was & 0xff) >= now) continue;
-            const int s = s_slot[j], pg = s >> a.page_shift, ip = s & ((1 << a.page_shift) - 1);
+        // Earlier rows of blocks whose unit grew, a row for 8 lanes.  Bit j, 16 + j: the run that starts at p0 + j, its K, V.
+        const uint32_t tops = s_top[(tid >> 4) & 1][tid & 15], olds = s_old[(tid >> 4) & 1][tid & 15];
+        const uint32_t grew = (uint32_t)__ballot((tid & 63) < 2 * kRun && p0 + (tid & 15) < p1 &&
+                                                 (starts >> (p0 + (tid & 15)) & 1) && (olds >> 8) != 0 &&
+                                                 (olds & 0xff) < unit_of(tops));
+        for (uint32_t todo = (grew | grew >> 16) & 0xffff; todo; todo &= todo - 1) {
+            const int j = __builtin_ctz(todo);
+            const uint32_t was = s_old[half][j];
+            if (!(grew >> (16 * half + j) & 1) || ar >= (int)(was >> 8)) continue;
+            const float from = unit_value(was & 0xff), to = unit_value(unit_of(s_top[half][j]));
+            const int s = s_slot[p0 + j], pg = s >> a.page_shift, ip = s & ((1 << a.page_shift) - 1);
             uint8_t* at = a.base + (int64_t)pg * a.page_stride + half * a.kv_stride + kvh * a.head_stride +
                           (int64_t)((ip & ~(kRun - 1)) + ar) * kHeadDim + d;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 uint2* x = (uint2*)(at + i * (kHeadDim / 2));
-                *x = narrow8(widen8(*x, unit_value(was & 0xff)), unit_value(now));
+                *x = narrow8(widen8(*x, from), to);
             }
         }
         __syncthreads();  // the LDS is used again
