@@ -30,7 +30,7 @@
 // f16 pages, without units, 3.1); 16 and 64 single rows 5.1 and 5.4 (6.5 and 6.8 where
 // every run is looked at for rows to be rounded again, not those found by a
 // ballot); 5185 rows of 16 prompts 20.0 (74 MB, 14.6 at the
-// rate of a large copy): 115 registers, 4 workgroups a CU.  Q and K or V in
+// rate of a large copy): 118 registers, 4 workgroups a CU.  Q and K or V in
 // separate threads with their own cos and sin and all of a head read ahead of its
 // sum took 179, 2 workgroups: 27.7 and 4.7.  5 a CU spill (32); loads of the rows
 // past the caches 21.6.

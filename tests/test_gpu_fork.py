@@ -221,6 +221,24 @@ def test_the_largest_fork(gpu):
     s.close()
 
 
+def test_copies_past_32_bits(gpu):
+    """Pages whose offsets pass 2^32 bytes."""
+    rnd = random.Random(11)
+    s = State(4, 9000, 256, 4, True, 1, 8)
+    for _ in range(3):
+        s.shuffle(rnd)
+        s.cursor[1] = 9000 - sum(-(-c // 256) for c in s.lens)
+        far = sorted((s.ring[(s.cursor[0] + j) % 9000] for j in range(s.cursor[1])), reverse=True)
+        for j, page in enumerate(far):
+            s.ring[(s.cursor[0] + j) % 9000] = page
+        for i in range(4):
+            s.grow(i, rnd.randint(1, 200))
+        status, copies = s.step([1, 1, 2, 2])
+        assert not any(status) and copies and min(to for _, to, _ in copies) * 2 * 8 * 256 * HD > 1 << 32
+        s.step([0, -1, 2, -1])
+    s.close()
+
+
 def test_replayed_with_copies(gpu):
     """A graph whose every replay shares, copies and gives back, of 8-bit pages,
     with eager work between the replays."""

@@ -338,6 +338,81 @@ def test_attn_ignores_what_lies_behind_the_keys(gpu, batch):
 
 # ---- together ---------------------------------------------------------------
 
+def test_replayed_token_after_token(gpu):
+    """A graph of a step (plan, stage (a), attention, two layers), captured on a
+    stream of its own, that moves on by itself, with eager work between the
+    replays: the same bits as the same steps without a graph."""
+    ps, steps = 16, 20  # past the end of blocks and pages
+    rnd = random.Random(3)
+    lens = [5, 15, 16, 60]
+    out = []
+    for captured in (False, True):
+        p = Paged8(40, ps, 4, 4, layers=2)
+        fill(p.pool, 1)
+        table, _ = shuffled_table(rnd if not captured else random.Random(3), [-(-(c + steps) // ps) for c in lens], 40, 8)
+        table, cur, one = i32(table), i32(lens), i32([1] * 4)
+        gains = randn(2, 2, 2, HD, std=0.1) + 1
+        x = torch.zeros((2, 4, TOT), dtype=torch.float16, device="cuda")
+        q, o = (torch.zeros((2, 4, QDIM), dtype=torch.float16, device="cuda") for _ in range(2))
+
+        def step():
+            Q.paged_plan(p.ctx, p.plan, p.plan.lens, one, table)
+            for l in range(2):
+                Q.paged_append(p.ctx, p.plan, l, x[l], gains[l, 0], gains[l, 1], q[l])
+                Q.paged_attn(p.ctx, p.plan, l, table, q[l], o[l])
+
+        if captured:
+            p.plan.lens.copy_(cur)
+            step()
+            fill(p.pool, 1)
+            torch.cuda.synchronize()
+            graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+            with torch.cuda.graph(graph, stream=stream):
+                step()
+        p.plan.lens.copy_(cur)
+        got = []
+        for k in range(steps):
+            x.copy_(randn(100 + k, 2, 4, TOT) * 2.0 ** (k % 5 - 2))
+            graph.replay() if captured else step()
+            assert p.plan.status.tolist() == [0] * 4
+            got.append(o.clone())
+        out.append((got, bits(p.pool.tensor()).clone(), bits(p.pool.scales()).clone()))
+        torch.cuda.synchronize()
+        if captured:
+            del graph
+        p.close()
+    (a, pool_a, units_a), (b, pool_b, units_b) = out
+    assert all(same_bits(s, t) for s, t in zip(a, b))
+    assert torch.equal(pool_a, pool_b) and torch.equal(units_a, units_b)
+
+
+def test_pages_past_32_bits(gpu):
+    """Stage (a) into pages whose offsets pass 2^32 bytes, a prompt and single
+    rows, and attention over them."""
+    ps, pages = 256, 9000
+    batch = [(0, 700), (0, 1), (0, 40)]
+    p8, p16 = Paged8(pages, ps, 3, 800), Paged(pages, ps, 3, 800)
+    table = [[pages - 1, pages - 300, pages - 7], [pages - 2, -1, -1], [pages - 400, -1, -1]]
+    assert (pages - 400) * 2 * NKVH * ps * HD > 1 << 32
+    qkv, gains = new_rows(5, 741), randn(6, 2, HD, std=0.1) + 1
+    run_append(p8, p16, batch, table, qkv, gains)
+    used = torch.tensor([x for t in table for x in t if x >= 0], device="cuda")
+    x, u = p8.pool.tensor()[0, used], p8.pool.scales()[0, used]
+    exact = (x.float().view(*u.shape, 16, HD) * u.float()[..., None, None]).flatten(-3, -2).half()
+    near = p16.pool.tensor()[0, used]
+    # Half a step of a value, or of the block's unit.
+    bound = near.float().abs() * 2.0 ** -4 + (u.float() * 2.0 ** -10).repeat_interleave(16, -1)[..., None]
+    assert bool(((exact.float() - near.float()).abs() <= bound).all())
+    p16.pool.tensor()[0, used] = exact
+    q = randn(7, 741, QDIM)
+    a, b = torch.zeros_like(q), torch.zeros_like(q)
+    for p, out in ((p8, a), (p16, b)):
+        Q.paged_attn(p.ctx, p.plan, 0, i32(table), q, out)
+    assert same_bits(a, b) and bool((a[700] != 0).any())
+    p8.close()
+    p16.close()
+
+
 def test_steps_of_a_server(gpu):
     """Admission, chunks and decoding over both kinds of pool, with a ring: the
     outputs over 8 bits are the definition's over what the pages stand for,
