@@ -109,12 +109,13 @@ struct Item {
 // (stage (a) keeps units within 2^-15 .. 2^8), and a product takes the same numbers in the same
 // places as from f16 pages: the outputs have the same bits as over f16 pages
 // that hold these numbers.
-// us a layer, e4m3 (f16): 1 row of 512 keys 8.9 (8.1), of 8192 13.2 (14.4), 16 rows
-// of 400-2400 16.1 (23.9), a prompt of 420 10.3 (9.6), 512 rows at 7680 53 (53.5).
+// us a layer, e4m3 (f16): 1 row of 512 keys 8.6 (8.1), of 8192 12.9 (14.1), 16 rows
+// of 400-2400 15.9 (23.6), a prompt of 420 10.1 (9.8), 512 rows at 7680 53 (53.5).
 // Half the bytes where bytes count; else the chain of a tile is that of f16 with
 // the conversions in it, 64 a slice of 32 keys, each about 2.4 clocks of its SIMD.
-// Two slices of a wave in flight, for which e4m3 has the LDS: 17.4 for the 16 rows,
-// 9.2 for 1; copies that pass the caches by: 16.4, 9.1, 12.9 for 8192 keys.
+// Against 16.1 for the 16 rows and 8.9 for 1, before units were asked for ahead of
+// the copies: two slices of a wave in flight, for which e4m3 has the LDS, 17.4 and
+// 9.2; copies that pass the caches by 16.4 and 9.1.
 struct F16Pages {
     using T = f16;
     static constexpr int kElem = 2;
@@ -1115,14 +1116,14 @@ __device__ __forceinline__ void run_narrow(const PagedAttnArgs& a, const Item& i
                           slabs ? kSlice * 64 : 1024);
         }
     };
+    uint32_t scales = 0;  // (before the copies: they come back in order)
+    if constexpr (kScaled<P>) scales = load_scales(a, it, pg, it.tile0 * kNarrowTile + wave * kSlice);
     W w;
     init_wave(w, a, it, rin, h, lane);
     if (it.tile0 < it.tile1) {
         copy_slice(it.tile0, false);
         copy_slice(it.tile0, true);
     }
-    uint32_t scales = 0;
-    if constexpr (kScaled<P>) scales = load_scales(a, it, pg, it.tile0 * kNarrowTile + wave * kSlice);
     wait_q(w);
     asm volatile("" : "+v"(scales));
     for (int t = it.tile0; t < it.tile1; ++t) {
@@ -1218,12 +1219,12 @@ __device__ __forceinline__ void run_item(const PagedAttnArgs& a, const Item& it,
     };
     PageWave<P> w;
     init_wave(w, a, it, rin, h, lane);
+    uint32_t scales = 0;
+    if constexpr (kScaled<P>) scales = load_scales(a, it, pg, it.tile0 * kWideTile);
     if (it.tile0 < it.tile1) copy_tile(it.tile0);
     const int first_pos = it.pos0 + rw * 16;
     const int last_pos = it.pos0 + min(rw * 16 + 15, it.rows - 1);
     const bool live = rw * 16 < it.rows;
-    uint32_t scales = 0;
-    if constexpr (kScaled<P>) scales = load_scales(a, it, pg, it.tile0 * kWideTile);
     wait_q(w);
     asm volatile("" : "+v"(scales));
     for (int t = it.tile0; t < it.tile1; ++t) {
