@@ -487,8 +487,7 @@ def _plain_beam(st):
     p = torch.where(ended, torch.where(at_end, 0.0, -math.inf), p)
     p = (p + st["scores"].double()[:, None]).view(g, w * v)
     # (Equal scores, next to none here, go to the lowest place.)
-    best, at = (torch.sort(p, dim=-1, descending=True, stable=True) if w * v <= 4096
-                else p.topk(min(k, w * v)))
+    best, at = torch.sort(p, -1, descending=True, stable=True) if w * v <= 4096 else p.topk(min(k, w * v))
     best, at = best[:, :k], at[:, :k]
     some = best > -math.inf
     row = at // v + torch.arange(0, g * w, w, device="cuda")[:, None]
