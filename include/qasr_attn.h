@@ -400,7 +400,9 @@ int qasr_paged_fork_get_info(const qasr_paged_fork_ws* fork, qasr_paged_fork_inf
  * All or nothing: status_dev[i] is QASR_EINVAL for a parent outside [-1, nreq) or
  * a length that is negative or past the table, QASR_ENOMEM for the requests that
  * want a copy when the free pages do not reach for all of them; if any is not
- * QASR_OK, nothing is changed.
+ * QASR_OK, nothing is changed.  A cursor whose head is not a place of the ring, or
+ * with less than 0 or more than `pages` free, has no free page and cannot take any
+ * back: where no copy is wanted, every request is QASR_EINVAL.
  *
  * A page lies at the same place of every table that lists it (a shared prefix
  * does), and shared_dev holds the truth about all requests of the pool, those of

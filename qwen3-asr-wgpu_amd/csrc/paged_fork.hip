@@ -54,7 +54,10 @@ __global__ __launch_bounds__(kPagedMaxRequests) void fork_rows_kernel(ForkArgs a
     }
     head = a.cursor[0];
     free = a.cursor[1];
-    if (head < 0 || head >= a.pages || free < 0 || free > a.pages) head = free = 0;
+    // A cursor that is none: no page is free, and pages given back have no place,
+    // so a call that wants no copy is refused too.
+    const bool lost = head < 0 || head >= a.pages || free < 0 || free > a.pages;
+    if (lost) head = free = 0;
     const bool bad = mine && (parent < -1 || parent >= a.nreq || len < 0 ||
                               ((int64_t)len + ps - 1) >> a.page_shift > a.stride);
     const bool refused = __syncthreads_or(bad);
@@ -92,9 +95,9 @@ __global__ __launch_bounds__(kPagedMaxRequests) void fork_rows_kernel(ForkArgs a
         rank += w < i >> 6 ? s_wave[w] : 0;
         copies += s_wave[w];
     }
-    const bool ok = copies <= free;
+    const bool ok = copies <= free && !lost;
     if (mine) {
-        a.status[i] = !ok && copy ? kNoPage : kOk;
+        a.status[i] = ok ? kOk : copies == 0 ? kInvalid : copy ? kNoPage : kOk;
         ForkRow r;
         r.parent = parent;
         r.used = (len + ps - 1) >> a.page_shift;
