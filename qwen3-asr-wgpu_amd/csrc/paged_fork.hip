@@ -100,7 +100,7 @@ __global__ __launch_bounds__(kPagedMaxRequests) void fork_rows_kernel(ForkArgs a
         a.status[i] = ok ? kOk : copies == 0 ? kInvalid : copy ? kNoPage : kOk;
         ForkRow r;
         r.parent = parent;
-        r.used = (len + ps - 1) >> a.page_shift;
+        r.used = whole + (rest != 0);  // (len + ps - 1 passes 2^31 for the longest)
         r.whole = whole;
         r.more = s_sons[i] - 1;
         r.more_last = (s_sons[i] > 0 && alone ? 1 : 0) - 1;

@@ -43,3 +43,33 @@ def test_a_cursor_that_is_none_takes_no_pages_back(gpu, cursor):
     s.step([-1] * 4)
     assert s.cursor[1] == 20
     s.close()
+
+
+def test_the_longest_request(gpu):
+    """2^31 - 1 rows, all but a few pages of them evicted: the table's last column
+    is shared out and given back as any other."""
+    ps, width, pages, most = 256, 1 << 23, 8, (1 << 31) - 1
+    p = Paged(pages, ps, 2, 4, nkvh=1, rope=False)
+    pool = p.pool.tensor()
+    pool.copy_(randn(1, *pool.shape))
+    fork = Q.PagedFork(p.ctx, p.pool, 2, width)
+    table = torch.full((2, width), -1, dtype=torch.int32, device="cuda")
+    table[0, 0], table[0, width - 1] = 3, 5
+    lens, shared = i32([most, 0]), p.pool.share_counts()
+    ring, cursor = i32([0, 1, 2, 4, 6, 7, -1, -1]), i32([0, 6])
+    call = lambda *parent: Q.paged_fork(p.ctx, fork, lens, i32(parent), table, shared, ring, cursor)  # noqa: E731
+    call(0, 0)
+    assert fork.status.tolist() == [0, 0] and lens.tolist() == [most, most]
+    assert table[:, 0].tolist() == [3, 3] and table[:, width - 1].tolist() == [5, 0]
+    assert int((table != -1).sum()) == 4
+    assert shared.tolist() == [0, 0, 0, 1, 0, 0, 0, 0] and cursor.tolist() == [1, 5]
+    assert torch.equal(pool[:, 0, :, :, :255], pool[:, 5, :, :, :255])
+    call(0, -1)
+    assert lens.tolist() == [most, 0] and shared.tolist() == [0] * 8
+    assert cursor.tolist() == [1, 6] and ring[6].item() == 0
+    call(-1, -1)
+    assert lens.tolist() == [0, 0] and cursor.tolist() == [1, 8]
+    assert ring.tolist() == [5, 1, 2, 4, 6, 7, 0, 3]
+    torch.cuda.synchronize()
+    fork.close()
+    p.close()
