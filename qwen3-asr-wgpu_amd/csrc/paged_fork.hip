@@ -275,7 +275,7 @@ __device__ __forceinline__ void rewrite_columns(const ForkArgs& a, int block, in
             a.ring[wrap(head + free + pushed + x, a.pages)] = __hip_atomic_load(
                 a.gone + (int64_t)(b0 + b) * a.nreq * C + at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
-        pushed += all;
+        pushed = min(pushed + all, a.pages);  // (that many are not stored any more; a sum of all passes 2^31 some time)
     }
     if (tid == 0) {
         a.cursor[0] = wrap(head + copies, a.pages);

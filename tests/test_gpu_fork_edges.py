@@ -73,3 +73,24 @@ def test_the_longest_request(gpu):
     torch.cuda.synchronize()
     fork.close()
     p.close()
+
+
+def test_pages_that_come_back_too_often_do_not_overfill_the_ring(gpu):
+    """Counts below the truth: each of many holders gives the same pages back."""
+    n, width, pages = 64, 300, 40
+    p = Paged(pages, 16, n, n, nkvh=1, rope=False)
+    fork = Q.PagedFork(p.ctx, p.pool, n, width)
+    table = torch.arange(width, device="cuda").remainder(pages).int().repeat(n, 1)
+    around = torch.full((3 * pages,), 77, dtype=torch.int32, device="cuda")
+    ring = around[pages:2 * pages]
+    for free in (0, 7, pages):
+        around.fill_(77)
+        lens, cursor = i32([16 * width] * n), i32([5, free])
+        Q.paged_fork(p.ctx, fork, lens, i32([-1] * n), table.clone(), p.pool.share_counts(), ring, cursor)
+        assert fork.status.tolist() == [0] * n and not bool(lens.any())
+        assert cursor.tolist() == [5, pages]
+        assert bool((around[:pages] == 77).all()) and bool((around[2 * pages:] == 77).all())
+        got = ring.roll(-5).tolist()
+        assert got[:free] == [77] * free and all(0 <= x < pages for x in got[free:])
+    fork.close()
+    p.close()
