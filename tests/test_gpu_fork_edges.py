@@ -45,6 +45,23 @@ def test_a_cursor_that_is_none_takes_no_pages_back(gpu, cursor):
     s.close()
 
 
+def test_an_empty_ring(gpu):
+    """Parents without rows or with whole pages alone want no copy, others do."""
+    s = State(4, 20, 16, 4)
+    s.cursor = [7, 0]
+    status, _ = s.step([0, 0, 0, 0])
+    assert status == [0] * 4
+    s.cursor = [0, 20]
+    s.grow(0, 32)
+    s.grow(1, 5)
+    s.new_pages(s.cursor[1])
+    status, copies = s.step([0, 1, 0, 0])
+    assert status == [0] * 4 and not copies
+    status, _ = s.step([0, 1, 1, 0])
+    assert status == [0, 0, B.ENOMEM, 0]
+    s.close()
+
+
 def test_the_longest_request(gpu):
     """2^31 - 1 rows, all but a few pages of them evicted: the table's last column
     is shared out and given back as any other."""
