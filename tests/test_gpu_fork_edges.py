@@ -111,3 +111,103 @@ def test_pages_that_come_back_too_often_do_not_overfill_the_ring(gpu):
         assert got[:free] == [77] * free and all(0 <= x < pages for x in got[free:])
     fork.close()
     p.close()
+
+
+@pytest.mark.parametrize("f8", [False, True])
+@pytest.mark.parametrize("ps", [16, 32])
+def test_each_beam_keeps_its_history(gpu, ps, f8):
+    """Steps of selection, fork, plan, stage (a) and attention, beside a pool in
+    which every beam has pages of its own, copied whole from its parent's by
+    torch: the same lengths, the same K and V at every position, the same bits of
+    outputs.  And V is the raw V that was appended for it."""
+    width, groups, vocab, layers, cols, steps = 3, 2, 500, 2, 6, 24
+    n = width * groups
+    make = Paged8 if f8 else Paged
+    p, own = make(60, ps, n, 100, layers=layers), make(n * cols, ps, n, 100, layers=layers)
+    sel, fork = Q.BeamSelect(p.ctx, groups, width, vocab), Q.PagedFork(p.ctx, p.pool, n, cols)
+    ring, cur = p.pool.free_ring()
+    shared, table = p.pool.share_counts(), torch.full((n, cols), -1, dtype=torch.int32, device="cuda")
+    own_table = torch.arange(n * cols, dtype=torch.int32, device="cuda").view(n, cols)
+    plan = p.plan
+    plan.cursor.copy_(cur)
+    plan.lens.zero_()
+    gains = randn(4, layers, 2, HD, std=0.1) + 1
+    scores = torch.full((n,), -float("inf"), device="cuda")
+    scores[::width] = 0.0
+    done, parent, token = (torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(3))
+    values = [torch.zeros((layers, 0, NKVH, HD), dtype=torch.float16, device="cuda")] * n  # raw V
+
+    def held(pool, ids, c):
+        """[layers][2][kvh][c][hd] of a request's pages."""
+        x = pool[:, ids[:-(-c // ps)].long()]
+        return x.permute(0, 2, 3, 1, 4, 5).flatten(3, 4)[:, :, :, :c]
+
+    def step(rows, seed):
+        total = sum(rows)
+        qkv = randn(seed, layers, total, TOT) * 2.0 ** (seed % 5 - 2)
+        before = [v.shape[1] for v in values]
+        Q.paged_plan(p.ctx, plan, plan.lens, i32(rows), table, ring, plan.cursor)
+        Q.paged_plan(own.ctx, own.plan, i32(before), i32(rows), own_table)
+        assert plan.status.tolist() == own.plan.status.tolist() == [0] * n
+        outs = []
+        for x, t in ((p, table), (own, own_table)):
+            q, out = (torch.zeros((layers, total, QDIM), dtype=torch.float16, device="cuda") for _ in range(2))
+            for l in range(layers):
+                Q.paged_append(x.ctx, x.plan, l, qkv[l], gains[l, 0], gains[l, 1], q[l])
+                Q.paged_attn(x.ctx, x.plan, l, t, q[l], out[l])
+            outs.append((q, out))
+        assert torch.equal(outs[0][0], outs[1][0]) and same_bits(outs[0][1], outs[1][1])
+        at = 0
+        for i, r in enumerate(rows):
+            v = qkv[:, at:at + r, -NKVH * HD:].view(layers, r, NKVH, HD)
+            values[i] = torch.cat([values[i], v], 1)
+            at += r
+
+    def compare():
+        assert plan.lens[:n].tolist() == [v.shape[1] for v in values]
+        for i, v in enumerate(values):
+            c = v.shape[1]
+            got = held(bits(p.pool.tensor()), table[i], c)
+            assert torch.equal(got, held(bits(own.pool.tensor()), own_table[i], c))
+            if f8:
+                unit = p.pool.scales().float().repeat_interleave(16, -1)[..., None]
+                unit = held(unit, table[i], c)[:, 1].transpose(1, 2)
+                x = held(p.pool.tensor().float(), table[i], c)[:, 1].transpose(1, 2) * unit
+                # Half a step of the value (e4m3: 2^-4 of it, or 2^-10 units); a
+                # unit that grew rounded once more, values below 2^-6 units.
+                bound = v.float().abs() * 2.0 ** -4 + unit * 2.0 ** -9
+                assert bool(((x - v.float()).abs() <= bound).all())
+            else:
+                assert torch.equal(held(p.pool.tensor(), table[i], c)[:, 1].transpose(1, 2), v)
+
+    step([30, 0, 0, 21, 0, 0], 100)
+    shuffled = 0
+    for k in range(steps):
+        say(f"beams ps={ps} f8={f8} step {k}")
+        g = torch.Generator(device="cuda")
+        g.manual_seed(k)
+        logits = torch.randn((n, vocab), device="cuda", generator=g) * 3
+        Q.beam_select(p.ctx, sel, logits, scores, parent, token, scores, done, 7, done)
+        Q.paged_fork(p.ctx, fork, plan.lens, parent, table, shared, ring, plan.cursor)
+        assert fork.status.tolist() == [0] * n
+        par = parent.tolist()
+        shuffled += par != list(range(n))
+        pool = bits(own.pool.tensor())
+        pool.copy_(pool.view(layers, n, cols, *pool.shape[2:])[:, par].reshape(pool.shape))
+        if f8:
+            units = bits(own.pool.scales())
+            units.copy_(units.view(layers, n, cols, *units.shape[2:])[:, par].reshape(units.shape))
+        values[:] = [values[j] for j in par]
+        compare()
+        rows = [1 - d for d in done.tolist()]
+        if not any(rows):
+            break
+        step(rows, 200 + k)
+        compare()
+    assert shuffled > steps // 2
+    Q.paged_fork(p.ctx, fork, plan.lens, i32([-1] * n), table, shared, ring, plan.cursor)
+    assert int(plan.cursor[1]) == 60 and not bool(shared.any())
+    fork.close()
+    sel.close()
+    own.close()
+    p.close()
