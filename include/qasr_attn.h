@@ -430,7 +430,9 @@ void qasr_beam_destroy(qasr_beam* beam);
  * log(sum over u of exp(logits[r][u])), logits row r at logits_dev +
  * r*logits_stride (floats; rows need not be aligned).  A beam that has ended
  * (done_dev[r] not 0; done_dev may be NULL) has one candidate, (r, eos) with
- * scores_dev[r], also where eos is -1.  Equal scores go to the lower beam, then to the lower token.
+ * scores_dev[r], also where eos is -1.  Of a beam's candidates the larger logit
+ * comes first, of equal logits (0 and -0 are) the lower token; of two beams' the larger score
+ * in f64, of equal scores the lower beam.
  * Place i of group g in the outputs, all [groups][k]: parent_dev the row r,
  * token_dev t, out_scores_dev the score, out_done_dev (or NULL) 1 if the beam has
  * ended or t is eos (-1: no token ends a beam), else 0.

@@ -2,8 +2,9 @@
 // beam's logits, selection over beams and vocabulary.
 //
 // Candidate (b, t) of a group has the score s_b + x_bt - log sum_u exp x_bu; an
-// ended beam has one, (b, eos) with s_b.  The k best of a group, ties to the
-// lower beam, then to the lower token.
+// ended beam has one, (b, eos) with s_b.  The k best of a group: within a beam by
+// logit, then the lower token, between beams by score in 64 bits, then the lower
+// beam.  (Logits that differ may have equal scores: 0 and 1e-20.)
 //
 // One pass over the logits.  A wave holds a tile of 2048 of a row's in registers:
 // their maximum, the sum of exponentials against it (published, a pair a tile),
