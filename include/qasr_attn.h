@@ -443,11 +443,16 @@ void qasr_beam_destroy(qasr_beam* beam);
  * parent and token -1, score -inf, done 0.  Rows that have no logits to offer
  * are not read.
  *
- * Sums are formed in f32 over pieces of 2048 tokens, everything behind them in
- * f64; scores are compared in f64 and rounded once (a difference of logits that no
- * f32 holds becomes -inf).  A group's results are a function of its own rows.  Outputs may be the inputs' arrays (out_scores
- * scores, out_done done) if k is width; they overlap nothing else.  Does not
- * allocate or synchronise, may be captured; calls that share the workspace are
+ * Exponentials are f32, summed in f32 over pieces of 2048 tokens and weighed in
+ * f32 by each piece's largest logit; the pieces are added and the logarithm is
+ * taken in f64.  A beam's scores are off by one amount together, at most (27 + 3 d) *
+ * 2^-24, d the mean distance of the row's logits from its largest, weighted by their
+ * probabilities.  So a beam's own candidates are always in order, those of
+ * different beams unless their scores are nearer than that.  Scores are compared in
+ * f64 and rounded once (a difference of logits that no f32 holds becomes -inf).  A
+ * group's results are a function of its own rows.  Outputs may be the inputs' arrays
+ * (out_scores scores, out_done done) if k is width; they overlap nothing else.  Does
+ * not allocate or synchronise, may be captured; calls that share the workspace are
  * ordered on one stream. */
 int qasr_beam_select(qasr_ctx* ctx, qasr_beam* beam, int groups, const float* logits_dev,
                      int64_t logits_stride, const float* scores_dev, const int32_t* done_dev, int eos,

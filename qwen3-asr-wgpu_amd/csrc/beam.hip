@@ -18,11 +18,11 @@
 // row has, which follows the number of rows: waves get one tile more at a time
 // once there are more than 16 a CU.
 //
-// The last workgroup of a group to arrive (ticket) merges: a wave a beam adds up
-// the tiles' sums, in order and in 64 bits, and takes the k best of the waves'
-// lists in the same way as of a tile; then each of the beams' candidates counts
-// those that come before it, in 64-bit scores.  Results are a function of the
-// group's rows alone.
+// The last workgroup of a group to arrive (ticket) merges: a wave a beam weighs the
+// tiles' sums by f32 exponentials of their largest logits, adds them in order and in
+// 64 bits, and takes the k best of the waves' lists in the same way as of a tile;
+// then each of the beams' candidates counts those that come before it, in 64-bit
+// scores.  Results are a function of the group's rows alone.
 //
 // What bounds it, us a call of 151936 tokens (bytes at the 5.1 TB/s of a large
 // copy in brackets): 1 x 5 beams 9.8 (0.6) and 16 x 5 with 10 candidates 18.9
