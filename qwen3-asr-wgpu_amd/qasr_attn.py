@@ -523,14 +523,20 @@ class PagePool:
 
     def __init__(self, ctx: Context, pages: int, page_rows: int = 16, fmt: str = "f16"):
         self.ctx = ctx
-        self.handle = None
+        self._handle = None
         if fmt not in ("f16", "e4m3"):
             raise QasrError(QASR_EINVAL, f'fmt must be "f16" or "e4m3", got {fmt!r}')
         h = _vp()
         create = load().qasr_pages_create if fmt == "f16" else load().qasr_pages_create_e4m3
         _check(create(ctx.handle, pages, page_rows, ctypes.byref(h)))
-        self.handle = h
+        self._handle = h
         self.pages, self.page_rows, self.fmt = pages, page_rows, fmt
+
+    @property
+    def handle(self):
+        """None once the pool or its context is closed: calls on it and on its plans
+        and forks are refused, also with a new context in the closed one's place."""
+        return self._handle if self.ctx.handle else None
 
     def info(self) -> PagesInfo:
         if not self.ctx.handle:
@@ -582,9 +588,9 @@ class PagePool:
     def close(self):
         """Free the pages now; their views must not be used any more, calls of
         the pool's plans are refused."""
-        if self.handle:
-            load().qasr_pages_destroy(self.handle)
-            self.handle = None
+        if self._handle:
+            load().qasr_pages_destroy(self._handle)
+            self._handle = None
 
     def __del__(self):
         try:
@@ -647,7 +653,8 @@ class PagedPlan:
 
     @property
     def handle(self):
-        """None once the plan or its pool is closed: calls on it are refused."""
+        """None once the plan, its pool or its context is closed: calls on it are
+        refused."""
         return self._mem.handle if self.pool.handle else None
 
     def close(self):
@@ -790,7 +797,8 @@ class PagedFork:
 
     @property
     def handle(self):
-        """None once the fork or its pool is closed: calls on it are refused."""
+        """None once the fork, its pool or its context is closed: calls on it are
+        refused."""
         return self._mem.handle if self.pool.handle else None
 
     def close(self):
@@ -827,17 +835,23 @@ class BeamSelect:
 
     def __init__(self, ctx: Context, max_groups: int, width: int, vocab: int, k: Optional[int] = None):
         self.ctx = ctx
-        self.handle = None
+        self._handle = None
         self.max_groups, self.width, self.vocab = max_groups, width, vocab
         self.k = width if k is None else k
         h = _vp()
         _check(load().qasr_beam_create(ctx.handle, max_groups, width, vocab, self.k, ctypes.byref(h)))
-        self.handle = h
+        self._handle = h
+
+    @property
+    def handle(self):
+        """None once the selection or its context is closed: calls on it are
+        refused."""
+        return self._handle if self.ctx.handle else None
 
     def close(self):
-        if self.handle:
-            load().qasr_beam_destroy(self.handle)
-            self.handle = None
+        if self._handle:
+            load().qasr_beam_destroy(self._handle)
+            self._handle = None
 
     def __del__(self):
         try:
