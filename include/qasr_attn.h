@@ -246,15 +246,15 @@ int qasr_pages_get_info(const qasr_pages* pool, qasr_pages_info* out);
  * the same place times the power of two that its block, 16 rows of a head of a
  * page, has: 2^(scale byte - 127) (e8m0), byte layer*layer_stride +
  * page*page_stride + kv*kv_stride + head*head_stride + row/block_rows at
- * base_dev.  Zeroed, the scales 2^0.  Half the memory of an f16 pool and an
- * eighth of a per cent.  All paged calls take such a pool:
+ * base_dev.  Zeroed, the scales 2^0.  Half the memory of an f16 pool, and 1/4096
+ * of it for the scales.  All paged calls take such a pool:
  *  - qasr_paged_append rounds K and V, once they are f16 as in an f16 pool, to
  *    the nearest e4m3 number (ties to even) in units of the smallest power of two
- *    from 2^-15 on of which the block's largest finite value is at most 448; with a
- *    unit of 2^8 magnitudes end at 240.  Rows that a block holds already keep
- *    their values if they fit; where a new row needs a larger unit they are
- *    rounded to it (exact but for values below 2^-6 of the unit).  Infinities and
- *    NaN become NaN.
+ *    from 2^-15 on of which the largest finite new value of the block is at most 448,
+ *    or in the block's unit if that is larger and the block holds earlier rows; with a
+ *    unit of 2^8 magnitudes end at 240.  Earlier rows keep their values unless the
+ *    unit grows: then they are rounded to it (exact but for values below 2^-6 of
+ *    it).  Infinities and NaN become NaN.
  *  - qasr_paged_attn gives the bits that it gives over an f16 pool of the values
  *    that the bytes stand for.  Each of these is an f16 number, as scales lie in
  *    2^-15 .. 2^8; with others, stored by the caller, a value is rounded to f16.
@@ -415,9 +415,11 @@ int qasr_paged_fork(qasr_ctx* ctx, qasr_paged_fork_ws* fork, int nreq, int32_t* 
                     int32_t* shared_dev, int32_t* ring_dev, int32_t* cursor_dev, void* stream);
 
 /* ---- Beam selection -------------------------------------------------------
- * The reference decodes greedily: no counterpart in it.  Takes the logits that
- * qasr_decoder_step writes (a row for each beam); what it selects is what
- * qasr_paged_fork takes. */
+ * The reference decodes greedily: no counterpart in it.  Takes rows of f32 logits,
+ * one for each beam, as qasr_decoder_step writes them; what it selects is what
+ * qasr_paged_fork takes.  That forks a paged cache, which belongs to a caller's own
+ * layers over qasr_paged_append and qasr_paged_attn: the text decoder below keeps
+ * its cache in slots, which no call reorders. */
 typedef struct qasr_beam qasr_beam;
 
 /* A workspace for up to max_groups (1 .. 1024) groups of `width` (1 .. 32) beams

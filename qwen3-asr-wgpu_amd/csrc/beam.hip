@@ -25,10 +25,10 @@
 // scores.  Results are a function of the group's rows alone.
 //
 // What bounds it, us a call of 151936 tokens (bytes at the 5.1 TB/s of a large
-// copy in brackets): 1 x 5 beams 9.8 (0.6) and 16 x 5 with 10 candidates 18.9
-// (9.5): a chain of launch 1.5, a tile 2.5-3 (loads 0.5, maximum and sum 0.6, border
+// copy in brackets): 1 x 5 beams 9.8-10.0 (0.6) and 16 x 5 with 10 candidates
+// 18.9-19.2 (9.5): a chain of launch 1.5, a tile 2.5-3 (loads 0.5, maximum and sum 0.6, border
 // 0.4, list 1), stores and ticket 2, the merge 4-5 (two trips to memory, list, ranks),
-// and behind it, for 16 x 5, the loads; 64 x 4 with 40 ended 30.0-30.6 (25.7): the loads, 4.4 TB/s.
+// and behind it, for 16 x 5, the loads; 64 x 4 with 40 ended 30.0-30.6 (25.7): the loads, 4.3 TB/s.
 // Measured against this: workgroups of 4 waves 12.5 / 23.0 / 31.7; keys ranked one
 // after the other by readlane 10.6 / 21.1 / 30.5; the next tile's loads ahead of a
 // tile (4 waves a SIMD instead of 6) 10.0 / 21.0 / 32.1; loads past the caches 9.8 /

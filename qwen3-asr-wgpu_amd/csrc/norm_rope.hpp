@@ -56,8 +56,8 @@ __device__ __forceinline__ float head_inv_rms(const f16* raw, float eps) {
     return 1.0f / sqrtf(sum2 / (float)kHeadDim + eps);
 }
 
-// The same in 32 registers less than half as many: a quarter of the head is read
-// while the one before is added.
+// The same with half the head in registers at a time: a quarter of it (16
+// registers) is read while the one before is added.
 __device__ __forceinline__ float head_inv_rms_lean(const f16* raw, float eps) {
 #pragma clang fp contract(off)
     constexpr int kPart = 4;

@@ -110,7 +110,8 @@ struct Item {
 // places as from f16 pages: the outputs have the same bits as over f16 pages
 // that hold these numbers.
 // us a layer, e4m3 (f16): 1 row of 512 keys 8.6 (8.1), of 8192 12.9 (14.1), 16 rows
-// of 400-2400 15.9 (23.6), a prompt of 420 10.1 (9.8), 512 rows at 7680 53 (53.5).
+// of 400-2400 15.9 (23.6), a prompt of 420 10.1-10.3 (9.8), 512 rows at 7680 53 (53.5),
+// 24 single rows with 4 chunks of 100-450 rows 38.6 (44.3).
 // Half the bytes where bytes count; else the chain of a tile is that of f16 with
 // the conversions in it, 64 a slice of 32 keys, each about 2.4 clocks of its SIMD.
 // Against 16.1 for the 16 rows and 8.9 for 1, before units were asked for ahead of

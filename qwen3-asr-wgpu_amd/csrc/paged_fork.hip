@@ -21,12 +21,14 @@
 // request that listed them, before the last workgroup to arrive moves them to
 // the ring.
 //
-// What bounds it, us a call: 1 x 5 beams of 523 rows on pages of 16 (28 layers) 10.7,
-// which is the call's own time on the host, with two launches; on the GPU the rows
-// take 4.0 and the pages 7.5, dependent trips to memory (row and table, count, ticket,
-// pages given back, ring).  16 x 5 of 400-1500 rows 12.8 (19 MB).  16 columns a
-// workgroup, each request's facts read again at each use: 24.9; 4 columns 15.9.
-// Where copies are large they are all: 1.0 GB in 175, 5.8 TB/s.
+// What bounds it, us a call: two launches, the second behind the first, and in each
+// dependent trips to memory (row and table; count, ticket, pages given back, ring).
+// 1 x 5 beams of 523 rows on pages of 16 (28 layers): 3.7 and 7.2 in a profile,
+// 9.4-10.1 a call in a replayed graph, 10.7-11.2 eagerly, where the host takes as
+// long.  16 x 5 of 400-1500 rows 12.2-12.8 either way (18 MB read and written).  16
+// columns a workgroup, each request's facts read again at each use: 24.9; 4 columns
+// 15.9.  Where copies are large they are all: 851 MB in 172-175, 4.9 TB/s (a large copy
+// reaches 5.1).
 #include "paged_fork.hpp"
 
 namespace qasr {
@@ -123,8 +125,8 @@ __global__ __launch_bounds__(kPagedMaxRequests) void fork_rows_kernel(ForkArgs a
 }
 
 // Rows of K and V, 16 bytes a thread: unit (copy, part of 1024 of them).  Past the
-// caches, as nothing here reads them again: 1.0 GB of 16 x 5 beams on pages of 256
-// rows 283 -> 175 us (5.8 TB/s), 104 MB on pages of 64 36 -> 26.
+// caches, as nothing here reads them again: 16 x 5 beams on f16 pages of 256 rows
+// (851 MB read and written) 283 -> 175 us, on e4m3 pages of 64 (88 MB) 36 -> 25.
 constexpr int kCopyVectors = 1024;
 typedef unsigned int Vector __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void copy_pages(const ForkArgs& a, int first, int step, int parts) {
