@@ -211,3 +211,65 @@ def test_each_beam_keeps_its_history(gpu, ps, f8):
     sel.close()
     own.close()
     p.close()
+
+
+def test_two_at_once_and_two_graphs_of_one_workspace(gpu):
+    """Forks on two streams, each with its own workspace and pool; then two graphs
+    of one workspace, of different requests, replayed in turn."""
+    def model(s, parent):
+        return B.fork(s.lens, parent, s.table, s.shared, s.ring, s.cursor, s.pages, s.ps)[1]
+
+    def same(s, d):
+        for got, want in zip(d, (s.lens, s.table, s.shared, s.ring, s.cursor)):
+            assert got.tolist() == want
+
+    states = [State(12, 300, 16, 20, True, 3, 2, seed=1), State(5, 90, 64, 9, False, 2, 8, seed=2)]
+    streams, held, pages = (torch.cuda.Stream(), torch.cuda.Stream()), [], []
+    for s in states:
+        for i in range(s.n):
+            s.grow(i, 37 + 11 * i)
+        held.append([i32(x) for x in (s.lens, s.table, s.shared, s.ring, s.cursor)])
+        pages.append(bits(s.p.pool.tensor()).clone())
+    parents = [[[(7 * k + 3 * i) % s.n for i in range(s.n)] for k in range(4)] for s in states]
+    dev = [[i32(p) for p in x] for x in parents]
+    torch.cuda.synchronize()
+    for k in range(4):
+        for s, d, p, stream in zip(states, held, dev, streams):
+            Q.paged_fork(s.p.ctx, s.fork, d[0], p[k], *d[1:], stream=stream.cuda_stream)
+    torch.cuda.synchronize()
+    for s, d, p, want in zip(states, held, parents, pages):
+        for x in p:
+            for a, b, r in model(s, x):
+                want[:, b, :, :, :r] = want[:, a, :, :, :r]
+        same(s, d)
+        assert torch.equal(bits(s.p.pool.tensor()), want)
+
+    # Requests 0 .. 4 and all 12 of one pool: rows of one table.
+    s, d = states[0], held[0]
+    parent = [i32([0] * 5), i32(list(range(12)))]
+    graphs = []
+    for p in parent:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            Q.paged_fork(s.p.ctx, s.fork, d[0], p, *d[1:])
+        graphs.append(g)
+    for k in range(6):
+        g, p = graphs[k % 2], parent[k % 2]
+        n = p.numel()
+        x = [(5 * k + i * (k + 1)) % n for i in range(n)]
+        p.copy_(i32(x))
+        g.replay()
+        torch.cuda.synchronize()
+        assert s.fork.status[:n].tolist() == [0] * n
+        # (The requests that are not in the call hold what they held.)
+        lens, table = s.lens[:n], s.table[:n]
+        B.fork(lens, x, table, s.shared, s.ring, s.cursor, s.pages, s.ps)
+        s.lens[:n], s.table[:n] = lens, table
+        same(s, d)
+        for i in range(s.n):
+            s.grow(i, k)
+        for t, v in zip(d, (s.lens, s.table, s.shared, s.ring, s.cursor)):
+            t.copy_(i32(v))
+    del g, graphs
+    for s in states:
+        s.close()
